@@ -367,6 +367,168 @@ int pkv_paged_attention_noalloc(void* out, const void* query, const void* key_ca
                                 float k_scale, float v_scale, void* stream);
 
 /*
+ * Tables of one step, built on the device from request lengths.  No
+ * counterpart in the reference, whose pool hands out token slots on the host.
+ *
+ * request_blocks: [num_requests, max_blocks], the block ids of every open
+ *                 request in context order (updated in place).
+ * rows          : [num_seqs], each sequence's row of request_blocks.  Rows of a
+ *                 call differ (of a row listed twice the ids stored are
+ *                 unspecified); a row outside [0, num_requests) is a sequence
+ *                 without tokens (padding).
+ * context_lens  : [num_seqs], tokens of each sequence with its new ones (what
+ *                 pkv_paged_attention takes); a context beyond max_blocks *
+ *                 block_size makes the sequence one without tokens.
+ * query_lens    : [num_seqs], new tokens of each sequence, taken as at least 0
+ *                 and at most the context.
+ * new_blocks    : [num_new_blocks], free blocks; sequences take from its start,
+ *                 in order, what their contexts need beyond the blocks that
+ *                 the tokens before the new ones fill: ceil(context /
+ *                 block_size) - ceil((context - new) / block_size) each.  A
+ *                 block that is missing becomes -1, and so do its tokens' slots.
+ * block_tables  : [num_seqs, max_blocks] out, -1 past each sequence's blocks.
+ * slot_mapping, positions: [num_tokens] out, the new tokens of all sequences
+ *                 end to end; past the last one slot -1 and position 0.  Tokens
+ *                 beyond num_tokens are not listed.
+ * query_start_loc: [num_seqs + 1] out, each sequence's first token, and the
+ *                 number of tokens.
+ * One launch; num_seqs is at most PKV_MAX_STEP_SEQS.
+ */
+#define PKV_MAX_STEP_SEQS 4096
+int pkv_build_step_tables(int32_t* request_blocks, const int32_t* rows,
+                          const int32_t* context_lens,
+                          const int32_t* query_lens, const int32_t* new_blocks,
+                          int32_t* block_tables, int32_t* slot_mapping,
+                          int32_t* positions, int32_t* query_start_loc,
+                          int32_t num_requests, int32_t num_seqs,
+                          int32_t max_blocks, int32_t num_new_blocks,
+                          int32_t num_tokens, int32_t block_size,
+                          void* stream);
+
+/*
+ * Norm of queries and keys for each head, and their rotation by position.  No
+ * counterpart in the reference, whose models do both in MLX.
+ *   y = x / sqrt(mean(x^2) + eps) * weight  over the head_size elements of each
+ *       (token, head), where a weight is given (x itself otherwise);
+ *   pairs (a, b) of y's first rotary_dim elements become
+ *       (a cos - b sin, b cos + a sin); pair i is elements (i, i + rotary_dim /
+ *       2), or (2 i, 2 i + 1) with `interleaved`.
+ * Computed in float32, rounded once.
+ *
+ * query, key: [num_tokens, heads, head_size], row strides q_stride and
+ *             k_stride, the inner two dimensions contiguous; q_out, k_out:
+ *             contiguous, of the same type, apart from the inputs.
+ * positions : [num_tokens]; positions outside [0, num_positions) take the
+ *             nearest of its rows.
+ * cos_sin   : [num_positions, rotary_dim] float32, rotary_dim / 2 cosines, then
+ *             rotary_dim / 2 sines.
+ * q_weight, k_weight: [head_size] or NULL, of type weight_dtype (dtype or F32).
+ * head_size is a multiple of 8, at most 256; rotary_dim is even, at least 2 and
+ * at most head_size.  Buffers and rows are 16-byte aligned.
+ */
+int pkv_qk_norm_rope(void* q_out, void* k_out, const void* query,
+                     const void* key, const int32_t* positions,
+                     const float* cos_sin, const void* q_weight,
+                     const void* k_weight, int64_t num_tokens,
+                     int32_t num_heads, int32_t num_kv_heads,
+                     int32_t head_size, int32_t rotary_dim,
+                     int64_t num_positions, int64_t q_stride, int64_t k_stride,
+                     float eps, int32_t interleaved, int32_t weight_dtype,
+                     int32_t dtype, void* stream);
+
+/*
+ * pkv_qk_norm_rope with the append of the rotated keys and of the values, in
+ * one launch: the caches receive what pkv_reshape_and_cache would store for
+ * them, keys rounded once from float32 to the cache's type.  Arguments as
+ * those of the two calls (dtype is that of queries, keys and values); paged
+ * caches have blocks of 8, 16 or 32 tokens.
+ */
+int pkv_qk_norm_rope_and_cache(void* q_out, const void* query, const void* key,
+                               const void* value, const int32_t* positions,
+                               const float* cos_sin, const void* q_weight,
+                               const void* k_weight, void* key_cache,
+                               void* value_cache, const int32_t* slot_mapping,
+                               int64_t num_tokens, int32_t num_heads,
+                               int32_t num_kv_heads, int32_t head_size,
+                               int32_t rotary_dim, int64_t num_positions,
+                               int64_t q_stride, int64_t k_stride,
+                               int64_t v_stride, float eps,
+                               int32_t interleaved, int32_t weight_dtype,
+                               int32_t layout, int32_t block_size, int32_t x,
+                               int64_t num_slots, int32_t dtype,
+                               int32_t cache_dtype, float k_scale,
+                               float v_scale, void* stream);
+
+/*
+ * Workspace bytes that pkv_paged_attention_extend needs for these sizes:
+ * PKV_COUNTER_BYTES of arrival counters (as pkv_paged_attention's, with which a
+ * workspace may be shared), then the states of split rows.  0 for invalid
+ * sizes.
+ */
+size_t pkv_paged_attention_extend_workspace_size(int32_t num_tokens,
+                                                 int32_t num_seqs,
+                                                 int32_t num_heads,
+                                                 int32_t num_kv_heads,
+                                                 int32_t head_size,
+                                                 int32_t max_seq_len,
+                                                 int32_t max_query_len,
+                                                 int32_t window,
+                                                 int32_t num_sinks);
+
+/*
+ * Attention of each sequence's newest tokens over the paged cache that holds
+ * them, causal.  No counterpart in the reference (whose prefill gathers the
+ * context and calls MLX).
+ *
+ * Sequence s brings query rows [query_start_loc[s], query_start_loc[s + 1]), n
+ * of them, its context's last tokens: row i sits at position p =
+ * context_lens[s] - n + i and attends to tokens t <= p, with a window (window >
+ * 0) to those of them with t > p - window or t < num_sinks:
+ *   out = sum_t softmax_t(scale * q . k_t) v_t,
+ * GQA as in pkv_paged_attention.  A row that sees no token is zero: position
+ * below 0, every block of its tokens outside [0, num_blocks) (such tokens are
+ * masked out), context 0 or beyond max_seq_len, or more than max_query_len
+ * query rows in its sequence.  What a token that a row does not see holds,
+ * infinities and NaN included, does not reach the row.
+ *
+ * query          : [num_tokens, num_heads, head_size], row stride q_stride.
+ * out            : [num_tokens, num_heads, head_size] contiguous; rows from
+ *                  query_start_loc[num_seqs] on become zeros.
+ * query_start_loc: [num_seqs + 1], from 0, not decreasing, at most num_tokens;
+ *                  NULL: one token per sequence (num_tokens == num_seqs).
+ * max_query_len  : at least the most query rows of a sequence; with 1 the
+ *                  decode kernel runs.
+ * window, num_sinks: window 0 attends to the whole context, and num_sinks is
+ *                  then not used.
+ * The other arguments as pkv_paged_attention's with PKV_LAYOUT_PAGED5D;
+ * (q_dtype, cache_dtype): (BF16, BF16), (F16, F16), (BF16 | F16, FP8_E4M3);
+ * max_seq_len is at most 2^30.  V's base and strides are 16-byte aligned (FP8:
+ * 8-byte).
+ * Launches: with max_query_len 1 one kernel, a workgroup per (sequence, KV
+ * head, part of the length), whose last arrival merges the parts in their
+ * order; otherwise one kernel of 128-row tiles, and where those would leave the
+ * chip idle their lengths are split too and a second kernel merges.
+ */
+int pkv_paged_attention_extend(void* out, const void* query,
+                               const void* key_cache, const void* value_cache,
+                               const int32_t* block_tables,
+                               const int32_t* context_lens,
+                               const int32_t* query_start_loc,
+                               int32_t num_tokens, int32_t num_seqs,
+                               int32_t num_heads, int32_t num_kv_heads,
+                               int32_t head_size, int32_t block_size,
+                               int32_t max_num_blocks_per_seq,
+                               int32_t max_seq_len, int32_t max_query_len,
+                               int32_t window, int32_t num_sinks,
+                               int64_t num_blocks, float scale,
+                               int64_t q_stride, int64_t k_block_stride,
+                               int64_t k_head_stride, int64_t v_block_stride,
+                               int64_t v_head_stride, void* workspace,
+                               size_t workspace_bytes, int32_t q_dtype,
+                               int32_t cache_dtype, float k_scale,
+                               float v_scale, void* stream);
+
+/*
  * Whole-block copies between paged caches.  A block is block_bytes
  * contiguous bytes of a plane (a [num_blocks, ...] cache tensor), so every
  * layout and dtype is the same copy.  For each (src, dst) pair of

@@ -1,0 +1,756 @@
+// Attention of new tokens over a paged KV cache, causal, over the whole context
+// or over a sliding window and the context's first tokens.
+//
+// Sequence s brings n query tokens, the last n of its c tokens: query i sits at
+// position p = c - n + i and sees the keys t <= p, of them only those with
+// t > p - window or t < sinks where there is a window.  A query row is one
+// (token, head); the rows of the heads that share a KV head are attended
+// together, row r of a sequence being head r % group of token r / group.
+//
+// Both kernels compute S^T = K Q^T and O^T = V^T P^T, so that a query row is a
+// column of every matrix: a lane holds scores, weights and outputs of one row
+// only, the running maximum and sum of its softmax are one register each, and a
+// tile's weights leave the score product in the lanes where the second product
+// wants them.  For that the K rows of a tile are taken in an order that gives
+// each lane the weights of consecutive tokens (see the kernels), which then
+// meet V's paged layout, [D][block_size], in whole 16-byte loads.
+//
+// Weights are rounded to the queries' 16-bit type for the second product (the
+// matrix units take no other), their sum is of the float32 weights.
+#pragma once
+
+#include "pkv_fp8.h"
+#include "pkv_launch.h"
+
+namespace pkv {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// D[32x32] += A[32x16] * B[16x32]: lane l supplies A[l % 32][8 (l / 32) ..+7]
+// and B[8 (l / 32) ..+7][l % 32]; register r of lane l is
+// D[r % 4 + 8 (r / 4) + 4 (l / 32)][l % 32].
+template <class T> __device__ __forceinline__ f32x16 mma32(uint4 a, uint4 b, f32x16 c);
+template <> __device__ __forceinline__ f32x16 mma32<BF16>(uint4 a, uint4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+                                                 0);
+}
+template <> __device__ __forceinline__ f32x16 mma32<F16>(uint4 a, uint4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
+                                                0);
+}
+
+// Two weights (finite, not negative) as 16-bit elements, rounded to nearest even.
+template <class T> __device__ __forceinline__ uint32_t pack_weights(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack_weights<BF16>(float a, float b) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  bf16x2 v;
+  v[0] = (__bf16)a;
+  v[1] = (__bf16)b;
+  return __builtin_bit_cast(uint32_t, v);
+}
+template <> __device__ __forceinline__ uint32_t pack_weights<F16>(float a, float b) {
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  f16x2 v;
+  v[0] = (_Float16)a;
+  v[1] = (_Float16)b;
+  return __builtin_bit_cast(uint32_t, v);
+}
+
+// Keeps the elements of eight 16-bit ones whose bit is set.
+__device__ __forceinline__ uint4 keep8(uint4 v, uint32_t bits) {
+  auto m = [&](int i) {
+    return ((bits >> (2 * i)) & 1u ? 0xffffu : 0u) | ((bits >> (2 * i + 1)) & 1u ? 0xffff0000u : 0u);
+  };
+  return make_uint4(v.x & m(0), v.y & m(1), v.z & m(2), v.w & m(3));
+}
+
+// The eight elements of an FP8 cache as 16-bit ones.
+template <class T> __device__ __forceinline__ uint4 decode8(uint2 codes) {
+  const uint2 a = fp8x4_exact_inline<T>(codes.x), b = fp8x4_exact_inline<T>(codes.y);
+  return make_uint4(a.x, a.y, b.x, b.y);
+}
+
+constexpr float kNoScore = -__builtin_inff();
+
+// States that cross workgroups inside one launch travel by agent-scope relaxed
+// atomic accesses, each coherent at agent scope by itself (the L2 caches are per
+// XCD and not coherent with one another for ordinary accesses); a workgroup
+// counts its arrival only when its stores have completed.
+__device__ __forceinline__ void store_agent(float* p, float a, float b) {
+  const uint64_t v = (uint64_t)__float_as_uint(a) | ((uint64_t)__float_as_uint(b) << 32);
+  __hip_atomic_store(reinterpret_cast<uint64_t*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 load_agent(const float* p) {
+  const uint64_t v =
+      __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+}
+__device__ __forceinline__ void wait_agent_stores() {
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0); expcnt and lgkmcnt left at their maxima
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+}
+// Counts one arrival; true for the expected-th, which sets the counter back to
+// zero (every arrival of the launch has happened by then).
+__device__ __forceinline__ bool arrived_last(int32_t* counter, int expected) {
+  const bool last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == expected - 1;
+  if (last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return last;
+}
+
+// What a sequence brings to this call.
+struct ExtendSeq {
+  int start, count;  // query rows [start, start + count) of the batch
+  int ctx;           // 0: nothing to attend (every row is zero)
+};
+__device__ __forceinline__ ExtendSeq extend_seq(const ExtendParams& p, int s) {
+  ExtendSeq q;
+  if (p.query_start_loc != nullptr) {
+    q.start = min(max(p.query_start_loc[s], 0), p.num_tokens);
+    q.count = min(max(p.query_start_loc[s + 1], q.start), p.num_tokens) - q.start;
+  } else {
+    q.start = s;
+    q.count = 1;
+  }
+  const uint32_t c = (uint32_t)p.context_lens[s];
+  q.ctx = c > (uint32_t)p.max_seq_len || q.count > p.max_query_len ? 0 : (int)c;
+  return q;
+}
+
+// Zeroes rows [r0, r1) of the output's tokens, the heads of one KV head
+// (slice), by all threads of the workgroup.
+template <class QT, int NT>
+__device__ __forceinline__ void zero_tokens(const ExtendParams& p, int D, int64_t t0, int64_t t1, int h0, int nh) {
+  using QS = typename Elem<QT>::storage;
+  const int per = nh * D;
+  for (int64_t i = threadIdx.x; i < (t1 - t0) * per; i += NT) {
+    const int64_t t = i / per;
+    static_cast<QS*>(p.out)[((t0 + t) * p.num_heads + h0) * D + (i - t * per)] = 0;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Tiles of query rows: one workgroup per (128 rows of a sequence, KV head,
+// split), four wavefronts of 32 rows.
+//
+// A tile of 64 tokens of K and V is staged in LDS as the matrix units read it:
+// K as [D / 8][64 tokens][8], V as [token group of 8][D][8], so that the 32
+// lanes of a half read 512 consecutive bytes.  Both are gathers of 16-byte
+// pieces of the paged layout (FP8 codes become 16-bit elements on the way).
+//
+// Row rho of a 32-token score product is token 16 (rho / 4 % 2) + 4 (rho / 8) +
+// rho % 4, so that register r of half h is token 16 h + r; the tokens of K's
+// image lie in that order (the token order would put two of every eight lanes'
+// reads on the same banks).
+//
+// Tiles that every row of a wavefront sees in full take no mask; a wavefront
+// skips tiles that none of its rows sees.
+// ---------------------------------------------------------------------------
+constexpr int kExtendTile = 64;
+constexpr int kExtendThreads = 256;
+
+// The token of a tile at place i of K's image.
+__device__ __forceinline__ int k_token(int i) { return (i & 32) + 16 * ((i >> 2) & 1) + 4 * ((i >> 3) & 3) + (i & 3); }
+
+template <class QT, class CT, int D>
+__global__ __launch_bounds__(kExtendThreads) void extend_kernel(ExtendParams p) {
+  using QS = typename Elem<QT>::storage;
+  using CS = typename Elem<CT>::storage;
+  constexpr bool F8 = std::is_same<CT, FP8>::value;
+  constexpr int KSTEPS = (D + 15) / 16;  // score products per 32 tokens
+  constexpr int DT = (D + 31) / 32;      // 32-dimension tiles of the output
+  constexpr int DK = KSTEPS * 2;         // 8-dimension chunks staged
+  constexpr int DV = DT * 32;            // dimensions of V staged
+  __shared__ uint4 s_k[DK * kExtendTile];
+  __shared__ uint4 s_v[kExtendTile / 8 * DV];
+  __shared__ int s_seq[3];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  const int kvh = blockIdx.x % p.num_kv_heads;
+  const int item = blockIdx.x / p.num_kv_heads;
+  const int split = blockIdx.y;
+  const int group = p.group, h0 = kvh * group;
+
+  // The workgroup's sequence and row tile: tiles of the sequences lie end to
+  // end, a sequence's last tile (the longest) first.
+  const int items = gridDim.x / p.num_kv_heads;
+  if (wave == 0) {
+    int base = 0, found = -1, z = 0;
+    for (int s0 = 0; s0 < p.num_seqs; s0 += 64) {
+      const int s = s0 + lane;
+      int tiles = 0;
+      if (s < p.num_seqs) tiles = (extend_seq(p, s).count * group + kExtendRows - 1) / kExtendRows;
+      int sum = tiles;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int a = __shfl_up(sum, d);
+        if (lane >= d) sum += a;
+      }
+      const uint64_t past = __ballot(base + sum > item);
+      if (past) {
+        const int w = __builtin_ctzll(past);
+        found = s0 + w;
+        z = base + __shfl(sum, w) - 1 - item;  // counted from the sequence's first tile
+        break;
+      }
+      base += __shfl(sum, 63);
+    }
+    if (lane == 0) s_seq[0] = found, s_seq[1] = z, s_seq[2] = base;
+  }
+  __syncthreads();
+  const int seq = __builtin_amdgcn_readfirstlane(s_seq[0]);
+  if (seq < 0) {
+    // Past the last tile: rows behind the last sequence become zeros.
+    const int tiles = s_seq[2];
+    if (split != 0) return;
+    const int last = p.query_start_loc ? min(max(p.query_start_loc[p.num_seqs], 0), p.num_tokens) : p.num_seqs;
+    for (int64_t t = last + (item - tiles); t < p.num_tokens; t += items - tiles)
+      zero_tokens<QT, kExtendThreads>(p, D, t, t + 1, h0, group);
+    return;
+  }
+  const int z = __builtin_amdgcn_readfirstlane(s_seq[1]);
+  const ExtendSeq q = extend_seq(p, seq);
+  const int first_pos = q.ctx - q.count;  // position of the sequence's first query token
+  const int rows = q.count * group;
+  const int row0 = z * kExtendRows;
+  const int row_end = min(row0 + kExtendRows, rows);
+  // Positions of the workgroup's rows; tokens before position 0 see nothing.
+  const int pmin = first_pos + row0 / group, pmax = first_pos + (row_end - 1) / group;
+
+  // This lane's row.
+  const int row = row0 + wave * 32 + col;
+  const bool live = row < rows;
+  const int tok = live ? row / group : 0;
+  const int head = h0 + (live ? row - tok * group : 0);
+  const int64_t qrow = q.start + tok;
+  const int pos = live && q.ctx > 0 ? first_pos + tok : -1;
+  // Positions of the wavefront's rows (uniform): none where w_min > w_max.
+  const int wr0 = row0 + wave * 32, wr1 = min(wr0 + 32, rows);
+  const bool w_any = wr0 < wr1 && q.ctx > 0;
+  const int w_min = w_any ? first_pos + wr0 / group : 0, w_max = w_any ? first_pos + (wr1 - 1) / group : -1;
+
+  // The tiles to visit: those of the sinks, then those of the window.
+  const int window = p.window > 0 ? p.window : p.max_seq_len;
+  const int sinks = p.window > 0 ? p.sinks : 0;
+  int lead = 0, base_tile = 0, ntiles = 0;
+  if (q.ctx > 0 && pmax >= 0) {
+    const int lo = max(0, max(pmin, 0) - window + 1);
+    lead = (min(sinks, lo) + kExtendTile - 1) / kExtendTile;
+    base_tile = max(lo / kExtendTile, lead);
+    ntiles = lead + max(0, pmax / kExtendTile + 1 - base_tile);
+  }
+  const int per = (ntiles + p.splits - 1) / p.splits;
+  const int v0 = min(split * per, ntiles), v1 = min(v0 + per, ntiles);
+
+  uint4 qf[KSTEPS];
+  {
+    const QS* src = static_cast<const QS*>(p.q) + qrow * p.q_stride + (int64_t)head * D;
+#pragma unroll
+    for (int j = 0; j < KSTEPS; ++j) {
+      const int d = 16 * j + 8 * half;
+      qf[j] = live && d < D ? *reinterpret_cast<const uint4*>(src + d) : make_uint4(0, 0, 0, 0);
+    }
+  }
+  f32x16 o[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
+  float m = kNoScore, l = 0.f;
+
+  const int shift = p.block_shift, bs = 1 << shift;
+  const int32_t* table = p.block_tables + (int64_t)seq * p.max_blocks_per_seq;
+  const CS* kc = static_cast<const CS*>(p.k_cache) + (int64_t)kvh * p.k_head_stride;
+  const CS* vc = static_cast<const CS*>(p.v_cache) + (int64_t)kvh * p.v_head_stride;
+
+  for (int v = v0; v < v1; ++v) {
+    const int t0 = (v < lead ? v : base_tile + v - lead) * kExtendTile;
+    // The block of this lane's token, -1 past the context or outside the pool.
+    int32_t bid = -1;
+    if (t0 + lane < q.ctx) {
+      bid = table[(t0 + lane) >> shift];
+      if (bid < 0 || (int64_t)bid >= p.num_blocks) bid = -1;
+    }
+    const uint64_t ok_tokens = __ballot(bid >= 0);
+    const int kt = t0 + k_token(lane);  // the token that this lane stages of K
+    const int kb = __shfl(bid, k_token(lane));
+    __syncthreads();  // the tile before has been read
+    if constexpr (!F8) {
+      for (int c = wave; c < DK; c += 4) {
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (kb >= 0 && c * 8 < D)
+          x = *reinterpret_cast<const uint4*>(kc + kb * p.k_block_stride + c * 8 * bs + (kt & (bs - 1)) * 8);
+        s_k[c * kExtendTile + lane] = x;
+      }
+    } else {
+      for (int c = wave; c < DK / 2; c += 4) {
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (kb >= 0 && c * 16 < D)
+          x = *reinterpret_cast<const uint4*>(kc + kb * p.k_block_stride + c * 16 * bs + (kt & (bs - 1)) * 16);
+        s_k[2 * c * kExtendTile + lane] = decode8<QT>(make_uint2(x.x, x.y));
+        s_k[(2 * c + 1) * kExtendTile + lane] = decode8<QT>(make_uint2(x.z, x.w));
+      }
+    }
+    for (int u0 = wave * 64; u0 < kExtendTile / 8 * DV; u0 += kExtendThreads) {
+      const int u = u0 + lane, tg = u / DV, d = u - tg * DV;
+      const int vb = __shfl(bid, 8 * tg);
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (vb >= 0 && d < D) {
+        const CS* src = vc + vb * p.v_block_stride + d * bs + ((t0 + 8 * tg) & (bs - 1));
+        if constexpr (F8)
+          x = decode8<QT>(*reinterpret_cast<const uint2*>(src));
+        else
+          x = *reinterpret_cast<const uint4*>(src);
+      }
+      s_v[u] = x;
+    }
+    __syncthreads();
+
+    // Whether any of the wavefront's rows sees a token of the tile, and whether all see all.
+    const bool in_sinks = t0 < sinks;
+    if (w_max < t0 || !(in_sinks || t0 + kExtendTile > w_min - window + 1)) continue;
+    const bool whole = t0 + kExtendTile - 1 <= w_min && (t0 > w_max - window || t0 + kExtendTile <= sinks) &&
+                       ok_tokens == ~0ull && wr0 + 32 <= rows;
+
+    f32x16 s[2];
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[sub][r] = 0.f;
+#pragma unroll
+      for (int j = 0; j < KSTEPS; ++j)
+        s[sub] = mma32<QT>(s_k[(2 * j + half) * kExtendTile + 32 * sub + col], qf[j], s[sub]);
+    }
+    // Bit r of sees[sub]: the row sees token 32 sub + 16 half + r.
+    uint32_t sees[2] = {0xffffu, 0xffffu};
+    if (!whole) {
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub) {
+        const int a = t0 + 32 * sub + 16 * half;
+        auto below = [&](int n) { return n <= 0 ? 0u : n >= 16 ? 0xffffu : (1u << n) - 1u; };  // the first n tokens
+        uint32_t b = below(pos + 1 - a) & (~below(pos - window + 1 - a) | below(sinks - a));
+        sees[sub] = b & (uint32_t)(ok_tokens >> (32 * sub + 16 * half)) & 0xffffu;
+      }
+    }
+    float mt = m;
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[sub][r] = whole || (sees[sub] >> r & 1u) ? s[sub][r] * p.scale_log2 : kNoScore;
+        mt = fmaxf(mt, s[sub][r]);
+      }
+    mt = xchg32_max(mt);
+    // (A row that has seen nothing keeps a finite reference point: no inf - inf.)
+    const float ref = mt == kNoScore ? 0.f : mt;
+    const float alpha = __builtin_amdgcn_exp2f(m - ref);
+    m = mt;
+    l *= alpha;
+    uint32_t w[2][8];
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) {
+        const float a = __builtin_amdgcn_exp2f(s[sub][r] - ref), b = __builtin_amdgcn_exp2f(s[sub][r + 1] - ref);
+        l += a + b;
+        w[sub][r / 2] = pack_weights<QT>(a, b);
+      }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
+
+    auto v_piece = [&](int dt, int sub, int k) {  // tokens 32 sub + 16 half + 8 k ..+7 of dimension 32 dt + col
+      return s_v[(4 * sub + 2 * half + k) * DV + 32 * dt + col];
+    };
+    auto weights = [&](int sub, int k) {
+      return make_uint4(w[sub][4 * k], w[sub][4 * k + 1], w[sub][4 * k + 2], w[sub][4 * k + 3]);
+    };
+    bool clean = true;
+    if (!whole) {
+      // A token that some rows do not see must not reach them, whatever its
+      // value: a weight of 0 times inf or NaN is NaN.  The product with zeros
+      // tells whether the tile has such a value.
+      f32x16 zero;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) zero[r] = 0.f;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) zero = mma32<QT>(v_piece(dt, sub, k), make_uint4(0, 0, 0, 0), zero);
+      float sum = 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sum += zero[r];
+      clean = !__any(sum != 0.f);
+    }
+    if (clean) {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) o[dt] = mma32<QT>(v_piece(dt, sub, k), weights(sub, k), o[dt]);
+    } else {
+      // One query position at a time, with the tokens that it does not see taken
+      // out of V; the other positions' rows keep their sums.
+      for (int at = w_min; at <= w_max; ++at) {
+        uint32_t keep[2];
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub) {
+          uint32_t b = 0;
+          for (int r = 0; r < 16; ++r) {
+            const int t = t0 + 32 * sub + 16 * half + r;
+            if (t <= at && (t > at - window || t < sinks) && (ok_tokens >> (t - t0) & 1u)) b |= 1u << r;
+          }
+          keep[sub] = b;
+        }
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          f32x16 n = o[dt];
+#pragma unroll
+          for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+              n = mma32<QT>(keep8(v_piece(dt, sub, k), keep[sub] >> (8 * k)), weights(sub, k), n);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[dt][r] = pos == at ? n[r] : o[dt][r];
+        }
+      }
+    }
+  }
+
+  l = xchg32_sum(l);
+  if (!live) return;
+  if (p.splits == 1) {
+    const float inv = l > 0.f ? p.v_scale / l : l == 0.f ? 0.f : l;  // (NaN stays NaN)
+    QS* out = static_cast<QS*>(p.out) + (qrow * p.num_heads + head) * D;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int d = 32 * dt + 2 * r + 4 * half;
+        if (D % 32 != 0 && d >= D) continue;
+        uint2 x;
+        x.x = pack2(from_f32<QT>(o[dt][r] * inv), from_f32<QT>(o[dt][r + 1] * inv));
+        x.y = pack2(from_f32<QT>(o[dt][r + 2] * inv), from_f32<QT>(o[dt][r + 3] * inv));
+        *reinterpret_cast<uint2*>(out + d) = x;
+      }
+    return;
+  }
+  const int64_t at = (qrow * p.num_heads + head) * p.splits + split;
+  float* wo = p.ws_o + at * D;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int d = 32 * dt + 2 * r + 4 * half;
+      if (D % 32 != 0 && d >= D) continue;
+      *reinterpret_cast<float4*>(wo + d) = make_float4(o[dt][r], o[dt][r + 1], o[dt][r + 2], o[dt][r + 3]);
+    }
+  if (half == 0) *reinterpret_cast<float2*>(p.ws_ml + at * 2) = make_float2(m, l);
+}
+
+// The outputs of a call whose row tiles are split: one wavefront per query row.
+template <class QT, int D>
+__global__ __launch_bounds__(256) void extend_merge_kernel(ExtendParams p) {
+  using QS = typename Elem<QT>::storage;
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);  // token * heads + head
+  if (row >= (int64_t)p.num_tokens * p.num_heads) return;
+  if (p.query_start_loc != nullptr && row / p.num_heads >= max(p.query_start_loc[p.num_seqs], 0))
+    return;  // a row behind the last sequence: the tiles' kernel zeroed it
+  const float* ml = p.ws_ml + row * p.splits * 2;
+  const float* wo = p.ws_o + row * p.splits * D;
+  float m = kNoScore;
+  for (int i = 0; i < p.splits; ++i) m = fmaxf(m, ml[2 * i]);
+  const float ref = m == kNoScore ? 0.f : m;
+  float l = 0.f, o[(D + 63) / 64];
+#pragma unroll
+  for (int k = 0; k < (D + 63) / 64; ++k) o[k] = 0.f;
+  for (int i = 0; i < p.splits; ++i) {
+    const float f = __builtin_amdgcn_exp2f(ml[2 * i] - ref);
+    l += f * ml[2 * i + 1];
+#pragma unroll
+    for (int k = 0; k < (D + 63) / 64; ++k)
+      if (lane + 64 * k < D) o[k] += f * wo[(int64_t)i * D + lane + 64 * k];
+  }
+  const float inv = l > 0.f ? p.v_scale / l : l == 0.f ? 0.f : l;
+  QS* out = static_cast<QS*>(p.out) + row * D;
+#pragma unroll
+  for (int k = 0; k < (D + 63) / 64; ++k)
+    if (lane + 64 * k < D) out[lane + 64 * k] = from_f32<QT>(o[k] * inv);
+}
+
+// ---------------------------------------------------------------------------
+// One new token per sequence: one workgroup per (sequence, up to 16 heads of a
+// KV head, split), four wavefronts that take tiles of 32 tokens in turn, K and
+// V from the cache straight into the matrix units' registers.
+//
+// Row i of score product u (of two) is token 8 (i / 4) + 4 u + i % 4, so that
+// the registers of both products in lane group g are tokens 8 g ..+7.
+// ---------------------------------------------------------------------------
+constexpr int kWindowTile = 32;
+
+template <class QT, class CT, int D>
+__global__ __launch_bounds__(256) void window_decode_kernel(ExtendParams p) {
+  using QS = typename Elem<QT>::storage;
+  using CS = typename Elem<CT>::storage;
+  constexpr bool F8 = std::is_same<CT, FP8>::value;
+  constexpr int KSTEPS = F8 ? (D + 63) / 64 * 2 : (D + 31) / 32;
+  constexpr int DT = (D + 15) / 16;
+  __shared__ float s_o[4][DT * 4][64];
+  __shared__ float s_m[4][16], s_l[4][16];
+  __shared__ int s_last;
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 4, col = lane & 15;
+  const int unit = blockIdx.x % p.units;
+  const int seq = blockIdx.x / p.units;
+  const int split = blockIdx.y;
+  const int kvh = unit / p.slices;
+  const int g0 = (unit - kvh * p.slices) * 16;
+  const int nh = min(16, p.group - g0), h0 = kvh * p.group + g0;
+  if (seq == p.num_seqs) {
+    // Rows behind the last sequence become zeros.
+    const int last = min(max(p.query_start_loc[p.num_seqs], 0), p.num_tokens);
+    if (split == 0) zero_tokens<QT, 256>(p, D, last, p.num_tokens, h0, nh);
+    return;
+  }
+  const ExtendSeq q = extend_seq(p, seq);
+  if (q.count == 0) return;
+  if (q.ctx == 0) {
+    if (split == 0) zero_tokens<QT, 256>(p, D, q.start, q.start + q.count, h0, nh);
+    return;
+  }
+  const int pos = q.ctx - 1;
+  const int lo = p.window > 0 ? max(0, q.ctx - p.window) : 0;
+  const int sinks = p.window > 0 ? min(p.sinks, lo) : 0;
+  const int lead = (sinks + kWindowTile - 1) / kWindowTile;
+  const int base_tile = max(lo / kWindowTile, lead);
+  const int ntiles = lead + pos / kWindowTile + 1 - base_tile;
+  // (At least one split: a sequence of few tiles leaves the others nothing.)
+  const int per = max((ntiles + p.splits - 1) / p.splits, 1);
+  const int parts = (ntiles + per - 1) / per;
+  const int v0 = split * per, v1 = min(v0 + per, ntiles);
+  if (split >= parts) return;
+
+  uint4 qf[KSTEPS];
+  {
+    const QS* src = static_cast<const QS*>(p.q) + q.start * p.q_stride + (int64_t)(h0 + min(col, nh - 1)) * D;
+#pragma unroll
+    for (int j = 0; j < KSTEPS; ++j) {
+      const int d = F8 ? 64 * (j / 2) + 16 * g + 8 * (j & 1) : 32 * j + 8 * g;
+      qf[j] = col < nh && d < D ? *reinterpret_cast<const uint4*>(src + d) : make_uint4(0, 0, 0, 0);
+    }
+  }
+  f32x4 o[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) o[dt] = {0.f, 0.f, 0.f, 0.f};
+  float m = kNoScore, l = 0.f;
+  const int shift = p.block_shift, bs = 1 << shift;
+  const int32_t* table = p.block_tables + (int64_t)seq * p.max_blocks_per_seq;
+  const CS* kc = static_cast<const CS*>(p.k_cache) + (int64_t)kvh * p.k_head_stride;
+  const CS* vc = static_cast<const CS*>(p.v_cache) + (int64_t)kvh * p.v_head_stride;
+
+  for (int v = v0 + wave; v < v1; v += 4) {
+    const int t0 = (v < lead ? v : base_tile + v - lead) * kWindowTile;
+    auto block_of = [&](int t) {
+      if (t >= q.ctx) return -1;
+      const int b = table[t >> shift];
+      return b >= 0 && (int64_t)b < p.num_blocks ? b : -1;
+    };
+    const int tk = t0 + 8 * (col >> 2), tv = t0 + 8 * g;  // first of the eight tokens of this lane's K row, of its V pieces
+    const int kb = block_of(tk), vb = block_of(tv);
+    f32x4 s[2];
+    const int64_t krow = (int64_t)max(kb, 0) * p.k_block_stride;
+    if constexpr (F8) {
+      uint4 kf[2][KSTEPS / 2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int j = 0; j < KSTEPS / 2; ++j) {
+          const int c = 4 * j + g;
+          kf[u][j] = c * 16 < D ? *reinterpret_cast<const uint4*>(
+                                      kc + krow + c * 16 * bs + ((tk & (bs - 1)) + 4 * u + (col & 3)) * 16)
+                                : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        s[u] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < KSTEPS / 2; ++j) {
+          s[u] = Mma<QT>::k32(decode8<QT>(make_uint2(kf[u][j].x, kf[u][j].y)), qf[2 * j], s[u]);
+          s[u] = Mma<QT>::k32(decode8<QT>(make_uint2(kf[u][j].z, kf[u][j].w)), qf[2 * j + 1], s[u]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        s[u] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < KSTEPS; ++j) {
+          const int c = 4 * j + g;
+          const uint4 k = c * 8 < D ? *reinterpret_cast<const uint4*>(
+                                          kc + krow + c * 8 * bs + ((tk & (bs - 1)) + 4 * u + (col & 3)) * 8)
+                                    : make_uint4(0, 0, 0, 0);
+          s[u] = Mma<QT>::k32(k, qf[j], s[u]);
+        }
+      }
+    }
+    // Bit i: token tv + i is seen (by every row alike).
+    uint32_t sees = 0;
+    if (vb >= 0) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (tv + i < q.ctx && (tv + i >= lo || tv + i < sinks)) sees |= 1u << i;
+    }
+    float mt = m;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        s[u][r] = sees >> (4 * u + r) & 1u ? s[u][r] * p.scale_log2 : kNoScore;
+        mt = fmaxf(mt, s[u][r]);
+      }
+    mt = column_max(mt);
+    const float ref = mt == kNoScore ? 0.f : mt;
+    const float alpha = __builtin_amdgcn_exp2f(m - ref);
+    m = mt;
+    l *= alpha;
+    uint32_t w[4];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; r += 2) {
+        const float a = __builtin_amdgcn_exp2f(s[u][r] - ref), b = __builtin_amdgcn_exp2f(s[u][r + 1] - ref);
+        l += a + b;
+        w[2 * u + r / 2] = pack_weights<QT>(a, b);
+      }
+    const uint4 wf = make_uint4(w[0], w[1], w[2], w[3]);
+    const int64_t vrow = (int64_t)max(vb, 0) * p.v_block_stride + (tv & (bs - 1));
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      const int d = min(16 * dt + col, D - 1);
+      uint4 x;
+      if constexpr (F8)
+        x = decode8<QT>(*reinterpret_cast<const uint2*>(vc + vrow + d * bs));
+      else
+        x = *reinterpret_cast<const uint4*>(vc + vrow + d * bs);
+      // What a token that is not seen holds must not matter.
+      if (sees != 0xffu) x = keep8(x, sees);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[dt][r] *= alpha;
+      o[dt] = Mma<QT>::k32(x, wf, o[dt]);
+    }
+  }
+
+  // The wavefronts' states: column col is head h0 + col.
+  l = column_sum(l);
+  if (g == 0) s_m[wave][col] = m, s_l[wave][col] = l;
+  __syncthreads();
+  float M = kNoScore, L = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) M = fmaxf(M, s_m[w][col]);
+  const float ref = M == kNoScore ? 0.f : M;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) L += s_l[w][col] * __builtin_amdgcn_exp2f(s_m[w][col] - ref);
+  const float f = __builtin_amdgcn_exp2f(m - ref);
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) s_o[wave][4 * dt + r][lane] = o[dt][r] * f;
+  __syncthreads();
+  // Wavefront w sums the 16-dimension tiles w, w + 4, ...
+  const float inv = L > 0.f ? p.v_scale / L : L == 0.f ? 0.f : L;
+  const int64_t row = (int64_t)q.start * p.num_heads + h0 + col;
+#pragma unroll
+  for (int k = 0; k < (DT + 3) / 4; ++k) {
+    const int dt = 4 * k + wave;
+    const int d = 16 * dt + 4 * g;
+    if (dt >= DT || col >= nh || d >= D) continue;
+    float x[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      x[r] = s_o[0][4 * dt + r][lane] + s_o[1][4 * dt + r][lane] + s_o[2][4 * dt + r][lane] + s_o[3][4 * dt + r][lane];
+    if (parts == 1) {
+      uint2 y;
+      y.x = pack2(from_f32<QT>(x[0] * inv), from_f32<QT>(x[1] * inv));
+      y.y = pack2(from_f32<QT>(x[2] * inv), from_f32<QT>(x[3] * inv));
+      *reinterpret_cast<uint2*>(static_cast<QS*>(p.out) + row * D + d) = y;
+    } else {
+      float* to = p.ws_o + (row * p.splits + split) * D + d;
+      store_agent(to, x[0], x[1]);
+      store_agent(to + 2, x[2], x[3]);
+    }
+  }
+  if (parts == 1) return;
+  if (wave == 0 && g == 0 && col < nh) store_agent(p.ws_ml + (row * p.splits + split) * 2, M, L);
+  // The workgroup whose part is the last to arrive merges all, in their order.
+  wait_agent_stores();
+  __syncthreads();
+  if (tid == 0) s_last = arrived_last(p.counters + (int64_t)seq * p.units + unit, parts);
+  __syncthreads();
+  if (!s_last) return;
+  for (int i = tid; i < nh * (D / 2); i += 256) {
+    const int h = i / (D / 2), d = 2 * (i - h * (D / 2));
+    const int64_t r = (int64_t)q.start * p.num_heads + h0 + h;
+    float mm = kNoScore;
+    for (int s = 0; s < parts; ++s) mm = fmaxf(mm, load_agent(p.ws_ml + (r * p.splits + s) * 2).x);
+    const float rf = mm == kNoScore ? 0.f : mm;
+    float ll = 0.f, x = 0.f, y = 0.f;
+    for (int s = 0; s < parts; ++s) {
+      const float2 ml = load_agent(p.ws_ml + (r * p.splits + s) * 2);
+      const float2 v = load_agent(p.ws_o + (r * p.splits + s) * D + d);
+      const float e = __builtin_amdgcn_exp2f(ml.x - rf);
+      ll += e * ml.y;
+      x += e * v.x;
+      y += e * v.y;
+    }
+    const float iv = ll > 0.f ? p.v_scale / ll : ll == 0.f ? 0.f : ll;
+    *reinterpret_cast<uint32_t*>(static_cast<QS*>(p.out) + r * D + d) =
+        pack2(from_f32<QT>(x * iv), from_f32<QT>(y * iv));
+  }
+}
+
+template <class QT, class CT, int D>
+hipError_t launch_extend_d(const ExtendParams& p, hipStream_t stream) {
+  if (p.max_query_len == 1) {
+    const int seqs = p.num_seqs + (p.query_start_loc != nullptr ? 1 : 0);
+    hipLaunchKernelGGL((window_decode_kernel<QT, CT, D>), dim3((unsigned)(seqs * p.units), (unsigned)p.splits),
+                       dim3(256), 0, stream, p);
+    return hipGetLastError();
+  }
+  const int64_t items = extend_items(p.num_tokens, p.num_seqs, p.group);
+  hipLaunchKernelGGL((extend_kernel<QT, CT, D>), dim3((unsigned)(items * p.num_kv_heads), (unsigned)p.splits),
+                     dim3(kExtendThreads), 0, stream, p);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || p.splits == 1) return e;
+  const int64_t rows = (int64_t)p.num_tokens * p.num_heads;
+  hipLaunchKernelGGL((extend_merge_kernel<QT, D>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, p);
+  return hipGetLastError();
+}
+
+template <class QT, class CT>
+hipError_t launch_extend_typed(const ExtendParams& p, int head_size, hipStream_t stream) {
+  switch (head_size) {
+    case 32: return launch_extend_d<QT, CT, 32>(p, stream);
+    case 64: return launch_extend_d<QT, CT, 64>(p, stream);
+    case 80: return launch_extend_d<QT, CT, 80>(p, stream);
+    case 96: return launch_extend_d<QT, CT, 96>(p, stream);
+    case 112: return launch_extend_d<QT, CT, 112>(p, stream);
+    case 120:
+      if constexpr (std::is_same<CT, FP8>::value) return hipErrorInvalidValue;  // (16 does not divide it)
+      else return launch_extend_d<QT, CT, 120>(p, stream);
+    case 128: return launch_extend_d<QT, CT, 128>(p, stream);
+    case 192: return launch_extend_d<QT, CT, 192>(p, stream);
+    case 256: return launch_extend_d<QT, CT, 256>(p, stream);
+  }
+  return hipErrorInvalidValue;
+}
+
+}  // namespace pkv

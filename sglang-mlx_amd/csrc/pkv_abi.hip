@@ -114,6 +114,7 @@ int resolve_partition(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
 }  // namespace
 
 static_assert(PKV_COUNTER_BYTES == pkv::kCounterBytes, "the header's counter region is the kernels'");
+static_assert(PKV_MAX_STEP_SEQS == pkv::kMaxStepSeqs, "the header's limit is the kernel's");
 
 namespace pkv {
 DecodeWorkspace decode_workspace_layout(int32_t num_seqs, int32_t num_heads, int32_t head_size,
@@ -521,6 +522,95 @@ int paged_attention_impl(void* out, const void* query, const void* key_cache, co
   return PKV_OK;
 }
 
+
+// ---- norm and rotation ---------------------------------------------------------
+
+// The arguments that the calls with and without a cache share, checked and put
+// into p (whose k_out, q_out and cache the caller has set).
+int norm_rope_args(pkv::NormRopeParams& p, const void* query, const int32_t* positions, const float* cos_sin,
+                   const void* q_weight, const void* k_weight, int64_t num_tokens, int32_t num_heads,
+                   int32_t num_kv_heads, int32_t head_size, int32_t rotary_dim, int64_t num_positions,
+                   int64_t q_stride, float eps, int32_t interleaved, int32_t weight_dtype, int32_t dtype) {
+  if (num_tokens < 0) return fail(PKV_ERR_INVALID, "num_tokens must be non-negative");
+  if (num_heads <= 0 || num_kv_heads <= 0) return fail(PKV_ERR_INVALID, "num_heads and num_kv_heads must be positive");
+  if (head_size <= 0 || head_size % 8 != 0 || head_size > 256)
+    return fail(PKV_ERR_UNSUPPORTED, "head_size must be a multiple of 8, at most 256");
+  if (rotary_dim < 2 || rotary_dim % 2 != 0 || rotary_dim > head_size)
+    return fail(PKV_ERR_INVALID, "rotary_dim must be even, at least 2 and at most head_size");
+  if (num_positions <= 0) return fail(PKV_ERR_INVALID, "num_positions must be positive");
+  if (!valid_dtype(dtype)) return fail(PKV_ERR_INVALID, "Unsupported dtype");
+  const bool weights = q_weight != nullptr || k_weight != nullptr;
+  if (weights && weight_dtype != dtype && weight_dtype != PKV_F32)
+    return fail(PKV_ERR_UNSUPPORTED, "weights must be of the queries' type or float32");
+  if (weights && !(eps >= 0.f && std::isfinite(eps))) return fail(PKV_ERR_INVALID, "eps must be finite and non-negative");
+  if (num_tokens == 0) return PKV_OK;
+  if (!query || !p.cache.key || !p.q_out || !positions || !cos_sin) return fail(PKV_ERR_INVALID, "null buffer");
+  const int eb = elem_bytes(dtype);
+  if (q_stride < (int64_t)num_heads * head_size || p.cache.key_stride < (int64_t)num_kv_heads * head_size)
+    return fail(PKV_ERR_INVALID, "query/key row stride is smaller than a row");
+  if (!aligned16(query) || !aligned16(p.cache.key) || !aligned16(p.q_out) || !aligned16(cos_sin) ||
+      (q_stride * eb) % 16 != 0 || (p.cache.key_stride * eb) % 16 != 0 || !aligned16(q_weight) || !aligned16(k_weight))
+    return fail(PKV_ERR_INVALID, "query and key rows, q_out, cos_sin and weights must be 16-byte aligned");
+  p.query = query;
+  p.positions = positions;
+  p.cos_sin = cos_sin;
+  p.q_weight = q_weight;
+  p.k_weight = k_weight;
+  p.q_stride = q_stride;
+  p.num_positions = num_positions;
+  p.num_heads = num_heads;
+  p.rot = rotary_dim;
+  p.interleaved = interleaved != 0;
+  p.weight_f32 = weight_dtype == PKV_F32;
+  p.eps = eps;
+  p.cache.num_tokens = num_tokens;
+  p.cache.num_heads = num_kv_heads;
+  p.cache.head_size = head_size;
+  p.cache.kv_dtype = dtype;
+  return PKV_OK;
+}
+
+int norm_rope_launch(const pkv::NormRopeParams& p, void* stream) {
+  clear_pending_error();
+  const hipError_t e = pkv::launch_norm_rope(p, static_cast<hipStream_t>(stream));
+  if (e == hipErrorInvalidConfiguration)
+    return fail(PKV_ERR_UNSUPPORTED, "num_tokens * num_heads exceeds the launch grid limit");
+  if (e != hipSuccess) return hip_fail(e, "qk_norm_rope launch");
+  return PKV_OK;
+}
+
+// ---- attention of new tokens ------------------------------------------------------
+
+constexpr int32_t kExtendMaxSeq = 1 << 30;
+
+// Parts that each (sequence, KV head) of a decode, or each row tile, is split
+// into along its keys: as many as make the launch fill the chip, none shorter
+// than a few tiles.
+int64_t extend_splits(int64_t num_tokens, int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads,
+                      int64_t max_seq_len, int64_t max_query_len, int64_t window, int64_t num_sinks) {
+  const int64_t group = num_heads / num_kv_heads;
+  const int64_t span = window > 0 ? std::min(max_seq_len, window + num_sinks + max_query_len) : max_seq_len;
+  if (max_query_len == 1) {
+    const int64_t items = num_seqs * num_kv_heads * ((group + 15) / 16);
+    if (items == 0 || items * 4 > pkv::kCounterBytes) return 1;
+    return std::max<int64_t>(1, std::min(ceil_div(1024, items), ceil_div(span, 32 * 8)));
+  }
+  const int64_t items = (ceil_div(num_tokens * group, pkv::kExtendRows)) * num_kv_heads;
+  if (items == 0) return 1;
+  return std::max<int64_t>(1, std::min(512 / items, ceil_div(span, 64 * 8)));
+}
+
+struct ExtendWorkspace {
+  size_t ml_bytes, total;
+};
+ExtendWorkspace extend_workspace(int64_t num_tokens, int64_t num_heads, int64_t head_size, int64_t splits) {
+  const size_t rows = splits > 1 ? (size_t)num_tokens * num_heads * splits : 0;
+  ExtendWorkspace w;
+  w.ml_bytes = (rows * 2 * sizeof(float) + 255) & ~size_t(255);
+  w.total = (size_t)pkv::kCounterBytes + w.ml_bytes + rows * head_size * sizeof(float);
+  return w;
+}
+
 }  // namespace
 
 extern "C" {
@@ -571,6 +661,227 @@ int pkv_paged_attention_cascade(void* out, const void* query, const void* key_ca
                               num_blocks, scale, q_stride, k_block_stride, k_head_stride, v_block_stride,
                               v_head_stride, PKV_LAYOUT_PAGED5D, 0, workspace, workspace_bytes, false, q_dtype,
                               cache_dtype, k_scale, v_scale, stream, plan);
+}
+
+int pkv_build_step_tables(int32_t* request_blocks, const int32_t* rows, const int32_t* context_lens,
+                          const int32_t* query_lens, const int32_t* new_blocks, int32_t* block_tables,
+                          int32_t* slot_mapping, int32_t* positions, int32_t* query_start_loc, int32_t num_requests,
+                          int32_t num_seqs, int32_t max_blocks, int32_t num_new_blocks, int32_t num_tokens,
+                          int32_t block_size, void* stream) {
+  if (num_requests < 0 || num_seqs < 0 || num_new_blocks < 0 || num_tokens < 0)
+    return fail(PKV_ERR_INVALID, "num_requests, num_seqs, num_new_blocks and num_tokens must be non-negative");
+  if (max_blocks <= 0 || block_size <= 0)
+    return fail(PKV_ERR_INVALID, "max_blocks and block_size must be positive");
+  if (num_seqs > PKV_MAX_STEP_SEQS) return fail(PKV_ERR_UNSUPPORTED, "a step holds at most 4096 sequences");
+  if (!query_start_loc || (num_tokens > 0 && (!slot_mapping || !positions)) || (num_new_blocks > 0 && !new_blocks) ||
+      (num_seqs > 0 && (!rows || !context_lens || !query_lens || !block_tables)) ||
+      (num_requests > 0 && !request_blocks))
+    return fail(PKV_ERR_INVALID, "null buffer");
+  pkv::StepTablesParams p;
+  p.request_blocks = request_blocks;
+  p.rows = rows;
+  p.context_lens = context_lens;
+  p.query_lens = query_lens;
+  p.new_blocks = new_blocks;
+  p.block_tables = block_tables;
+  p.slot_mapping = slot_mapping;
+  p.positions = positions;
+  p.query_start_loc = query_start_loc;
+  p.num_requests = num_requests;
+  p.num_seqs = num_seqs;
+  p.max_blocks = max_blocks;
+  p.num_new_blocks = num_new_blocks;
+  p.num_tokens = num_tokens;
+  p.block_size = block_size;
+  clear_pending_error();
+  const hipError_t e = pkv::launch_step_tables(p, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "build_step_tables launch");
+  return PKV_OK;
+}
+
+int pkv_qk_norm_rope(void* q_out, void* k_out, const void* query, const void* key, const int32_t* positions,
+                     const float* cos_sin, const void* q_weight, const void* k_weight, int64_t num_tokens,
+                     int32_t num_heads, int32_t num_kv_heads, int32_t head_size, int32_t rotary_dim,
+                     int64_t num_positions, int64_t q_stride, int64_t k_stride, float eps, int32_t interleaved,
+                     int32_t weight_dtype, int32_t dtype, void* stream) {
+  pkv::NormRopeParams p = {};
+  p.q_out = q_out;
+  p.k_out = k_out;
+  p.cache.cache_dtype = dtype;
+  p.cache.key = key;
+  p.cache.key_stride = k_stride;
+  const int st = norm_rope_args(p, query, positions, cos_sin, q_weight, k_weight, num_tokens, num_heads, num_kv_heads,
+                                head_size, rotary_dim, num_positions, q_stride, eps, interleaved, weight_dtype, dtype);
+  if (st != PKV_OK || num_tokens == 0) return st;
+  if (!k_out || !aligned16(k_out)) return fail(PKV_ERR_INVALID, "k_out must be a 16-byte aligned buffer");
+  return norm_rope_launch(p, stream);
+}
+
+int pkv_qk_norm_rope_and_cache(void* q_out, const void* query, const void* key, const void* value,
+                               const int32_t* positions, const float* cos_sin, const void* q_weight,
+                               const void* k_weight, void* key_cache, void* value_cache, const int32_t* slot_mapping,
+                               int64_t num_tokens, int32_t num_heads, int32_t num_kv_heads, int32_t head_size,
+                               int32_t rotary_dim, int64_t num_positions, int64_t q_stride, int64_t k_stride,
+                               int64_t v_stride, float eps, int32_t interleaved, int32_t weight_dtype, int32_t layout,
+                               int32_t block_size, int32_t x, int64_t num_slots, int32_t dtype, int32_t cache_dtype,
+                               float k_scale, float v_scale, void* stream) {
+  const bool fp8 = cache_dtype == PKV_FP8_E4M3;
+  if (!valid_dtype(dtype) || !(valid_dtype(cache_dtype) || fp8)) return fail(PKV_ERR_INVALID, "Unsupported dtype");
+  if (!(dtype == cache_dtype || fp8 || (dtype == PKV_F32 && cache_dtype != PKV_F32)))
+    return fail(PKV_ERR_UNSUPPORTED, "Unsupported key/cache dtype pair");
+  if (fp8 && !(std::isfinite(k_scale) && std::isfinite(v_scale) && k_scale != 0.f && v_scale != 0.f))
+    return fail(PKV_ERR_INVALID, "k_scale and v_scale must be finite and nonzero for FP8 caches");
+  if (layout != PKV_LAYOUT_PAGED5D && layout != PKV_LAYOUT_TOKEN_MAJOR)
+    return fail(PKV_ERR_INVALID, "Unknown cache layout");
+  if (num_slots <= 0 || num_slots > INT32_MAX) return fail(PKV_ERR_INVALID, "num_slots must be in [1, 2^31)");
+  pkv::NormRopeParams p = {};
+  pkv::RacParams& c = p.cache;
+  p.q_out = q_out;
+  c.key = key;
+  c.value = value;
+  c.key_cache = key_cache;
+  c.value_cache = value_cache;
+  c.slot_mapping = slot_mapping;
+  c.key_stride = k_stride;
+  c.value_stride = v_stride;
+  c.num_slots = num_slots;
+  c.block_size = layout == PKV_LAYOUT_PAGED5D ? block_size : 1;
+  c.layout = layout;
+  c.cache_dtype = cache_dtype;
+  c.k_scale = k_scale;
+  c.v_scale = v_scale;
+  c.fast_div = fp8 && fast_scale(k_scale) && fast_scale(v_scale);
+  c.k_inv = c.fast_div ? 1.f / k_scale : 0.f;
+  c.v_inv = c.fast_div ? 1.f / v_scale : 0.f;
+  const int st = norm_rope_args(p, query, positions, cos_sin, q_weight, k_weight, num_tokens, num_heads, num_kv_heads,
+                                head_size, rotary_dim, num_positions, q_stride, eps, interleaved, weight_dtype, dtype);
+  if (st != PKV_OK) return st;
+  if (layout == PKV_LAYOUT_PAGED5D) {
+    if (!valid_block_size(block_size)) return fail(PKV_ERR_UNSUPPORTED, "block_size must be 8, 16 or 32");
+    if (x != 16 / elem_bytes(cache_dtype))
+      return fail(PKV_ERR_INVALID, "key_cache last dimension must be 16 / sizeof(cache element)");
+    if (head_size % x != 0) return fail(PKV_ERR_INVALID, "head_size must be a multiple of x");
+    if (num_slots % block_size != 0) return fail(PKV_ERR_INVALID, "num_slots must be a multiple of block_size");
+  }
+  if (num_tokens == 0) return PKV_OK;
+  if (!value || !key_cache || !value_cache || !slot_mapping) return fail(PKV_ERR_INVALID, "null buffer");
+  if (v_stride < (int64_t)num_kv_heads * head_size || !aligned16(value) || (v_stride * elem_bytes(dtype)) % 16 != 0 ||
+      !aligned16(key_cache) || !aligned16(value_cache))
+    return fail(PKV_ERR_INVALID, "value rows and caches must be 16-byte aligned, rows num_kv_heads * head_size long");
+  return norm_rope_launch(p, stream);
+}
+
+size_t pkv_paged_attention_extend_workspace_size(int32_t num_tokens, int32_t num_seqs, int32_t num_heads,
+                                                 int32_t num_kv_heads, int32_t head_size, int32_t max_seq_len,
+                                                 int32_t max_query_len, int32_t window, int32_t num_sinks) {
+  if (num_tokens < 0 || num_seqs < 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 ||
+      head_size <= 0 || max_seq_len <= 0 || max_seq_len > kExtendMaxSeq || max_query_len <= 0 || window < 0 ||
+      num_sinks < 0)
+    return 0;
+  const int64_t splits = extend_splits(num_tokens, num_seqs, num_heads, num_kv_heads, max_seq_len, max_query_len,
+                                       window, num_sinks);
+  return extend_workspace(num_tokens, num_heads, head_size, splits).total;
+}
+
+int pkv_paged_attention_extend(void* out, const void* query, const void* key_cache, const void* value_cache,
+                               const int32_t* block_tables, const int32_t* context_lens,
+                               const int32_t* query_start_loc, int32_t num_tokens, int32_t num_seqs, int32_t num_heads,
+                               int32_t num_kv_heads, int32_t head_size, int32_t block_size,
+                               int32_t max_num_blocks_per_seq, int32_t max_seq_len, int32_t max_query_len,
+                               int32_t window, int32_t num_sinks, int64_t num_blocks, float scale, int64_t q_stride,
+                               int64_t k_block_stride, int64_t k_head_stride, int64_t v_block_stride,
+                               int64_t v_head_stride, void* workspace, size_t workspace_bytes, int32_t q_dtype,
+                               int32_t cache_dtype, float k_scale, float v_scale, void* stream) {
+  if (num_tokens < 0 || num_seqs < 0)
+    return fail(PKV_ERR_INVALID, "num_tokens and num_seqs must be non-negative");
+  if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0)
+    return fail(PKV_ERR_INVALID, "num_heads must be divisible by num_kv_heads");
+  if (max_seq_len <= 0) return fail(PKV_ERR_INVALID, "max_seq_len must be positive");
+  if (max_seq_len > kExtendMaxSeq) return fail(PKV_ERR_UNSUPPORTED, "max_seq_len must be at most 2^30");
+  if (max_query_len <= 0) return fail(PKV_ERR_INVALID, "max_query_len must be positive");
+  if (window < 0 || num_sinks < 0) return fail(PKV_ERR_INVALID, "window and num_sinks must be non-negative");
+  if (query_start_loc == nullptr && (num_tokens != num_seqs || max_query_len != 1))
+    return fail(PKV_ERR_INVALID, "without query_start_loc a call has one token per sequence");
+  if (!valid_head_size(head_size) || !valid_block_size(block_size))
+    return fail(PKV_ERR_UNSUPPORTED, "Unsupported head_size/block_size for paged_attention");
+  if (max_num_blocks_per_seq <= 0 || (int64_t)max_seq_len > (int64_t)max_num_blocks_per_seq * block_size)
+    return fail(PKV_ERR_INVALID, "max_seq_len exceeds block table capacity");
+  const bool fp8 = cache_dtype == PKV_FP8_E4M3;
+  if (!(q_dtype == PKV_BF16 || q_dtype == PKV_F16) || !(cache_dtype == q_dtype || fp8))
+    return fail(PKV_ERR_UNSUPPORTED, "Unsupported query/cache dtype pair for paged_attention");
+  if (fp8 && head_size % 16 != 0)
+    return fail(PKV_ERR_UNSUPPORTED, "FP8 caches are read in the paged layout with head_size a multiple of 16");
+  if (fp8 && !(std::isfinite(k_scale) && std::isfinite(v_scale) && k_scale != 0.f && v_scale != 0.f))
+    return fail(PKV_ERR_INVALID, "k_scale and v_scale must be finite and nonzero for FP8 caches");
+  if (num_blocks <= 0) return fail(PKV_ERR_INVALID, "num_blocks must be positive");
+  const int64_t splits = extend_splits(num_tokens, num_seqs, num_heads, num_kv_heads, max_seq_len, max_query_len,
+                                       window, num_sinks);
+  const int32_t group = num_heads / num_kv_heads, slices = (group + 15) / 16;
+  const int64_t groups = max_query_len == 1 ? ((int64_t)num_seqs + 1) * num_kv_heads * slices
+                                            : pkv::extend_items(num_tokens, num_seqs, group) * num_kv_heads;
+  // (HIP bounds a launch to 2^32 work-items; rows of a sequence are counted in 32 bits.)
+  if (groups * splits * 256 >= ((int64_t)1 << 32) || (int64_t)num_tokens * num_heads >= ((int64_t)1 << 30))
+    return fail(PKV_ERR_UNSUPPORTED, "num_tokens * num_heads exceeds the launch grid limit");
+  if (num_tokens == 0) return PKV_OK;
+  if (!out || !query || !key_cache || !value_cache || (num_seqs > 0 && (!block_tables || !context_lens)))
+    return fail(PKV_ERR_INVALID, "null buffer");
+  if (!aligned16(out)) return fail(PKV_ERR_INVALID, "out must be 16-byte aligned");
+  if (!aligned16(query) || (q_stride * 2) % 16 != 0 || q_stride < (int64_t)num_heads * head_size)
+    return fail(PKV_ERR_INVALID, "query rows must be 16-byte aligned with stride >= num_heads * head_size");
+  const int64_t cb = elem_bytes(cache_dtype), v_align = fp8 ? 8 : 16;
+  if (!aligned16(key_cache) || (k_block_stride * cb) % 16 != 0 || (k_head_stride * cb) % 16 != 0 ||
+      (reinterpret_cast<uintptr_t>(value_cache) % v_align) != 0 || (v_block_stride * cb) % v_align != 0 ||
+      (v_head_stride * cb) % v_align != 0)
+    return fail(PKV_ERR_INVALID, "cache base or strides are not aligned for vector loads");
+  const ExtendWorkspace w = extend_workspace(num_tokens, num_heads, head_size, splits);
+  if (workspace == nullptr || workspace_bytes < w.total)
+    return fail(PKV_ERR_INVALID, "workspace is smaller than pkv_paged_attention_extend_workspace_size()");
+  if (!aligned16(workspace)) return fail(PKV_ERR_INVALID, "workspace must be 16-byte aligned");
+  char* ws = static_cast<char*>(workspace);
+  pkv::ExtendParams p;
+  p.out = out;
+  p.q = query;
+  p.k_cache = key_cache;
+  p.v_cache = value_cache;
+  p.block_tables = block_tables;
+  p.context_lens = context_lens;
+  p.query_start_loc = query_start_loc;
+  p.counters = reinterpret_cast<int32_t*>(ws);
+  p.ws_ml = reinterpret_cast<float*>(ws + pkv::kCounterBytes);
+  p.ws_o = reinterpret_cast<float*>(ws + pkv::kCounterBytes + w.ml_bytes);
+  p.num_blocks = num_blocks;
+  p.q_stride = q_stride;
+  p.k_block_stride = k_block_stride;
+  p.k_head_stride = k_head_stride;
+  p.v_block_stride = v_block_stride;
+  p.v_head_stride = v_head_stride;
+  p.scale_log2 = scale * 1.4426950408889634f * (fp8 ? k_scale : 1.f);
+  p.v_scale = fp8 ? v_scale : 1.f;
+  p.num_tokens = num_tokens;
+  p.num_seqs = num_seqs;
+  p.num_heads = num_heads;
+  p.num_kv_heads = num_kv_heads;
+  p.group = group;
+  p.slices = slices;
+  p.units = num_kv_heads * slices;
+  p.max_blocks_per_seq = max_num_blocks_per_seq;
+  p.max_seq_len = max_seq_len;
+  p.max_query_len = max_query_len;
+  p.window = std::min(window, max_seq_len);  // (a longer one sees no more)
+  p.sinks = std::min(num_sinks, max_seq_len);
+  p.block_shift = block_size == 8 ? 3 : block_size == 16 ? 4 : 5;
+  p.splits = (int32_t)splits;
+  clear_pending_error();
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  hipError_t e;
+  if (fp8)
+    e = q_dtype == PKV_BF16 ? pkv::launch_extend_typed<pkv::BF16, pkv::FP8>(p, head_size, s)
+                            : pkv::launch_extend_typed<pkv::F16, pkv::FP8>(p, head_size, s);
+  else
+    e = q_dtype == PKV_BF16 ? pkv::launch_extend_typed<pkv::BF16, pkv::BF16>(p, head_size, s)
+                            : pkv::launch_extend_typed<pkv::F16, pkv::F16>(p, head_size, s);
+  if (e != hipSuccess) return hip_fail(e, "paged_attention_extend launch");
+  return PKV_OK;
 }
 
 int pkv_max_shared_memory_per_block(int32_t device_id, int64_t* out) {

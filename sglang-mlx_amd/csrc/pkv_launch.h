@@ -5,6 +5,7 @@
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <algorithm>
 #include <atomic>
 #include <type_traits>
 
@@ -237,6 +238,79 @@ struct BlockCopyParams {
 hipError_t launch_copy_blocks(const BlockCopyParams& p, bool aligned, hipStream_t stream);
 // Most pairs one launch can take for this block size.
 int64_t copy_blocks_max_grid_pairs(int64_t block_bytes, bool aligned);
+
+// Tables of one step (step_tables.hip; the rules of pkv_build_step_tables).
+constexpr int kMaxStepSeqs = 4096;  // their prefix sums sit in LDS
+struct StepTablesParams {
+  int32_t* request_blocks;      // [num_requests, max_blocks]
+  const int32_t* rows;          // [num_seqs]
+  const int32_t* context_lens;  // [num_seqs], new tokens included
+  const int32_t* query_lens;    // [num_seqs]
+  const int32_t* new_blocks;    // [num_new_blocks]
+  int32_t* block_tables;        // [num_seqs, max_blocks]
+  int32_t* slot_mapping;        // [num_tokens]
+  int32_t* positions;           // [num_tokens]
+  int32_t* query_start_loc;     // [num_seqs + 1]
+  int32_t num_requests, num_seqs, max_blocks, num_new_blocks, num_tokens, block_size;
+};
+hipError_t launch_step_tables(const StepTablesParams& p, hipStream_t stream);
+
+// Norm and rotation of queries and keys (norm_rope.hip), the keys and the
+// values written to a cache as `cache` says (its source fields are this call's
+// key and value), or the keys to k_out.
+struct NormRopeParams {
+  RacParams cache;          // key_cache null: no cache
+  void* q_out;              // [num_tokens, num_heads, head_size]
+  void* k_out;              // [num_tokens, kv heads, head_size], or null
+  const void* query;
+  const int32_t* positions; // [num_tokens]
+  const float* cos_sin;     // [num_positions, rot]: rot / 2 cosines, rot / 2 sines
+  const void* q_weight;     // [head_size] or null
+  const void* k_weight;
+  int64_t q_stride;
+  int64_t num_positions;
+  int32_t num_heads;        // query heads
+  int32_t rot;
+  int32_t interleaved;
+  int32_t weight_f32;       // weights are float32 (else of the queries' type)
+  float eps;
+};
+hipError_t launch_norm_rope(const NormRopeParams& p, hipStream_t stream);
+
+// Attention of new tokens (extend_impl.h; the rules of pkv_paged_attention_extend).
+struct ExtendParams {
+  void* out;                       // [num_tokens, Hq, D]
+  const void* q;                   // [num_tokens, Hq, D], row stride q_stride
+  const void* k_cache;             // paged 5-D
+  const void* v_cache;
+  const int32_t* block_tables;
+  const int32_t* context_lens;
+  const int32_t* query_start_loc;  // [num_seqs + 1], null: one token per sequence
+  float* ws_ml;                    // [num_tokens, Hq, splits, 2]: (max, sum) per split, log2 domain
+  float* ws_o;                     // [num_tokens, Hq, splits, D]: outputs before the division by the sum
+  int32_t* counters;               // one token per sequence: arrivals per (sequence, unit), zero between launches
+  int64_t num_blocks;
+  int64_t q_stride;
+  int64_t k_block_stride, k_head_stride;
+  int64_t v_block_stride, v_head_stride;
+  float scale_log2;                // scale * log2(e) (FP8 caches: times k_scale)
+  float v_scale;                   // 1 but for FP8 caches
+  int32_t num_tokens, num_seqs, num_heads, num_kv_heads;
+  int32_t group, slices, units;    // as in DecodeParams
+  int32_t max_blocks_per_seq, max_seq_len, max_query_len;
+  int32_t window, sinks;           // window 0: the whole context
+  int32_t block_shift;             // log2(block_size)
+  int32_t splits;
+};
+// Row tiles (of kExtendRows) that num_tokens query tokens of num_seqs
+// sequences can make, and at least one more.
+constexpr int kExtendRows = 128;
+constexpr int64_t extend_items(int64_t num_tokens, int64_t num_seqs, int64_t group) {
+  return (num_tokens * group + kExtendRows - 1) / kExtendRows + std::min(num_seqs, num_tokens) + 1;
+}
+// Defined in extend_impl.h, instantiated per (query, cache) pair in extend_<q>_<cache>.hip.
+template <class QT, class CT>
+hipError_t launch_extend_typed(const ExtendParams& p, int head_size, hipStream_t stream);
 
 struct F32;
 struct F16;

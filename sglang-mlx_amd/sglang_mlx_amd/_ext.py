@@ -462,6 +462,287 @@ def reshape_and_cache_flash(key, value, key_cache, value_cache, slot_mapping, k_
                               True, k_scale, v_scale)
 
 
+# ---------------------------------------------------------------------------
+# Around the cache: a step's tables, norm and rotation with the append, and
+# attention of new tokens.  None has a counterpart in the reference.
+# ---------------------------------------------------------------------------
+
+
+def build_step_tables(request_blocks, rows, context_lens, query_lens, new_blocks, block_size, num_tokens):
+    """Block tables, slots and positions of one step, built on the device from
+    request lengths (rules: ``kernels.build_step_tables``)."""
+    for t in (request_blocks, rows, context_lens, query_lens, new_blocks):
+        _tensor(t)
+    block_size, num_tokens = int(block_size), int(num_tokens)
+    if request_blocks.dim() != 2:
+        raise ValueError("request_blocks must have shape [num_requests, max_blocks]")
+    if rows.dim() != 1 or context_lens.shape != rows.shape or query_lens.shape != rows.shape:
+        raise ValueError("rows, context_lens and query_lens must have shape [num_seqs]")
+    if new_blocks.dim() != 1:
+        raise ValueError("new_blocks must be 1-D")
+    if request_blocks.dtype != torch.int32 or not request_blocks.is_contiguous():
+        raise ValueError("request_blocks must be a contiguous int32 tensor (it is updated in place)")
+    if request_blocks.shape[1] == 0 or block_size <= 0:
+        raise ValueError("max_blocks and block_size must be positive")
+    if num_tokens < 0:
+        raise ValueError("num_tokens must be non-negative")
+    R, W = request_blocks.shape
+    B = rows.shape[0]
+    if B > _lib.PKV_MAX_STEP_SEQS:
+        raise ValueError(f"a step holds at most {_lib.PKV_MAX_STEP_SEQS} sequences")
+    for t in (rows, context_lens, query_lens, new_blocks):
+        _check_index(t)
+    dev = _on_gpu("BuildStepTables", request_blocks, rows, context_lens, query_lens, new_blocks)
+    rows, lens, new, fresh = _as_i32(rows), _as_i32(context_lens), _as_i32(query_lens), _as_i32(new_blocks)
+    tables = torch.empty((B, W), dtype=torch.int32, device=dev)
+    slots = torch.empty(num_tokens, dtype=torch.int32, device=dev)
+    positions = torch.empty(num_tokens, dtype=torch.int32, device=dev)
+    start = torch.empty(B + 1, dtype=torch.int32, device=dev)
+    lib = _lib.lib()
+    with torch.cuda.device(dev):
+        st = lib.pkv_build_step_tables(
+            request_blocks.data_ptr(), rows.data_ptr(), lens.data_ptr(), new.data_ptr(), fresh.data_ptr(),
+            tables.data_ptr(), slots.data_ptr(), positions.data_ptr(), start.data_ptr(), R, B, W, fresh.shape[0],
+            num_tokens, block_size, _stream(dev))
+    _lib.check(st)
+    return tables, slots, positions, start
+
+
+def _aligned_rows(t: torch.Tensor):
+    """(tensor, row stride) of [num_tokens, heads, head_size] rows as the norm
+    and rotation kernel reads them: a row contiguous, 16-byte aligned."""
+    N, H, D = t.shape
+    if t.stride()[1:] != (D, 1) or (N > 1 and (t.stride(0) < H * D or (t.stride(0) * t.element_size()) % 16)):
+        t = t.contiguous()
+    if t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.stride(0) if N > 1 else H * D
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
+def _check_norm_rope(query, key, positions, cos_sin, q_weight, k_weight, eps):
+    for t in (query, key, positions, cos_sin):
+        _tensor(t)
+    _tensor(q_weight, allow_none=True)
+    _tensor(k_weight, allow_none=True)
+    if query.dim() != 3 or key.dim() != 3 or key.shape[0] != query.shape[0] or key.shape[2] != query.shape[2]:
+        raise ValueError("query and key must have shapes [num_tokens, num_heads, head_size] and "
+                         "[num_tokens, num_kv_heads, head_size]")
+    N, Hq, D = query.shape
+    if Hq == 0 or key.shape[1] == 0:
+        raise ValueError("num_heads and num_kv_heads must be positive")
+    if D == 0 or D % 8 or D > 256:
+        raise ValueError("head_size must be a multiple of 8, at most 256")
+    code = _dtype_code(query)
+    if key.dtype != query.dtype:
+        raise ValueError("query and key dtypes differ")
+    if positions.dim() != 1 or positions.shape[0] != N:
+        raise ValueError("positions must have shape [num_tokens]")
+    if cos_sin.dim() != 2 or cos_sin.dtype != torch.float32 or cos_sin.shape[0] == 0:
+        raise ValueError("cos_sin must be a float32 tensor [num_positions, rotary_dim]")
+    rot = cos_sin.shape[1]
+    if rot < 2 or rot % 2 or rot > D:
+        raise ValueError("rotary_dim must be even, at least 2 and at most head_size")
+    weights = [w for w in (q_weight, k_weight) if w is not None]
+    for w in weights:
+        if w.dim() != 1 or w.shape[0] != D:
+            raise ValueError("norm weights must have shape [head_size]")
+        if w.dtype != weights[0].dtype or w.dtype not in (query.dtype, torch.float32):
+            raise ValueError("norm weights must be of the queries' type or float32, both alike")
+    if weights and not (math.isfinite(eps) and eps >= 0.0):
+        raise ValueError("eps must be finite and non-negative")
+    _check_index(positions)
+    return code, _DTYPE_CODE[weights[0].dtype] if weights else code
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def qk_norm_rope(query, key, positions, cos_sin, q_weight=None, k_weight=None, eps=1e-6, interleaved=False):
+    """Norm of queries and keys for each head and their rotation by position;
+    returns new (query, key) tensors (rules: ``kernels.qk_norm_rope``)."""
+    eps = float(eps)
+    code, wcode = _check_norm_rope(query, key, positions, cos_sin, q_weight, k_weight, eps)
+    dev = _on_gpu("QkNormRope", query, key, positions, cos_sin, q_weight, k_weight)
+    N, Hq, D = query.shape
+    H = key.shape[1]
+    q_out = torch.empty((N, Hq, D), dtype=query.dtype, device=dev)
+    k_out = torch.empty((N, H, D), dtype=query.dtype, device=dev)
+    if N == 0:
+        return q_out, k_out
+    query, q_stride = _aligned_rows(query)
+    key, k_stride = _aligned_rows(key)
+    positions, cos_sin = _as_i32(positions), _aligned(cos_sin)
+    qw, kw = (None if w is None else _aligned(w) for w in (q_weight, k_weight))
+    lib = _lib.lib()
+    with torch.cuda.device(dev):
+        st = lib.pkv_qk_norm_rope(
+            q_out.data_ptr(), k_out.data_ptr(), query.data_ptr(), key.data_ptr(), positions.data_ptr(),
+            cos_sin.data_ptr(), _ptr(qw), _ptr(kw), N, Hq, H, D, cos_sin.shape[1], cos_sin.shape[0], q_stride,
+            k_stride, eps, int(bool(interleaved)), wcode, code, _stream(dev))
+    _lib.check(st)
+    return q_out, k_out
+
+
+def qk_norm_rope_and_cache(query, key, value, positions, cos_sin, key_cache, value_cache, slot_mapping, q_weight=None,
+                           k_weight=None, eps=1e-6, interleaved=False, k_scale: float = 1.0, v_scale: float = 1.0):
+    """``qk_norm_rope`` with the append of the rotated keys and the values, one
+    launch; returns [query, key_cache, value_cache], the caches updated in
+    place (rules: ``kernels.qk_norm_rope_and_cache``)."""
+    eps = float(eps)
+    for t in (value, key_cache, value_cache, slot_mapping):
+        _tensor(t)
+    code, wcode = _check_norm_rope(query, key, positions, cos_sin, q_weight, k_weight, eps)
+    if value.shape != key.shape:
+        raise ValueError("key and value must have shape [num_tokens, num_kv_heads, head_size]")
+    if value.dtype != key.dtype:
+        raise ValueError("key and value dtypes differ")
+    if slot_mapping.dim() != 1 or slot_mapping.shape[0] != key.shape[0]:
+        raise ValueError("slot_mapping must have shape [num_tokens]")
+    N, Hq, D = query.shape
+    H = key.shape[1]
+    if value_cache.dtype != key_cache.dtype:
+        raise ValueError("key_cache and value_cache dtypes differ")
+    try:
+        cc = _FP8_DTYPE_CODE[key_cache.dtype]
+    except KeyError:
+        raise ValueError("Unsupported dtype") from None
+    fp8 = cc == _lib.PKV_FP8_E4M3
+    if not (code == cc or code == _lib.PKV_F32 or fp8):
+        raise ValueError(f"Unsupported key/cache dtype pair: {key.dtype} -> {key_cache.dtype}")
+    k_scale, v_scale = float(k_scale), float(v_scale)
+    if fp8 and not all(math.isfinite(v) and v != 0.0 for v in (k_scale, v_scale)):
+        raise ValueError("k_scale and v_scale must be finite and nonzero for FP8 caches")
+    x = 16 // _ELEM_BYTES[key_cache.dtype]
+    if key_cache.dim() == 5:
+        layout = _lib.PKV_LAYOUT_PAGED5D
+        nb, bs = key_cache.shape[0], key_cache.shape[3]
+        if tuple(key_cache.shape) != (nb, H, D // x, bs, x) or D % x:
+            raise ValueError("key_cache must have shape [num_blocks, num_kv_heads, head_size/x, block_size, x]")
+        if tuple(value_cache.shape) != (nb, H, D, bs):
+            raise ValueError("value_cache must have shape [num_blocks, num_kv_heads, head_size, block_size]")
+        if bs not in _BLOCK_SIZES:
+            raise ValueError("block_size must be 8, 16 or 32")
+        num_slots = nb * bs
+    elif key_cache.dim() in (3, 4):
+        layout = _lib.PKV_LAYOUT_TOKEN_MAJOR
+        if tuple(key_cache.shape[-2:]) != (H, D) or value_cache.shape != key_cache.shape:
+            raise ValueError("token-major caches must have shape [..., num_kv_heads, head_size]")
+        bs, num_slots = 1, key_cache.numel() // (H * D)
+    else:
+        raise ValueError("key_cache/value_cache must use a paged or token-major layout")
+    if not key_cache.is_contiguous() or not value_cache.is_contiguous():
+        raise ValueError("key_cache and value_cache must be contiguous (they are updated in place)")
+    _check_index(slot_mapping)
+    dev = _on_gpu("QkNormRopeAndCache", query, key, value, positions, cos_sin, key_cache, value_cache, slot_mapping,
+                  q_weight, k_weight)
+    q_out = torch.empty((N, Hq, D), dtype=query.dtype, device=dev)
+    if N == 0:
+        return [q_out, key_cache, value_cache]
+    query, q_stride = _aligned_rows(query)
+    key, k_stride = _aligned_rows(key)
+    value, v_stride = _aligned_rows(value)
+    positions, cos_sin, slots = _as_i32(positions), _aligned(cos_sin), _as_i32(slot_mapping)
+    qw, kw = (None if w is None else _aligned(w) for w in (q_weight, k_weight))
+    lib = _lib.lib()
+    with torch.cuda.device(dev):
+        st = lib.pkv_qk_norm_rope_and_cache(
+            q_out.data_ptr(), query.data_ptr(), key.data_ptr(), value.data_ptr(), positions.data_ptr(),
+            cos_sin.data_ptr(), _ptr(qw), _ptr(kw), key_cache.data_ptr(), value_cache.data_ptr(), slots.data_ptr(),
+            N, Hq, H, D, cos_sin.shape[1], cos_sin.shape[0], q_stride, k_stride, v_stride, eps,
+            int(bool(interleaved)), wcode, layout, bs, x, num_slots, code, cc, k_scale, v_scale, _stream(dev))
+    _lib.check(st)
+    return [q_out, key_cache, value_cache]
+
+
+def _new_token_attention(op, query, key_cache, value_cache, block_tables, context_lens, query_start_loc, num_kv_heads,
+                         scale, block_size, max_seq_len, max_query_len, window, num_sinks, k_scale, v_scale):
+    for t in (query, key_cache, value_cache, block_tables, context_lens):
+        _tensor(t)
+    _tensor(query_start_loc, allow_none=True)
+    num_kv_heads, block_size, max_seq_len = int(num_kv_heads), int(block_size), int(max_seq_len)
+    max_query_len, window, num_sinks = int(max_query_len), int(window), int(num_sinks)
+    k_scale, v_scale = float(k_scale), float(v_scale)
+    if query.dim() != 3:
+        raise ValueError("query must have shape [num_tokens, num_heads, head_size]")
+    if block_tables.dim() != 2 or context_lens.dim() != 1:
+        raise ValueError("block_tables must be 2D and context_lens must be 1D")
+    B = context_lens.shape[0]
+    if block_tables.shape[0] != B or (query_start_loc is None and query.shape[0] != B):
+        raise ValueError("query, block_tables, and context_lens sequence counts differ")
+    if query_start_loc is not None and (query_start_loc.dim() != 1 or query_start_loc.shape[0] != B + 1):
+        raise ValueError("query_start_loc must have shape [num_seqs + 1]")
+    if max_query_len <= 0:
+        raise ValueError("max_query_len must be positive")
+    if window < 0 or num_sinks < 0:
+        raise ValueError("window and num_sinks must be non-negative")
+    # (The decode's checks, with a query row for each of its sequences.)
+    qc, cc, layout = _check_paged_attention(query[:1].expand(B, -1, -1) if query.shape[0] else query.new_empty(
+        (B,) + query.shape[1:]), key_cache, value_cache, block_tables, context_lens, num_kv_heads, block_size,
+        max_seq_len, None)
+    if layout != _lib.PKV_LAYOUT_PAGED5D:
+        raise ValueError(f"{op} reads the paged 5-D layout")
+    fp8 = cc == _lib.PKV_FP8_E4M3
+    if qc == _lib.PKV_F32:
+        raise ValueError(f"Unsupported query/cache dtype pair for paged_attention: {query.dtype}/{key_cache.dtype}")
+    if max_seq_len > 1 << 30:
+        raise ValueError("max_seq_len must be at most 2^30")
+    if fp8 and not all(math.isfinite(v) and v != 0.0 for v in (k_scale, v_scale)):
+        raise ValueError("k_scale and v_scale must be finite and nonzero for FP8 caches")
+    _check_index(block_tables)
+    _check_index(context_lens)
+    if query_start_loc is not None:
+        _check_index(query_start_loc)
+    dev = _on_gpu(op, query, key_cache, value_cache, block_tables, context_lens, query_start_loc)
+    N, Hq, D = query.shape
+    out = torch.empty((N, Hq, D), dtype=query.dtype, device=dev)
+    if N == 0:
+        return out
+    query, q_stride = _aligned_rows(query)
+    bt, lens = _as_i32(block_tables), _as_i32(context_lens)
+    start = None if query_start_loc is None else _as_i32(query_start_loc)
+    lib = _lib.lib()
+    with torch.cuda.device(dev):
+        stream = _stream(dev)
+        need = lib.pkv_paged_attention_extend_workspace_size(N, B, Hq, num_kv_heads, D, max_seq_len, max_query_len,
+                                                             window, num_sinks)
+        ws = _decode_scratch(dev, stream, need)
+        st = lib.pkv_paged_attention_extend(
+            out.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), bt.data_ptr(),
+            lens.data_ptr(), _ptr(start), N, B, Hq, num_kv_heads, D, block_size, bt.shape[1], max_seq_len,
+            max_query_len, window, num_sinks, key_cache.shape[0], float(scale), q_stride, key_cache.stride(0),
+            key_cache.stride(1), value_cache.stride(0), value_cache.stride(1), ws.data_ptr(), ws.numel(), qc, cc,
+            k_scale, v_scale, stream)
+    _lib.check(st)
+    return out
+
+
+def paged_attention_window(query, key_cache, value_cache, block_tables, seq_lens, num_kv_heads, scale, block_size,
+                           max_seq_len, window, num_sinks=0, k_scale=1.0, v_scale=1.0):
+    """Decode attention over each context's last ``window`` tokens and its first
+    ``num_sinks`` (rules: ``kernels.paged_attention_window``)."""
+    if int(window) <= 0:
+        raise ValueError("window must be positive")
+    return _new_token_attention("PagedAttentionWindow", query, key_cache, value_cache, block_tables, seq_lens, None,
+                                num_kv_heads, scale, block_size, max_seq_len, 1, window, num_sinks, k_scale, v_scale)
+
+
+def paged_attention_extend(query, key_cache, value_cache, block_tables, seq_lens, query_start_loc, num_kv_heads,
+                           scale, block_size, max_seq_len, max_query_len, window=0, num_sinks=0, k_scale=1.0,
+                           v_scale=1.0):
+    """Causal attention of each sequence's new tokens over its cached context
+    (rules: ``kernels.paged_attention_extend``)."""
+    _tensor(query_start_loc)
+    return _new_token_attention("PagedAttentionExtend", query, key_cache, value_cache, block_tables, seq_lens,
+                                query_start_loc, num_kv_heads, scale, block_size, max_seq_len, max_query_len, window,
+                                num_sinks, k_scale, v_scale)
+
+
 def _block_mapping(block_mapping) -> torch.Tensor:
     _tensor(block_mapping)
     if block_mapping.dim() != 2 or block_mapping.shape[1] != 2:

@@ -25,6 +25,7 @@ PKV_ERR_HIP = 3
 PKV_F32, PKV_F16, PKV_BF16, PKV_FP8_E4M3 = 0, 1, 2, 3
 PKV_LAYOUT_PAGED5D, PKV_LAYOUT_TOKEN_MAJOR = 0, 1
 PKV_NOALLOC_SCRATCH_BYTES = 32 << 20  # static scratch of pkv_paged_attention_noalloc, per GPU
+PKV_MAX_STEP_SEQS = 4096  # sequences of one pkv_build_step_tables call
 PKV_COUNTER_BYTES = 65536  # arrival counters at the start of every decode workspace (zero between calls)
 
 _c_void_p = ctypes.c_void_p
@@ -105,6 +106,34 @@ SIGNATURES = {
         _i32, _i32,                                               # q dtype, cache dtype
         _f32, _f32, _c_void_p,                                    # k_scale, v_scale (FP8), stream
     ]),
+    "pkv_build_step_tables": (ctypes.c_int, [
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,    # request_blocks, rows, ctx, query_lens, new_blocks
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p,               # block_tables, slots, positions, query_start_loc
+        _i32, _i32, _i32, _i32, _i32, _i32,                       # requests, B, max_blocks, new blocks, tokens, bs
+        _c_void_p]),                                              # stream
+    "pkv_qk_norm_rope": (ctypes.c_int, [
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p,               # q_out, k_out, query, key
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p,               # positions, cos_sin, q_weight, k_weight
+        _i64, _i32, _i32, _i32, _i32, _i64,                       # tokens, Hq, Hkv, D, rotary_dim, num_positions
+        _i64, _i64, _f32, _i32, _i32, _i32,                       # q/k stride, eps, interleaved, weight dtype, dtype
+        _c_void_p]),                                              # stream
+    "pkv_qk_norm_rope_and_cache": (ctypes.c_int, [
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p,               # q_out, query, key, value
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p,               # positions, cos_sin, q_weight, k_weight
+        _c_void_p, _c_void_p, _c_void_p,                          # kc, vc, slots
+        _i64, _i32, _i32, _i32, _i32, _i64,                       # tokens, Hq, Hkv, D, rotary_dim, num_positions
+        _i64, _i64, _i64, _f32, _i32, _i32,                       # q/k/v stride, eps, interleaved, weight dtype
+        _i32, _i32, _i32, _i64, _i32, _i32,                       # layout, bs, x, num_slots, dtype, cache dtype
+        _f32, _f32, _c_void_p]),                                  # k_scale, v_scale (FP8), stream
+    "pkv_paged_attention_extend_workspace_size": (_size, [_i32] * 9),
+    "pkv_paged_attention_extend": (ctypes.c_int, [
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p,               # out, q, kc, vc
+        _c_void_p, _c_void_p, _c_void_p,                          # block_tables, ctx, query_start_loc
+        _i32, _i32, _i32, _i32, _i32, _i32,                       # tokens, B, Hq, Hkv, D, bs
+        _i32, _i32, _i32, _i32, _i32, _i64,                       # max_blocks, max_seq, max_query, window, sinks, nb
+        _f32, _i64, _i64, _i64, _i64, _i64,                       # scale, q_stride, k/v block & head strides
+        _c_void_p, _size, _i32, _i32,                             # workspace, bytes, q dtype, cache dtype
+        _f32, _f32, _c_void_p]),                                  # k_scale, v_scale (FP8), stream
     "pkv_copy_blocks": (ctypes.c_int, [
         ctypes.POINTER(_c_void_p), ctypes.POINTER(_c_void_p), _i32,  # src/dst planes, count
         _i64, _i64, _i64,                                            # src/dst blocks, block bytes

@@ -8,6 +8,14 @@ Operations:
     paged_attention_cascade  decode with radix-shared prefixes computed once
                          per group of sequences (a host-built plan)
     reshape_and_cache    scatter new KV tokens into the cache (in place)
+    build_step_tables    block tables, slots and positions of a step, from
+                         request lengths
+    qk_norm_rope         per-head norm of queries and keys and their rotation
+                         by position (rotary.rotary_table makes the table)
+    qk_norm_rope_and_cache  the same with the append of keys and values
+    paged_attention_window  decode over a sliding window and a few first tokens
+    paged_attention_extend  causal attention of several new tokens per sequence
+                         (prefills, chunks of them, drafted tokens)
     copy_blocks          block copies inside the caches
     swap_blocks          block copies between two buffers
     convert_fp8          element-wise conversion with a scale, FP8 E4M3 codes
@@ -126,6 +134,167 @@ def reshape_and_cache(
     key / k_scale and value / v_scale; the paged layout then has x = 16.
     """
     return _ext.reshape_and_cache(key, value, key_cache, value_cache, slot_mapping, k_scale, v_scale)
+
+
+def build_step_tables(
+    request_blocks: torch.Tensor,
+    rows: torch.Tensor,
+    context_lens: torch.Tensor,
+    query_lens: torch.Tensor,
+    new_blocks: torch.Tensor,
+    block_size: int,
+    num_tokens: int,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Block tables, slots and positions of one step, on the device.
+
+    Args:
+        request_blocks: [num_requests, max_blocks] int32, contiguous: each open
+            request's block ids in context order.  The blocks that the step
+            adds are stored into it.
+        rows: [num_seqs], each sequence's row of request_blocks, all different;
+            -1 (any row outside the table) is a padding sequence without tokens
+        context_lens: [num_seqs], tokens of each sequence with its new ones
+        query_lens: [num_seqs], its new tokens
+        new_blocks: 1-D, free block ids: sequences take theirs from it in order,
+            ceil(context / block_size) - ceil((context - new) / block_size) each
+        block_size: Number of tokens per block
+        num_tokens: length of the token outputs (padding included)
+
+    Returns:
+        block_tables [num_seqs, max_blocks] (-1 past a sequence's blocks),
+        slot_mapping and positions [num_tokens] of the new tokens end to end
+        (-1 and 0 past the last), query_start_loc [num_seqs + 1]; all int32.
+
+    A sequence whose context exceeds max_blocks * block_size has no tokens; with
+    too few new_blocks the blocks and slots that are missing are -1.
+    """
+    return _ext.build_step_tables(request_blocks, rows, context_lens, query_lens, new_blocks, block_size, num_tokens)
+
+
+def qk_norm_rope(
+    query: torch.Tensor,
+    key: torch.Tensor,
+    positions: torch.Tensor,
+    cos_sin: torch.Tensor,
+    q_weight: torch.Tensor | None = None,
+    k_weight: torch.Tensor | None = None,
+    eps: float = 1e-6,
+    interleaved: bool = False,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Norm of each head of queries and keys, then their rotation by position.
+
+    Args:
+        query: [num_tokens, num_heads, head_size], head_size a multiple of 8 up
+            to 256; rows may be views of a wider projection
+        key: [num_tokens, num_kv_heads, head_size], the same type
+        positions: [num_tokens] (32-bit ids); those outside the table take its
+            nearest row
+        cos_sin: [num_positions, rotary_dim] float32, rotary_dim / 2 cosines,
+            then as many sines (rotary.rotary_table); the head's first
+            rotary_dim elements turn, the others stay
+        q_weight, k_weight: [head_size], of the queries' type or float32: rows
+            become x / sqrt(mean(x^2) + eps) * weight first; None: no norm
+        interleaved: pairs are neighbours (2 i, 2 i + 1) rather than halves
+            (i, i + rotary_dim / 2)
+
+    Returns:
+        New contiguous (query, key).  Computed in float32, rounded once.
+    """
+    return _ext.qk_norm_rope(query, key, positions, cos_sin, q_weight, k_weight, eps, interleaved)
+
+
+def qk_norm_rope_and_cache(
+    query: torch.Tensor,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    positions: torch.Tensor,
+    cos_sin: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    slot_mapping: torch.Tensor,
+    q_weight: torch.Tensor | None = None,
+    k_weight: torch.Tensor | None = None,
+    eps: float = 1e-6,
+    interleaved: bool = False,
+    k_scale: float = 1.0,
+    v_scale: float = 1.0,
+) -> list[torch.Tensor]:
+    """``qk_norm_rope`` and ``reshape_and_cache`` of its keys and of the values
+    in one launch; returns [query, key_cache, value_cache].
+
+    Caches, slot_mapping and scales as in ``reshape_and_cache`` (paged 5-D with
+    blocks of 8, 16 or 32 tokens, or token rows [..., num_kv_heads, head_size]).
+    Keys are rounded once, from float32 to the cache's type.
+    """
+    return _ext.qk_norm_rope_and_cache(query, key, value, positions, cos_sin, key_cache, value_cache, slot_mapping,
+                                       q_weight, k_weight, eps, interleaved, k_scale, v_scale)
+
+
+def paged_attention_window(
+    query: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    block_tables: torch.Tensor,
+    context_lens: torch.Tensor,
+    num_kv_heads: int,
+    scale: float,
+    block_size: int,
+    max_seq_len: int,
+    window: int,
+    num_sinks: int = 0,
+    k_scale: float = 1.0,
+    v_scale: float = 1.0,
+) -> torch.Tensor:
+    """Decode attention over a sliding window: each sequence's query attends to
+    the last ``window`` tokens of its context (its own among them) and to the
+    first ``num_sinks``.  Arguments as ``paged_attention_v1`` (paged 5-D caches;
+    bfloat16 or float16 queries over caches of their type or uint8); only the
+    tokens that are attended to are read.
+    """
+    return _ext.paged_attention_window(query, key_cache, value_cache, block_tables, context_lens, num_kv_heads, scale,
+                                       block_size, max_seq_len, window, num_sinks, k_scale, v_scale)
+
+
+def paged_attention_extend(
+    query: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    block_tables: torch.Tensor,
+    context_lens: torch.Tensor,
+    query_start_loc: torch.Tensor,
+    num_kv_heads: int,
+    scale: float,
+    block_size: int,
+    max_seq_len: int,
+    max_query_len: int,
+    window: int = 0,
+    num_sinks: int = 0,
+    k_scale: float = 1.0,
+    v_scale: float = 1.0,
+) -> torch.Tensor:
+    """Causal attention of each sequence's new tokens over its cached context,
+    the new tokens among it (prefills, chunks of them, drafted tokens; a batch
+    may mix them with single tokens).
+
+    Args:
+        query: [num_tokens, num_heads, head_size], the sequences end to end
+        context_lens: [num_seqs], tokens in the cache, the new ones included: the
+            n query rows of a sequence are its context's last n tokens
+        query_start_loc: [num_seqs + 1], each sequence's first query row, and
+            the number of rows; output rows behind it are zero
+        max_query_len: at least the most query rows of one sequence
+        window, num_sinks: with a window > 0 a query sees the ``window`` last
+            tokens up to its own, and the context's first ``num_sinks``
+        The others as ``paged_attention_window``.
+
+    Returns:
+        [num_tokens, num_heads, head_size]; a row that sees no token (context 0
+        or beyond max_seq_len, more rows than max_query_len or than tokens) is
+        zero.
+    """
+    return _ext.paged_attention_extend(query, key_cache, value_cache, block_tables, context_lens, query_start_loc,
+                                       num_kv_heads, scale, block_size, max_seq_len, max_query_len, window, num_sinks,
+                                       k_scale, v_scale)
 
 
 def copy_blocks(

@@ -11,10 +11,12 @@ from .memory_pool import MHATokenPool, PooledKVCache, TokenPoolAllocator, decode
 from .paged_pool import (BlockAllocator, BlockRadixCache, BlockTable, CascadePlan, build_block_tables,
                          build_cascade_plan, plan_prefix_groups, tail_partitions)
 from .radix_cache import RadixCache, TreeNode
+from .request_blocks import RequestBlocks, StepTables
 
 __all__ = [
     "BasePrefixCache", "BlockAllocator", "BlockRadixCache", "BlockTable", "build_block_tables", "build_cascade_plan",
     "CascadePlan", "plan_prefix_groups", "tail_partitions", "CacheInitParams", "EvictParams", "EvictResult", "EvictionStrategy", "FIFOStrategy",
     "FILOStrategy", "InsertParams", "InsertResult", "LFUStrategy", "LRUStrategy", "MHATokenPool", "MRUStrategy",
-    "MatchResult", "PooledKVCache", "PriorityStrategy", "decode_batch", "RadixCache", "TokenPoolAllocator", "TreeNode",
+    "MatchResult", "PooledKVCache", "PriorityStrategy", "decode_batch", "RadixCache", "RequestBlocks", "StepTables",
+    "TokenPoolAllocator", "TreeNode",
 ]

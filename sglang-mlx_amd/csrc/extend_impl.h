@@ -64,9 +64,12 @@ __device__ __forceinline__ uint4 keep8(uint4 v, uint32_t bits) {
   return make_uint4(v.x & m(0), v.y & m(1), v.z & m(2), v.w & m(3));
 }
 
-// The eight elements of an FP8 cache as 16-bit ones.
-template <class T> __device__ __forceinline__ uint4 decode8(uint2 codes) {
-  const uint2 a = fp8x4_exact_inline<T>(codes.x), b = fp8x4_exact_inline<T>(codes.y);
+// Eight elements of an FP8 cache as 16-bit ones.  special: the wavefront has a
+// code with exponent 15 among those that it converts (the hardware conversion is
+// right for all others).
+template <class T> __device__ __forceinline__ uint4 decode8(uint2 codes, bool special) {
+  const uint2 a = special ? fp8x4_exact_inline<T>(codes.x) : fp8x4_cvt<T>(codes.x);
+  const uint2 b = special ? fp8x4_exact_inline<T>(codes.y) : fp8x4_cvt<T>(codes.y);
   return make_uint4(a.x, a.y, b.x, b.y);
 }
 
@@ -130,13 +133,14 @@ __device__ __forceinline__ void zero_tokens(const ExtendParams& p, int D, int64_
 }
 
 // ---------------------------------------------------------------------------
-// Tiles of query rows: one workgroup per (128 rows of a sequence, KV head,
-// split), four wavefronts of 32 rows.
+// Tiles of query rows: one workgroup per (128 RS rows of a sequence, KV head,
+// split), four wavefronts of 32 RS rows.
 //
-// A tile of 64 tokens of K and V is staged in LDS as the matrix units read it:
-// K as [D / 8][64 tokens][8], V as [token group of 8][D][8], so that the 32
-// lanes of a half read 512 consecutive bytes.  Both are gathers of 16-byte
-// pieces of the paged layout (FP8 codes become 16-bit elements on the way).
+// A tile of 64 tokens of K and V lies in LDS as the matrix units read it: K as
+// [D / 8][64 tokens][8], V as [token group of 8][D][8], so that the 32 lanes of
+// a half read 512 consecutive bytes.  Both are gathers of 16-byte pieces of the
+// paged layout: 16-bit caches go there by direct-to-LDS loads, a tile ahead of
+// the one in use; FP8 codes pass through registers and become 16-bit elements.
 //
 // Row rho of a 32-token score product is token 16 (rho / 4 % 2) + 4 (rho / 8) +
 // rho % 4, so that register r of half h is token 16 h + r; the tokens of K's
@@ -148,12 +152,31 @@ __device__ __forceinline__ void zero_tokens(const ExtendParams& p, int D, int64_
 // ---------------------------------------------------------------------------
 constexpr int kExtendTile = 64;
 constexpr int kExtendThreads = 256;
+// A row's reference point moves only when its maximum passes it by this much
+// (log2): weights then stay below 2^8, which changes no rounding, and most
+// tiles leave the outputs unscaled.
+constexpr float kExtendSlack = 8.f;
 
 // The token of a tile at place i of K's image.
 __device__ __forceinline__ int k_token(int i) { return (i & 32) + 16 * ((i >> 2) & 1) + 4 * ((i >> 3) & 3) + (i & 3); }
 
-template <class QT, class CT, int D>
-__global__ __launch_bounds__(kExtendThreads) void extend_kernel(ExtendParams p) {
+// Bit r of 16: a query at position pos sees token a + r.
+__device__ __forceinline__ uint32_t seen16(int pos, int a, int window, int sinks) {
+  auto below = [](int n) { return n <= 0 ? 0u : n >= 16 ? 0xffffu : (1u << n) - 1u; };  // the first n
+  return below(pos + 1 - a) & (~below(pos - window + 1 - a) | below(sinks - a));
+}
+
+// What lanes without a token load in its place.
+static __device__ const uint4 kNothing = {0, 0, 0, 0};
+
+// 16 bytes per lane, memory -> LDS at dst + 16 lane.
+__device__ __forceinline__ void load_to_lds(const void* src, uint4* dst) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                   (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+}
+
+template <class QT, class CT, int D, int RS>
+__global__ __launch_bounds__(kExtendThreads, RS == 1 ? 2 : 1) void extend_kernel(ExtendParams p) {
   using QS = typename Elem<QT>::storage;
   using CS = typename Elem<CT>::storage;
   constexpr bool F8 = std::is_same<CT, FP8>::value;
@@ -161,27 +184,41 @@ __global__ __launch_bounds__(kExtendThreads) void extend_kernel(ExtendParams p) 
   constexpr int DT = (D + 31) / 32;      // 32-dimension tiles of the output
   constexpr int DK = KSTEPS * 2;         // 8-dimension chunks staged
   constexpr int DV = DT * 32;            // dimensions of V staged
-  __shared__ uint4 s_k[DK * kExtendTile];
-  __shared__ uint4 s_v[kExtendTile / 8 * DV];
-  __shared__ int s_seq[3];
+  constexpr int KU = DK, VU = DV / 8;    // 64-lane loads per tile of K and of V
+  constexpr int ROWS = kExtendRows * RS, WROWS = 32 * RS;
+  // Two stages, arrays of their own: the compiler then knows that the loads in
+  // flight do not touch what is read.
+  __shared__ uint4 s_k0[DK * 64], s_k1[DK * 64];
+  __shared__ uint4 s_v0[8 * DV], s_v1[8 * DV];
+  __shared__ int s_seq[3], s_again;
+  using I0 = std::integral_constant<int, 0>;
+  using I1 = std::integral_constant<int, 1>;
+  auto k_image = [&](auto k) __attribute__((always_inline)) -> uint4* {
+    if constexpr (decltype(k)::value == 0) return s_k0;
+    else return s_k1;
+  };
+  auto v_image = [&](auto k) __attribute__((always_inline)) -> uint4* {
+    if constexpr (decltype(k)::value == 0) return s_v0;
+    else return s_v1;
+  };
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int kvh = blockIdx.x % p.num_kv_heads;
   const int item = blockIdx.x / p.num_kv_heads;
+  const int items = gridDim.x / p.num_kv_heads;
   const int split = blockIdx.y;
   const int group = p.group, h0 = kvh * group;
 
   // The workgroup's sequence and row tile: tiles of the sequences lie end to
   // end, a sequence's last tile (the longest) first.
-  const int items = gridDim.x / p.num_kv_heads;
   if (wave == 0) {
     int base = 0, found = -1, z = 0;
     for (int s0 = 0; s0 < p.num_seqs; s0 += 64) {
       const int s = s0 + lane;
       int tiles = 0;
-      if (s < p.num_seqs) tiles = (extend_seq(p, s).count * group + kExtendRows - 1) / kExtendRows;
+      if (s < p.num_seqs) tiles = (extend_seq(p, s).count * group + ROWS - 1) / ROWS;
       int sum = tiles;
 #pragma unroll
       for (int d = 1; d < 64; d <<= 1) {
@@ -197,7 +234,7 @@ __global__ __launch_bounds__(kExtendThreads) void extend_kernel(ExtendParams p) 
       }
       base += __shfl(sum, 63);
     }
-    if (lane == 0) s_seq[0] = found, s_seq[1] = z, s_seq[2] = base;
+    if (lane == 0) s_seq[0] = found, s_seq[1] = z, s_seq[2] = base, s_again = 0;
   }
   __syncthreads();
   const int seq = __builtin_amdgcn_readfirstlane(s_seq[0]);
@@ -214,20 +251,26 @@ __global__ __launch_bounds__(kExtendThreads) void extend_kernel(ExtendParams p) 
   const ExtendSeq q = extend_seq(p, seq);
   const int first_pos = q.ctx - q.count;  // position of the sequence's first query token
   const int rows = q.count * group;
-  const int row0 = z * kExtendRows;
-  const int row_end = min(row0 + kExtendRows, rows);
+  const int row0 = z * ROWS;
+  const int row_end = min(row0 + ROWS, rows);
   // Positions of the workgroup's rows; tokens before position 0 see nothing.
   const int pmin = first_pos + row0 / group, pmax = first_pos + (row_end - 1) / group;
 
-  // This lane's row.
-  const int row = row0 + wave * 32 + col;
-  const bool live = row < rows;
-  const int tok = live ? row / group : 0;
-  const int head = h0 + (live ? row - tok * group : 0);
-  const int64_t qrow = q.start + tok;
-  const int pos = live && q.ctx > 0 ? first_pos + tok : -1;
+  // This lane's rows.
+  bool live[RS];
+  int head[RS], pos[RS];
+  int64_t qrow[RS];
+  const int wr0 = row0 + wave * WROWS, wr1 = min(wr0 + WROWS, rows);
+#pragma unroll
+  for (int i = 0; i < RS; ++i) {
+    const int row = wr0 + 32 * i + col;
+    live[i] = row < rows;
+    const int tok = live[i] ? row / group : 0;
+    head[i] = h0 + (live[i] ? row - tok * group : 0);
+    qrow[i] = q.start + tok;
+    pos[i] = live[i] && q.ctx > 0 ? first_pos + tok : -1;
+  }
   // Positions of the wavefront's rows (uniform): none where w_min > w_max.
-  const int wr0 = row0 + wave * 32, wr1 = min(wr0 + 32, rows);
   const bool w_any = wr0 < wr1 && q.ctx > 0;
   const int w_min = w_any ? first_pos + wr0 / group : 0, w_max = w_any ? first_pos + (wr1 - 1) / group : -1;
 
@@ -243,215 +286,344 @@ __global__ __launch_bounds__(kExtendThreads) void extend_kernel(ExtendParams p) 
   }
   const int per = (ntiles + p.splits - 1) / p.splits;
   const int v0 = min(split * per, ntiles), v1 = min(v0 + per, ntiles);
+  auto tile_start = [&](int v) { return (v < lead ? v : base_tile + v - lead) * kExtendTile; };
 
-  uint4 qf[KSTEPS];
-  {
-    const QS* src = static_cast<const QS*>(p.q) + qrow * p.q_stride + (int64_t)head * D;
+  uint4 qf[RS][KSTEPS];
+  const uint32_t sign = p.scale_log2 < 0.f ? 0x80008000u : 0u;  // (a negative scale goes into the queries)
+  const float scale = fmaxf(__builtin_fabsf(p.scale_log2), 0x1p-120f);
+#pragma unroll
+  for (int i = 0; i < RS; ++i) {
+    const QS* src = static_cast<const QS*>(p.q) + qrow[i] * p.q_stride + (int64_t)head[i] * D;
 #pragma unroll
     for (int j = 0; j < KSTEPS; ++j) {
       const int d = 16 * j + 8 * half;
-      qf[j] = live && d < D ? *reinterpret_cast<const uint4*>(src + d) : make_uint4(0, 0, 0, 0);
+      const uint4 x = live[i] && d < D ? *reinterpret_cast<const uint4*>(src + d) : make_uint4(0, 0, 0, 0);
+      qf[i][j] = make_uint4(x.x ^ sign, x.y ^ sign, x.z ^ sign, x.w ^ sign);
     }
   }
-  f32x16 o[DT];
+  f32x16 o[RS][DT];
+  float m[RS], l[RS];
+  auto reset = [&]() __attribute__((always_inline)) {
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
+    for (int i = 0; i < RS; ++i) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
-  float m = kNoScore, l = 0.f;
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[i][dt][r] = 0.f;
+      m[i] = kNoScore;
+      l[i] = 0.f;
+    }
+  };
+  reset();
 
   const int shift = p.block_shift, bs = 1 << shift;
   const int32_t* table = p.block_tables + (int64_t)seq * p.max_blocks_per_seq;
   const CS* kc = static_cast<const CS*>(p.k_cache) + (int64_t)kvh * p.k_head_stride;
   const CS* vc = static_cast<const CS*>(p.v_cache) + (int64_t)kvh * p.v_head_stride;
 
-  for (int v = v0; v < v1; ++v) {
-    const int t0 = (v < lead ? v : base_tile + v - lead) * kExtendTile;
-    // The block of this lane's token, -1 past the context or outside the pool.
+  // The block of this lane's token of tile v, -1 past the context, outside the
+  // pool or past the last tile.
+  auto load_bid = [&](int v) __attribute__((always_inline)) {
     int32_t bid = -1;
-    if (t0 + lane < q.ctx) {
-      bid = table[(t0 + lane) >> shift];
-      if (bid < 0 || (int64_t)bid >= p.num_blocks) bid = -1;
+    if (v < v1) {
+      const int t = tile_start(v) + lane;
+      if (t < q.ctx) bid = table[t >> shift];
     }
-    const uint64_t ok_tokens = __ballot(bid >= 0);
+    return bid >= 0 && (int64_t)bid < p.num_blocks ? bid : -1;
+  };
+  // FP8: a tile's codes on their way to LDS.
+  constexpr int FK = F8 ? (KU / 2 + 3) / 4 : 1, FV = F8 ? (VU + 3) / 4 : 1;
+  uint4 fk[FK] = {};
+  uint2 fv[FV] = {};
+  // Issues the loads of the tile at t0, whose tokens' blocks are bid.
+  auto stage = [&](auto k, int t0, int32_t bid) __attribute__((always_inline)) {
     const int kt = t0 + k_token(lane);  // the token that this lane stages of K
     const int kb = __shfl(bid, k_token(lane));
-    __syncthreads();  // the tile before has been read
+    const CS* kp = kc + (int64_t)max(kb, 0) * p.k_block_stride;
     if constexpr (!F8) {
-      for (int c = wave; c < DK; c += 4) {
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (kb >= 0 && c * 8 < D)
-          x = *reinterpret_cast<const uint4*>(kc + kb * p.k_block_stride + c * 8 * bs + (kt & (bs - 1)) * 8);
-        s_k[c * kExtendTile + lane] = x;
+#pragma unroll
+      for (int j = 0; j < (KU + 3) / 4; ++j) {
+        const int c = 4 * j + wave;
+        if (KU % 4 != 0 && c >= KU) continue;
+        const CS* src = kp + (c * 8 * bs + (kt & (bs - 1)) * 8);
+        const bool have = kb >= 0 && (D % 16 == 0 || c * 8 < D);
+        load_to_lds(have ? (const void*)src : (const void*)&kNothing, k_image(k) + c * 64);
       }
     } else {
-      for (int c = wave; c < DK / 2; c += 4) {
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (kb >= 0 && c * 16 < D)
-          x = *reinterpret_cast<const uint4*>(kc + kb * p.k_block_stride + c * 16 * bs + (kt & (bs - 1)) * 16);
-        s_k[2 * c * kExtendTile + lane] = decode8<QT>(make_uint2(x.x, x.y));
-        s_k[(2 * c + 1) * kExtendTile + lane] = decode8<QT>(make_uint2(x.z, x.w));
+#pragma unroll
+      for (int j = 0; j < FK; ++j) {
+        const int c = 4 * j + wave;
+        fk[j] = make_uint4(0, 0, 0, 0);
+        if (kb >= 0 && c * 16 < D) fk[j] = *reinterpret_cast<const uint4*>(kp + (c * 16 * bs + (kt & (bs - 1)) * 16));
       }
     }
-    for (int u0 = wave * 64; u0 < kExtendTile / 8 * DV; u0 += kExtendThreads) {
+#pragma unroll
+    for (int j = 0; j < (VU + 3) / 4; ++j) {
+      const int u0 = (4 * j + wave) * 64;
+      if (VU % 4 != 0 && u0 >= 8 * DV) continue;
       const int u = u0 + lane, tg = u / DV, d = u - tg * DV;
       const int vb = __shfl(bid, 8 * tg);
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (vb >= 0 && d < D) {
-        const CS* src = vc + vb * p.v_block_stride + d * bs + ((t0 + 8 * tg) & (bs - 1));
-        if constexpr (F8)
-          x = decode8<QT>(*reinterpret_cast<const uint2*>(src));
-        else
-          x = *reinterpret_cast<const uint4*>(src);
+      const CS* src = vc + (int64_t)max(vb, 0) * p.v_block_stride + (d * bs + ((t0 + 8 * tg) & (bs - 1)));
+      const bool have = vb >= 0 && (D % 32 == 0 || d < D);
+      if constexpr (!F8) {
+        load_to_lds(have ? (const void*)src : (const void*)&kNothing, v_image(k) + u0);
+      } else {
+        fv[j] = make_uint2(0, 0);
+        if (have) fv[j] = *reinterpret_cast<const uint2*>(src);
       }
-      s_v[u] = x;
     }
-    __syncthreads();
+  };
+  auto finish_stage = [&](auto k) __attribute__((always_inline)) {
+    if constexpr (F8) {
+      uint32_t probe = 0;
+#pragma unroll
+      for (int j = 0; j < FK; ++j)
+        probe |= fp8x4_special(fk[j].x) | fp8x4_special(fk[j].y) | fp8x4_special(fk[j].z) | fp8x4_special(fk[j].w);
+#pragma unroll
+      for (int j = 0; j < FV; ++j) probe |= fp8x4_special(fv[j].x) | fp8x4_special(fv[j].y);
+      auto write = [&](bool special) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < FK; ++j) {
+          const int c = 4 * j + wave;
+          if (2 * c < DK) {
+            k_image(k)[2 * c * 64 + lane] = decode8<QT>(make_uint2(fk[j].x, fk[j].y), special);
+            k_image(k)[(2 * c + 1) * 64 + lane] = decode8<QT>(make_uint2(fk[j].z, fk[j].w), special);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < FV; ++j) {
+          const int u0 = (4 * j + wave) * 64;
+          if (VU % 4 == 0 || u0 < 8 * DV) v_image(k)[u0 + lane] = decode8<QT>(fv[j], special);
+        }
+      };
+      if (__any(probe != 0u))
+        write(true);
+      else
+        write(false);
+    }
+  };
+  // The workgroup meets at a bare s_barrier, each wavefront's own loads and LDS
+  // accesses awaited before (a __syncthreads would do the same).
+  auto meet = [] __attribute__((always_inline)) {
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+    asm volatile("s_barrier" ::: "memory");
+  };
 
-    // Whether any of the wavefront's rows sees a token of the tile, and whether all see all.
-    const bool in_sinks = t0 < sinks;
-    if (w_max < t0 || !(in_sinks || t0 + kExtendTile > w_min - window + 1)) continue;
-    const bool whole = t0 + kExtendTile - 1 <= w_min && (t0 > w_max - window || t0 + kExtendTile <= sinks) &&
-                       ok_tokens == ~0ull && wr0 + 32 <= rows;
-
-    f32x16 s[2];
+  // The tile at t0, in image k.  whole: every row of the wavefront sees all of it.
+  // CAREFUL: what a row does not see is kept out of its products.
+  auto attend = [&](auto k, auto careful, bool whole, int t0, uint64_t ok_tokens) __attribute__((always_inline)) {
+    constexpr bool CAREFUL = decltype(careful)::value;
+    const uint4* ki = k_image(k);
+    const uint4* vi = v_image(k);
+    f32x16 s[RS][2];
 #pragma unroll
     for (int sub = 0; sub < 2; ++sub) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[sub][r] = 0.f;
+      for (int i = 0; i < RS; ++i)
 #pragma unroll
-      for (int j = 0; j < KSTEPS; ++j)
-        s[sub] = mma32<QT>(s_k[(2 * j + half) * kExtendTile + 32 * sub + col], qf[j], s[sub]);
+        for (int r = 0; r < 16; ++r) s[i][sub][r] = 0.f;
+#pragma unroll
+      for (int j = 0; j < KSTEPS; ++j) {
+        const uint4 kf = ki[(2 * j + half) * 64 + 32 * sub + col];
+#pragma unroll
+        for (int i = 0; i < RS; ++i) s[i][sub] = mma32<QT>(kf, qf[i][j], s[i][sub]);
+      }
     }
-    // Bit r of sees[sub]: the row sees token 32 sub + 16 half + r.
-    uint32_t sees[2] = {0xffffu, 0xffffu};
     if (!whole) {
 #pragma unroll
       for (int sub = 0; sub < 2; ++sub) {
-        const int a = t0 + 32 * sub + 16 * half;
-        auto below = [&](int n) { return n <= 0 ? 0u : n >= 16 ? 0xffffu : (1u << n) - 1u; };  // the first n tokens
-        uint32_t b = below(pos + 1 - a) & (~below(pos - window + 1 - a) | below(sinks - a));
-        sees[sub] = b & (uint32_t)(ok_tokens >> (32 * sub + 16 * half)) & 0xffffu;
+        const int a = t0 + 32 * sub + 16 * half;  // token of register 0
+#pragma unroll
+        for (int i = 0; i < RS; ++i) {
+          const uint32_t sees = seen16(pos[i], a, window, sinks) & (uint32_t)(ok_tokens >> (32 * sub + 16 * half));
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[i][sub][r] = sees >> r & 1u ? s[i][sub][r] : kNoScore;
+        }
       }
     }
-    float mt = m;
+    float ref[RS];
 #pragma unroll
-    for (int sub = 0; sub < 2; ++sub)
+    for (int i = 0; i < RS; ++i) {
+      float mt = kNoScore;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[sub][r] = whole || (sees[sub] >> r & 1u) ? s[sub][r] * p.scale_log2 : kNoScore;
-        mt = fmaxf(mt, s[sub][r]);
+      for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[i][sub][r]);
+      mt = fmaxf(xchg32_max(mt), m[i]);
+      if (__any(mt * scale > m[i] * scale + kExtendSlack || (m[i] == kNoScore && mt != kNoScore))) {
+        const float alpha = mt == kNoScore ? 1.f : __builtin_amdgcn_exp2f((m[i] - mt) * scale);
+        m[i] = mt;
+        l[i] *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[i][dt][r] *= alpha;
       }
-    mt = xchg32_max(mt);
-    // (A row that has seen nothing keeps a finite reference point: no inf - inf.)
-    const float ref = mt == kNoScore ? 0.f : mt;
-    const float alpha = __builtin_amdgcn_exp2f(m - ref);
-    m = mt;
-    l *= alpha;
-    uint32_t w[2][8];
+      // (A row that has seen nothing keeps a finite reference point: no inf - inf.)
+      ref[i] = m[i] == kNoScore ? 0.f : m[i] * scale;
+    }
+    uint32_t w[RS][2][8];
+    auto exponentials = [&](int sub) __attribute__((always_inline)) {
 #pragma unroll
-    for (int sub = 0; sub < 2; ++sub)
+      for (int i = 0; i < RS; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; r += 2) {
-        const float a = __builtin_amdgcn_exp2f(s[sub][r] - ref), b = __builtin_amdgcn_exp2f(s[sub][r + 1] - ref);
-        l += a + b;
-        w[sub][r / 2] = pack_weights<QT>(a, b);
-      }
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
-
-    auto v_piece = [&](int dt, int sub, int k) {  // tokens 32 sub + 16 half + 8 k ..+7 of dimension 32 dt + col
-      return s_v[(4 * sub + 2 * half + k) * DV + 32 * dt + col];
+        for (int r = 0; r < 16; r += 2) {
+          const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][sub][r], scale, -ref[i]));
+          const float b = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][sub][r + 1], scale, -ref[i]));
+          l[i] += a + b;
+          w[i][sub][r / 2] = pack_weights<QT>(a, b);
+        }
     };
-    auto weights = [&](int sub, int k) {
-      return make_uint4(w[sub][4 * k], w[sub][4 * k + 1], w[sub][4 * k + 2], w[sub][4 * k + 3]);
+    auto v_piece = [&](int dt, int sub, int k8) {  // tokens 32 sub + 16 half + 8 k8 ..+7 of dimension 32 dt + col
+      return vi[(4 * sub + 2 * half + k8) * DV + 32 * dt + col];
     };
-    bool clean = true;
-    if (!whole) {
+    auto weights = [&](int i, int sub, int k8) {
+      return make_uint4(w[i][sub][4 * k8], w[i][sub][4 * k8 + 1], w[i][sub][4 * k8 + 2], w[i][sub][4 * k8 + 3]);
+    };
+    auto products = [&](int sub) __attribute__((always_inline)) {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int k8 = 0; k8 < 2; ++k8) {
+          const uint4 vf = v_piece(dt, sub, k8);
+#pragma unroll
+          for (int i = 0; i < RS; ++i) o[i][dt] = mma32<QT>(vf, weights(i, sub, k8), o[i][dt]);
+        }
+    };
+    exponentials(0);
+    if constexpr (!CAREFUL) {
+      products(0);
+      exponentials(1);
+      products(1);
+    } else {
+      exponentials(1);
+      // One query position at a time, with the tokens that it does not see taken
+      // out of V; the other positions' rows keep their sums.
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll 1
+        for (int at = w_min; at <= w_max; ++at)
+#pragma unroll
+          for (int sub = 0; sub < 2; ++sub) {
+            const uint32_t keep = seen16(at, t0 + 32 * sub + 16 * half, window, sinks);
+            const uint4 va = keep8(v_piece(dt, sub, 0), keep), vb = keep8(v_piece(dt, sub, 1), keep >> 8);
+#pragma unroll
+            for (int i = 0; i < RS; ++i) {
+              f32x16 n = mma32<QT>(va, weights(i, sub, 0), o[i][dt]);
+              n = mma32<QT>(vb, weights(i, sub, 1), n);
+#pragma unroll
+              for (int r = 0; r < 16; ++r) o[i][dt][r] = pos[i] == at ? n[r] : o[i][dt][r];
+            }
+          }
+    }
+    if (!CAREFUL && !whole) {
       // A token that some rows do not see must not reach them, whatever its
-      // value: a weight of 0 times inf or NaN is NaN.  The product with zeros
-      // tells whether the tile has such a value.
+      // value, but a weight of 0 times inf or NaN is NaN.  The product with zeros
+      // tells whether the tile has such a value: the rows are then done again.
       f32x16 zero;
 #pragma unroll
       for (int r = 0; r < 16; ++r) zero[r] = 0.f;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-          for (int k = 0; k < 2; ++k) zero = mma32<QT>(v_piece(dt, sub, k), make_uint4(0, 0, 0, 0), zero);
+        for (int j = 0; j < 4; ++j) zero = mma32<QT>(v_piece(dt, j >> 1, j & 1), make_uint4(0, 0, 0, 0), zero);
       float sum = 0.f;
 #pragma unroll
       for (int r = 0; r < 16; ++r) sum += zero[r];
-      clean = !__any(sum != 0.f);
+      if (__any(sum != 0.f)) s_again = 1;
     }
-    if (clean) {
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-          for (int k = 0; k < 2; ++k) o[dt] = mma32<QT>(v_piece(dt, sub, k), weights(sub, k), o[dt]);
-    } else {
-      // One query position at a time, with the tokens that it does not see taken
-      // out of V; the other positions' rows keep their sums.
-      for (int at = w_min; at <= w_max; ++at) {
-        uint32_t keep[2];
-#pragma unroll
-        for (int sub = 0; sub < 2; ++sub) {
-          uint32_t b = 0;
-          for (int r = 0; r < 16; ++r) {
-            const int t = t0 + 32 * sub + 16 * half + r;
-            if (t <= at && (t > at - window || t < sinks) && (ok_tokens >> (t - t0) & 1u)) b |= 1u << r;
-          }
-          keep[sub] = b;
-        }
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-          f32x16 n = o[dt];
-#pragma unroll
-          for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-              n = mma32<QT>(keep8(v_piece(dt, sub, k), keep[sub] >> (8 * k)), weights(sub, k), n);
-#pragma unroll
-          for (int r = 0; r < 16; ++r) o[dt][r] = pos == at ? n[r] : o[dt][r];
-        }
+  };
+  auto consume = [&](auto k, auto careful, int t0, uint64_t ok_tokens) __attribute__((always_inline)) {
+    // Whether any of the wavefront's rows sees a token of the tile, and whether all see all.
+    if (w_max < t0 || !(t0 < sinks || t0 + kExtendTile > w_min - window + 1)) return;
+    const bool whole = t0 + kExtendTile - 1 <= w_min && (t0 > w_max - window || t0 + kExtendTile <= sinks) &&
+                       ok_tokens == ~0ull && wr0 + WROWS <= rows;
+    attend(k, careful, whole, t0, ok_tokens);
+  };
+
+  // Takes the tokens past the context out of the last tile's image of V (K's are
+  // masked out): the 8-token group in which the context ends was loaded whole.
+  auto trim = [&](auto k, int t0) __attribute__((always_inline)) {
+    if (t0 + kExtendTile <= q.ctx || q.ctx % 8 == 0) return;
+    uint4* group8 = v_image(k) + (q.ctx - t0) / 8 * DV;
+    for (int d = tid; d < DV; d += kExtendThreads) group8[d] = keep8(group8[d], (1u << q.ctx % 8) - 1u);
+    meet();
+  };
+  // Tile v is consumed while tile v + 1 loads and the blocks of tile v + 2 are
+  // looked up.
+  if (v0 < v1) {
+    int32_t bid = load_bid(v0), next = load_bid(v0 + 1);
+    uint64_t ok_tokens = __ballot(bid >= 0);
+    stage(I0{}, tile_start(v0), bid);
+    finish_stage(I0{});
+    auto step = [&](auto k, int v) __attribute__((always_inline)) {
+      using KN = std::integral_constant<int, decltype(k)::value ^ 1>;
+      const int t0 = tile_start(v);
+      meet();  // tile v has landed, tile v - 1 has been read
+      trim(k, t0);
+      const uint64_t ok_next = __ballot(next >= 0);
+      if (v + 1 < v1) stage(KN{}, tile_start(v + 1), next);
+      next = load_bid(v + 2);
+      consume(k, std::false_type{}, t0, ok_tokens);
+      if (v + 1 < v1) finish_stage(KN{});
+      ok_tokens = ok_next;
+    };
+    for (int v = v0; v < v1; v += 2) {
+      step(I0{}, v);
+      if (v + 1 >= v1) break;
+      step(I1{}, v + 1);
+    }
+    meet();
+    if (__builtin_expect(s_again, 0)) {
+      reset();
+#pragma unroll 1
+      for (int v = v0; v < v1; ++v) {
+        const int t0 = tile_start(v);
+        bid = load_bid(v);
+        ok_tokens = __ballot(bid >= 0);
+        meet();
+        stage(I0{}, t0, bid);
+        finish_stage(I0{});
+        meet();
+        trim(I0{}, t0);
+        consume(I0{}, std::true_type{}, t0, ok_tokens);
       }
     }
   }
 
-  l = xchg32_sum(l);
-  if (!live) return;
-  if (p.splits == 1) {
-    const float inv = l > 0.f ? p.v_scale / l : l == 0.f ? 0.f : l;  // (NaN stays NaN)
-    QS* out = static_cast<QS*>(p.out) + (qrow * p.num_heads + head) * D;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
+  for (int i = 0; i < RS; ++i) {
+    const float sum = xchg32_sum(l[i]);
+    if (!live[i]) continue;
+    if (p.splits == 1) {
+      const float inv = sum > 0.f ? p.v_scale / sum : sum == 0.f ? 0.f : sum;  // (NaN stays NaN)
+      QS* out = static_cast<QS*>(p.out) + (qrow[i] * p.num_heads + head[i]) * D;
 #pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        const int d = 32 * dt + 2 * r + 4 * half;
-        if (D % 32 != 0 && d >= D) continue;
-        uint2 x;
-        x.x = pack2(from_f32<QT>(o[dt][r] * inv), from_f32<QT>(o[dt][r + 1] * inv));
-        x.y = pack2(from_f32<QT>(o[dt][r + 2] * inv), from_f32<QT>(o[dt][r + 3] * inv));
-        *reinterpret_cast<uint2*>(out + d) = x;
-      }
-    return;
-  }
-  const int64_t at = (qrow * p.num_heads + head) * p.splits + split;
-  float* wo = p.ws_o + at * D;
+      for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
+        for (int r = 0; r < 16; r += 4) {
+          const int d = 32 * dt + 2 * r + 4 * half;
+          if (D % 32 != 0 && d >= D) continue;
+          uint2 x;
+          x.x = pack2(from_f32<QT>(o[i][dt][r] * inv), from_f32<QT>(o[i][dt][r + 1] * inv));
+          x.y = pack2(from_f32<QT>(o[i][dt][r + 2] * inv), from_f32<QT>(o[i][dt][r + 3] * inv));
+          *reinterpret_cast<uint2*>(out + d) = x;
+        }
+    } else {
+      const int64_t at = (qrow[i] * p.num_heads + head[i]) * p.splits + split;
+      float* wo = p.ws_o + at * D;
 #pragma unroll
-    for (int r = 0; r < 16; r += 4) {
-      const int d = 32 * dt + 2 * r + 4 * half;
-      if (D % 32 != 0 && d >= D) continue;
-      *reinterpret_cast<float4*>(wo + d) = make_float4(o[dt][r], o[dt][r + 1], o[dt][r + 2], o[dt][r + 3]);
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+          const int d = 32 * dt + 2 * r + 4 * half;
+          if (D % 32 != 0 && d >= D) continue;
+          *reinterpret_cast<float4*>(wo + d) =
+              make_float4(o[i][dt][r], o[i][dt][r + 1], o[i][dt][r + 2], o[i][dt][r + 3]);
+        }
+      if (half == 0) *reinterpret_cast<float2*>(p.ws_ml + at * 2) = make_float2(m[i] * scale, sum);
     }
-  if (half == 0) *reinterpret_cast<float2*>(p.ws_ml + at * 2) = make_float2(m, l);
+  }
 }
 
 // The outputs of a call whose row tiles are split: one wavefront per query row.
@@ -496,10 +668,11 @@ __global__ __launch_bounds__(256) void extend_merge_kernel(ExtendParams p) {
 constexpr int kWindowTile = 32;
 
 template <class QT, class CT, int D>
-__global__ __launch_bounds__(256) void window_decode_kernel(ExtendParams p) {
+__global__ __launch_bounds__(256, 2) void window_decode_kernel(ExtendParams p) {
   using QS = typename Elem<QT>::storage;
   using CS = typename Elem<CT>::storage;
   constexpr bool F8 = std::is_same<CT, FP8>::value;
+  constexpr int X = F8 ? 16 : 8;  // elements of a 16-byte K chunk
   constexpr int KSTEPS = F8 ? (D + 63) / 64 * 2 : (D + 31) / 32;
   constexpr int DT = (D + 15) / 16;
   __shared__ float s_o[4][DT * 4][64];
@@ -533,8 +706,8 @@ __global__ __launch_bounds__(256) void window_decode_kernel(ExtendParams p) {
   const int lead = (sinks + kWindowTile - 1) / kWindowTile;
   const int base_tile = max(lo / kWindowTile, lead);
   const int ntiles = lead + pos / kWindowTile + 1 - base_tile;
-  // (At least one split: a sequence of few tiles leaves the others nothing.)
-  const int per = max((ntiles + p.splits - 1) / p.splits, 1);
+  // Parts of one length for all sequences, that of the longest cut in p.splits.
+  const int per = p.part_tiles;
   const int parts = (ntiles + per - 1) / per;
   const int v0 = split * per, v1 = min(v0 + per, ntiles);
   if (split >= parts) return;
@@ -557,57 +730,79 @@ __global__ __launch_bounds__(256) void window_decode_kernel(ExtendParams p) {
   const CS* kc = static_cast<const CS*>(p.k_cache) + (int64_t)kvh * p.k_head_stride;
   const CS* vc = static_cast<const CS*>(p.v_cache) + (int64_t)kvh * p.v_head_stride;
 
-  for (int v = v0 + wave; v < v1; v += 4) {
-    const int t0 = (v < lead ? v : base_tile + v - lead) * kWindowTile;
-    auto block_of = [&](int t) {
-      if (t >= q.ctx) return -1;
-      const int b = table[t >> shift];
-      return b >= 0 && (int64_t)b < p.num_blocks ? b : -1;
-    };
-    const int tk = t0 + 8 * (col >> 2), tv = t0 + 8 * g;  // first of the eight tokens of this lane's K row, of its V pieces
-    const int kb = block_of(tk), vb = block_of(tv);
-    f32x4 s[2];
-    const int64_t krow = (int64_t)max(kb, 0) * p.k_block_stride;
+  // A tile's blocks (of this lane's K row and of its V pieces), and its K and V.
+  struct Blocks {
+    int k, v;
+  };
+  auto tile_start = [&](int v) { return (v < lead ? v : base_tile + v - lead) * kWindowTile; };
+  auto load_blocks = [&](int v) __attribute__((always_inline)) {
+    Blocks b{-1, -1};
+    if (v < v1) {
+      const int t0 = tile_start(v), tk = t0 + 8 * (col >> 2), tv = t0 + 8 * g;
+      if (tk < q.ctx) b.k = table[tk >> shift];
+      if (tv < q.ctx) b.v = table[tv >> shift];
+    }
+    auto valid = [&](int id) { return id >= 0 && (int64_t)id < p.num_blocks ? id : -1; };
+    return Blocks{valid(b.k), valid(b.v)};
+  };
+  using VR = typename std::conditional<F8, uint2, uint4>::type;
+  constexpr int KL = F8 ? KSTEPS / 2 : KSTEPS;  // 16-byte loads of K per product
+  struct Tile {
+    uint4 k[2][KL];
+    VR v[DT];
+  };
+  // (A missing block's loads go to block 0; its tokens are masked.)
+  auto load_tile = [&](Tile& x, int v, const Blocks& b) __attribute__((always_inline)) {
+    const int t0 = tile_start(v), tk = t0 + 8 * (col >> 2), tv = t0 + 8 * g;
+    const CS* kp = kc + (int64_t)max(b.k, 0) * p.k_block_stride + ((tk & (bs - 1)) + (col & 3)) * X;
+    const CS* vp = vc + (int64_t)max(b.v, 0) * p.v_block_stride + (tv & (bs - 1));
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int j = 0; j < KL; ++j) {
+        const int c = 4 * j + g;
+        x.k[u][j] = c * X < D ? *reinterpret_cast<const uint4*>(kp + (c * bs + 4 * u) * X) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+      x.v[dt] = *reinterpret_cast<const VR*>(vp + (D % 16 == 0 ? 16 * dt + col : min(16 * dt + col, D - 1)) * bs);
+  };
+  auto attend = [&](const Tile& x, int v, const Blocks& b) __attribute__((always_inline)) {
+    const int tv = tile_start(v) + 8 * g;
+    bool special = false;
     if constexpr (F8) {
-      uint4 kf[2][KSTEPS / 2];
+      uint32_t probe = 0;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int j = 0; j < KSTEPS / 2; ++j) {
-          const int c = 4 * j + g;
-          kf[u][j] = c * 16 < D ? *reinterpret_cast<const uint4*>(
-                                      kc + krow + c * 16 * bs + ((tk & (bs - 1)) + 4 * u + (col & 3)) * 16)
-                                : make_uint4(0, 0, 0, 0);
-        }
+        for (int j = 0; j < KL; ++j)
+          probe |= fp8x4_special(x.k[u][j].x) | fp8x4_special(x.k[u][j].y) | fp8x4_special(x.k[u][j].z) |
+                   fp8x4_special(x.k[u][j].w);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        s[u] = {0.f, 0.f, 0.f, 0.f};
+      for (int dt = 0; dt < DT; ++dt) probe |= fp8x4_special(x.v[dt].x) | fp8x4_special(x.v[dt].y);
+      special = __any(probe != 0u);
+    }
+    f32x4 s[2];
 #pragma unroll
-        for (int j = 0; j < KSTEPS / 2; ++j) {
-          s[u] = Mma<QT>::k32(decode8<QT>(make_uint2(kf[u][j].x, kf[u][j].y)), qf[2 * j], s[u]);
-          s[u] = Mma<QT>::k32(decode8<QT>(make_uint2(kf[u][j].z, kf[u][j].w)), qf[2 * j + 1], s[u]);
-        }
-      }
-    } else {
+    for (int u = 0; u < 2; ++u) {
+      s[u] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        s[u] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int j = 0; j < KSTEPS; ++j) {
-          const int c = 4 * j + g;
-          const uint4 k = c * 8 < D ? *reinterpret_cast<const uint4*>(
-                                          kc + krow + c * 8 * bs + ((tk & (bs - 1)) + 4 * u + (col & 3)) * 8)
-                                    : make_uint4(0, 0, 0, 0);
-          s[u] = Mma<QT>::k32(k, qf[j], s[u]);
+      for (int j = 0; j < KL; ++j) {
+        if constexpr (F8) {
+          s[u] = Mma<QT>::k32(decode8<QT>(make_uint2(x.k[u][j].x, x.k[u][j].y), special), qf[2 * j], s[u]);
+          s[u] = Mma<QT>::k32(decode8<QT>(make_uint2(x.k[u][j].z, x.k[u][j].w), special), qf[2 * j + 1], s[u]);
+        } else {
+          s[u] = Mma<QT>::k32(x.k[u][j], qf[j], s[u]);
         }
       }
     }
     // Bit i: token tv + i is seen (by every row alike).
-    uint32_t sees = 0;
-    if (vb >= 0) {
+    uint32_t sees = 0xffu;
+    if (!(tv >= lo && tv + 8 <= q.ctx && b.v >= 0)) {
+      sees = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (tv + i < q.ctx && (tv + i >= lo || tv + i < sinks)) sees |= 1u << i;
+        if (b.v >= 0 && tv + i < q.ctx && (tv + i >= lo || tv + i < sinks)) sees |= 1u << i;
     }
     float mt = m;
 #pragma unroll
@@ -627,25 +822,53 @@ __global__ __launch_bounds__(256) void window_decode_kernel(ExtendParams p) {
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int r = 0; r < 4; r += 2) {
-        const float a = __builtin_amdgcn_exp2f(s[u][r] - ref), b = __builtin_amdgcn_exp2f(s[u][r + 1] - ref);
-        l += a + b;
-        w[2 * u + r / 2] = pack_weights<QT>(a, b);
+        const float a = __builtin_amdgcn_exp2f(s[u][r] - ref), c = __builtin_amdgcn_exp2f(s[u][r + 1] - ref);
+        l += a + c;
+        w[2 * u + r / 2] = pack_weights<QT>(a, c);
       }
     const uint4 wf = make_uint4(w[0], w[1], w[2], w[3]);
-    const int64_t vrow = (int64_t)max(vb, 0) * p.v_block_stride + (tv & (bs - 1));
+    // What a token that is not seen holds must not matter.
+    const bool hidden = __any(sees != 0xffu);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
-      const int d = min(16 * dt + col, D - 1);
-      uint4 x;
+      uint4 y;
       if constexpr (F8)
-        x = decode8<QT>(*reinterpret_cast<const uint2*>(vc + vrow + d * bs));
+        y = decode8<QT>(x.v[dt], special);
       else
-        x = *reinterpret_cast<const uint4*>(vc + vrow + d * bs);
-      // What a token that is not seen holds must not matter.
-      if (sees != 0xffu) x = keep8(x, sees);
+        y = x.v[dt];
+      if (hidden) y = keep8(y, sees);
 #pragma unroll
       for (int r = 0; r < 4; ++r) o[dt][r] *= alpha;
-      o[dt] = Mma<QT>::k32(x, wf, o[dt]);
+      o[dt] = Mma<QT>::k32(y, wf, o[dt]);
+    }
+  };
+  // Each wavefront takes every fourth tile.  While one is attended, the next one
+  // loads (where the registers hold two, which stops at head size 128) and the
+  // blocks of the one after are looked up.
+  constexpr int NW = 4;
+  Blocks b0 = load_blocks(v0 + wave);
+  if constexpr (D <= 128) {
+    Blocks b1 = load_blocks(v0 + wave + NW);
+    Tile x0, x1;
+    if (v0 + wave < v1) load_tile(x0, v0 + wave, b0);
+    for (int v = v0 + wave; v < v1; v += 2 * NW) {
+      Blocks b2 = load_blocks(v + 2 * NW);
+      if (v + NW < v1) load_tile(x1, v + NW, b1);
+      attend(x0, v, b0);
+      if (v + NW >= v1) break;
+      b0 = b2;
+      b2 = load_blocks(v + 3 * NW);
+      if (v + 2 * NW < v1) load_tile(x0, v + 2 * NW, b0);
+      attend(x1, v + NW, b1);
+      b1 = b2;
+    }
+  } else {
+    for (int v = v0 + wave; v < v1; v += NW) {
+      const Blocks b1 = load_blocks(v + NW);
+      Tile x;
+      load_tile(x, v, b0);
+      attend(x, v, b0);
+      b0 = b1;
     }
   }
 
@@ -667,7 +890,7 @@ __global__ __launch_bounds__(256) void window_decode_kernel(ExtendParams p) {
   __syncthreads();
   // Wavefront w sums the 16-dimension tiles w, w + 4, ...
   const float inv = L > 0.f ? p.v_scale / L : L == 0.f ? 0.f : L;
-  const int64_t row = (int64_t)q.start * p.num_heads + h0 + col;
+  const int64_t row0 = (int64_t)q.start * p.num_heads + h0, row = row0 + col;
 #pragma unroll
   for (int k = 0; k < (DT + 3) / 4; ++k) {
     const int dt = 4 * k + wave;
@@ -696,23 +919,38 @@ __global__ __launch_bounds__(256) void window_decode_kernel(ExtendParams p) {
   if (tid == 0) s_last = arrived_last(p.counters + (int64_t)seq * p.units + unit, parts);
   __syncthreads();
   if (!s_last) return;
+  // (The states lie in what was the wavefronts' outputs.)
+  static_assert(sizeof(s_o) >= 16 * kWindowMaxSplits * sizeof(float2), "room for every state");
+  float2* s_ml = reinterpret_cast<float2*>(&s_o[0][0][0]);
+  for (int i = tid; i < nh * parts; i += 256) {
+    const int h = i / parts;
+    s_ml[i] = load_agent(p.ws_ml + ((row0 + h) * p.splits + (i - h * parts)) * 2);
+  }
+  __syncthreads();
   for (int i = tid; i < nh * (D / 2); i += 256) {
     const int h = i / (D / 2), d = 2 * (i - h * (D / 2));
-    const int64_t r = (int64_t)q.start * p.num_heads + h0 + h;
+    const float2* state = s_ml + h * parts;
+    const float* from = p.ws_o + (row0 + h) * p.splits * D + d;
     float mm = kNoScore;
-    for (int s = 0; s < parts; ++s) mm = fmaxf(mm, load_agent(p.ws_ml + (r * p.splits + s) * 2).x);
+    for (int s = 0; s < parts; ++s) mm = fmaxf(mm, state[s].x);
     const float rf = mm == kNoScore ? 0.f : mm;
     float ll = 0.f, x = 0.f, y = 0.f;
-    for (int s = 0; s < parts; ++s) {
-      const float2 ml = load_agent(p.ws_ml + (r * p.splits + s) * 2);
-      const float2 v = load_agent(p.ws_o + (r * p.splits + s) * D + d);
-      const float e = __builtin_amdgcn_exp2f(ml.x - rf);
-      ll += e * ml.y;
-      x += e * v.x;
-      y += e * v.y;
+    constexpr int U = 8;  // loads in flight
+    for (int s = 0; s < parts; s += U) {
+      float2 v[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k) v[k] = load_agent(from + (int64_t)min(s + k, parts - 1) * D);
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        if (s + k >= parts) continue;
+        const float e = __builtin_amdgcn_exp2f(state[s + k].x - rf);
+        ll += e * state[s + k].y;
+        x += e * v[k].x;
+        y += e * v[k].y;
+      }
     }
     const float iv = ll > 0.f ? p.v_scale / ll : ll == 0.f ? 0.f : ll;
-    *reinterpret_cast<uint32_t*>(static_cast<QS*>(p.out) + r * D + d) =
+    *reinterpret_cast<uint32_t*>(static_cast<QS*>(p.out) + (row0 + h) * D + d) =
         pack2(from_f32<QT>(x * iv), from_f32<QT>(y * iv));
   }
 }
@@ -726,7 +964,7 @@ hipError_t launch_extend_d(const ExtendParams& p, hipStream_t stream) {
     return hipGetLastError();
   }
   const int64_t items = extend_items(p.num_tokens, p.num_seqs, p.group);
-  hipLaunchKernelGGL((extend_kernel<QT, CT, D>), dim3((unsigned)(items * p.num_kv_heads), (unsigned)p.splits),
+  hipLaunchKernelGGL((extend_kernel<QT, CT, D, 1>), dim3((unsigned)(items * p.num_kv_heads), (unsigned)p.splits),
                      dim3(kExtendThreads), 0, stream, p);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.splits == 1) return e;

@@ -300,11 +300,13 @@ struct ExtendParams {
   int32_t max_blocks_per_seq, max_seq_len, max_query_len;
   int32_t window, sinks;           // window 0: the whole context
   int32_t block_shift;             // log2(block_size)
-  int32_t splits;
+  int32_t splits;                  // the most parts of a row
+  int32_t part_tiles;              // one token per sequence: 32-token tiles of a part
 };
 // Row tiles (of kExtendRows) that num_tokens query tokens of num_seqs
 // sequences can make, and at least one more.
 constexpr int kExtendRows = 128;
+constexpr int kWindowMaxSplits = 64;  // parts of a decode's length (their states meet in LDS)
 constexpr int64_t extend_items(int64_t num_tokens, int64_t num_seqs, int64_t group) {
   return (num_tokens * group + kExtendRows - 1) / kExtendRows + std::min(num_seqs, num_tokens) + 1;
 }

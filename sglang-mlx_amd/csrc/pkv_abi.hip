@@ -724,6 +724,7 @@ int pkv_qk_norm_rope(void* q_out, void* k_out, const void* query, const void* ke
   pkv::NormRopeParams p = {};
   p.q_out = q_out;
   p.k_out = k_out;
+  p.cache.block_size = 1;
   p.cache.cache_dtype = dtype;
   p.cache.key = key;
   p.cache.key_stride = k_stride;

@@ -274,6 +274,7 @@ struct NormRopeParams {
   int32_t interleaved;
   int32_t weight_f32;       // weights are float32 (else of the queries' type)
   float eps;
+  float inv_head_size;      // set by the launcher
 };
 hipError_t launch_norm_rope(const NormRopeParams& p, hipStream_t stream);
 

@@ -471,6 +471,11 @@ def reshape_and_cache_flash(key, value, key_cache, value_cache, slot_mapping, k_
 def build_step_tables(request_blocks, rows, context_lens, query_lens, new_blocks, block_size, num_tokens):
     """Block tables, slots and positions of one step, built on the device from
     request lengths (rules: ``kernels.build_step_tables``)."""
+    if _native is not None:
+        out = _native.build_step_tables(request_blocks, rows, context_lens, query_lens, new_blocks, block_size,
+                                        num_tokens)
+        if _done(out):
+            return out
     for t in (request_blocks, rows, context_lens, query_lens, new_blocks):
         _tensor(t)
     block_size, num_tokens = int(block_size), int(num_tokens)
@@ -566,6 +571,10 @@ def _ptr(t):
 def qk_norm_rope(query, key, positions, cos_sin, q_weight=None, k_weight=None, eps=1e-6, interleaved=False):
     """Norm of queries and keys for each head and their rotation by position;
     returns new (query, key) tensors (rules: ``kernels.qk_norm_rope``)."""
+    if _native is not None:
+        out = _native.qk_norm_rope(query, key, positions, cos_sin, q_weight, k_weight, eps, interleaved)
+        if _done(out):
+            return out
     eps = float(eps)
     code, wcode = _check_norm_rope(query, key, positions, cos_sin, q_weight, k_weight, eps)
     dev = _on_gpu("QkNormRope", query, key, positions, cos_sin, q_weight, k_weight)
@@ -594,6 +603,11 @@ def qk_norm_rope_and_cache(query, key, value, positions, cos_sin, key_cache, val
     """``qk_norm_rope`` with the append of the rotated keys and the values, one
     launch; returns [query, key_cache, value_cache], the caches updated in
     place (rules: ``kernels.qk_norm_rope_and_cache``)."""
+    if _native is not None:
+        out = _native.qk_norm_rope_and_cache(query, key, positions, cos_sin, q_weight, k_weight, eps, interleaved,
+                                             value, key_cache, value_cache, slot_mapping, k_scale, v_scale)
+        if _done(out):
+            return out
     eps = float(eps)
     for t in (value, key_cache, value_cache, slot_mapping):
         _tensor(t)
@@ -662,6 +676,12 @@ def qk_norm_rope_and_cache(query, key, value, positions, cos_sin, key_cache, val
 
 def _new_token_attention(op, query, key_cache, value_cache, block_tables, context_lens, query_start_loc, num_kv_heads,
                          scale, block_size, max_seq_len, max_query_len, window, num_sinks, k_scale, v_scale):
+    if _native is not None:
+        out = _native.new_token_attention(_ws_cache, query, key_cache, value_cache, block_tables, context_lens,
+                                          query_start_loc, num_kv_heads, scale, block_size, max_seq_len,
+                                          max_query_len, window, num_sinks, k_scale, v_scale)
+        if _done(out):
+            return out
     for t in (query, key_cache, value_cache, block_tables, context_lens):
         _tensor(t)
     _tensor(query_start_loc, allow_none=True)

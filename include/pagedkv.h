@@ -496,18 +496,20 @@ size_t pkv_paged_attention_extend_workspace_size(int32_t num_tokens,
  *                  query_start_loc[num_seqs] on become zeros.
  * query_start_loc: [num_seqs + 1], from 0, not decreasing, at most num_tokens;
  *                  NULL: one token per sequence (num_tokens == num_seqs).
- * max_query_len  : at least the most query rows of a sequence; with 1 the
- *                  decode kernel runs.
+ * max_query_len  : at least the most query rows of a sequence.  A tight bound
+ *                  chooses the faster kernel (see below), no more.
  * window, num_sinks: window 0 attends to the whole context, and num_sinks is
  *                  then not used.
  * The other arguments as pkv_paged_attention's with PKV_LAYOUT_PAGED5D;
  * (q_dtype, cache_dtype): (BF16, BF16), (F16, F16), (BF16 | F16, FP8_E4M3);
  * max_seq_len is at most 2^30.  V's base and strides are 16-byte aligned (FP8:
  * 8-byte).
- * Launches: with max_query_len 1 one kernel, a workgroup per (sequence, KV
- * head, part of the length), whose last arrival merges the parts in their
- * order; otherwise one kernel of 128-row tiles, and where those would leave the
- * chip idle their lengths are split too and a second kernel merges.
+ * Launches: with single tokens (max_query_len 1), or few rows per KV head
+ * (max_query_len * num_heads / num_kv_heads at most 16), one kernel, a workgroup
+ * per (sequence, 16 rows of a KV head, part of the length), whose last arrival
+ * merges the parts in their order; otherwise one kernel of 128-row tiles, and
+ * where those would leave the chip idle their lengths are split too and a second
+ * kernel merges.
  */
 int pkv_paged_attention_extend(void* out, const void* query,
                                const void* key_cache, const void* value_cache,

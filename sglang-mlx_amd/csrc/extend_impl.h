@@ -133,22 +133,32 @@ __device__ __forceinline__ void zero_tokens(const ExtendParams& p, int D, int64_
 }
 
 // ---------------------------------------------------------------------------
-// Tiles of query rows: one workgroup per (128 RS rows of a sequence, KV head,
-// split), four wavefronts of 32 RS rows.
+// Tiles of query rows: one workgroup per (128 rows of a sequence, KV head,
+// split), four wavefronts of 32 rows.
 //
 // A tile of 64 tokens of K and V lies in LDS as the matrix units read it: K as
-// [D / 8][64 tokens][8], V as [token group of 8][D][8], so that the 32 lanes of
-// a half read 512 consecutive bytes.  Both are gathers of 16-byte pieces of the
-// paged layout: 16-bit caches go there by direct-to-LDS loads, a tile ahead of
-// the one in use; FP8 codes pass through registers and become 16-bit elements.
+// [token group of 16][D / 8][16 tokens][8], V as [token group of 8][D][8].  Both
+// are gathers of 16-byte pieces of the paged layout: 16-bit caches go there by
+// direct-to-LDS loads, a tile ahead of the one in use; FP8 codes pass through
+// registers and become 16-bit elements.  A load takes its pieces from one block
+// (K of 8-token blocks: from two), so that its address is a scalar and a lane
+// offset that stays: with an address per lane and load the vector unit spent
+// 110 of 243 instructions a tile on them.
 //
 // Row rho of a 32-token score product is token 16 (rho / 4 % 2) + 4 (rho / 8) +
-// rho % 4, so that register r of half h is token 16 h + r; the tokens of K's
-// image lie in that order (the token order would put two of every eight lanes'
-// reads on the same banks).
+// rho % 4, so that register r of half h is token 16 h + r.  K's groups lie 64
+// bytes further apart than they are long: eight lanes' reads, four tokens of
+// either group, then touch different banks.
 //
 // Tiles that every row of a wavefront sees in full take no mask; a wavefront
 // skips tiles that none of its rows sees.
+//
+// Bound: the matrix units, which a tile's softmax and its barrier keep waiting:
+// 8192 new tokens on 8192, 32 heads of 128, bf16, take 1.75 ms, 943 TFLOP/s of the
+// 1381 that a large matrix product reaches.  Matrix units busy 42 % and vector units
+// 50 % of the time; 32-token tiles in four stages with the softmax of one beside the
+// products of the next came to 952 TFLOP/s.  Cuts of the workgroup: 128 rows let two
+// workgroups share a CU, so that one computes while the other waits.
 // ---------------------------------------------------------------------------
 constexpr int kExtendTile = 64;
 constexpr int kExtendThreads = 256;
@@ -156,9 +166,6 @@ constexpr int kExtendThreads = 256;
 // (log2): weights then stay below 2^8, which changes no rounding, and most
 // tiles leave the outputs unscaled.
 constexpr float kExtendSlack = 8.f;
-
-// The token of a tile at place i of K's image.
-__device__ __forceinline__ int k_token(int i) { return (i & 32) + 16 * ((i >> 2) & 1) + 4 * ((i >> 3) & 3) + (i & 3); }
 
 // Bit r of 16: a query at position pos sees token a + r.
 __device__ __forceinline__ uint32_t seen16(int pos, int a, int window, int sinks) {
@@ -175,8 +182,8 @@ __device__ __forceinline__ void load_to_lds(const void* src, uint4* dst) {
                                    (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
 }
 
-template <class QT, class CT, int D, int RS>
-__global__ __launch_bounds__(kExtendThreads, RS == 1 ? 2 : 1) void extend_kernel(ExtendParams p) {
+template <class QT, class CT, int D>
+__global__ __launch_bounds__(kExtendThreads, 2) void extend_kernel(ExtendParams p) {
   using QS = typename Elem<QT>::storage;
   using CS = typename Elem<CT>::storage;
   constexpr bool F8 = std::is_same<CT, FP8>::value;
@@ -184,11 +191,11 @@ __global__ __launch_bounds__(kExtendThreads, RS == 1 ? 2 : 1) void extend_kernel
   constexpr int DT = (D + 31) / 32;      // 32-dimension tiles of the output
   constexpr int DK = KSTEPS * 2;         // 8-dimension chunks staged
   constexpr int DV = DT * 32;            // dimensions of V staged
-  constexpr int KU = DK, VU = DV / 8;    // 64-lane loads per tile of K and of V
-  constexpr int ROWS = kExtendRows * RS, WROWS = 32 * RS;
+  constexpr int KG = DK * 16 + 4;        // 16-byte pieces from one token group of K's image to the next
+  constexpr int VU = DV / 8;             // 64-lane loads of a tile of V
   // Two stages, arrays of their own: the compiler then knows that the loads in
   // flight do not touch what is read.
-  __shared__ uint4 s_k0[DK * 64], s_k1[DK * 64];
+  __shared__ uint4 s_k0[4 * KG], s_k1[4 * KG];
   __shared__ uint4 s_v0[8 * DV], s_v1[8 * DV];
   __shared__ int s_seq[3], s_again;
   using I0 = std::integral_constant<int, 0>;
@@ -218,7 +225,7 @@ __global__ __launch_bounds__(kExtendThreads, RS == 1 ? 2 : 1) void extend_kernel
     for (int s0 = 0; s0 < p.num_seqs; s0 += 64) {
       const int s = s0 + lane;
       int tiles = 0;
-      if (s < p.num_seqs) tiles = (extend_seq(p, s).count * group + ROWS - 1) / ROWS;
+      if (s < p.num_seqs) tiles = (extend_seq(p, s).count * group + kExtendRows - 1) / kExtendRows;
       int sum = tiles;
 #pragma unroll
       for (int d = 1; d < 64; d <<= 1) {
@@ -251,25 +258,19 @@ __global__ __launch_bounds__(kExtendThreads, RS == 1 ? 2 : 1) void extend_kernel
   const ExtendSeq q = extend_seq(p, seq);
   const int first_pos = q.ctx - q.count;  // position of the sequence's first query token
   const int rows = q.count * group;
-  const int row0 = z * ROWS;
-  const int row_end = min(row0 + ROWS, rows);
+  const int row0 = z * kExtendRows;
+  const int row_end = min(row0 + kExtendRows, rows);
   // Positions of the workgroup's rows; tokens before position 0 see nothing.
   const int pmin = first_pos + row0 / group, pmax = first_pos + (row_end - 1) / group;
 
-  // This lane's rows.
-  bool live[RS];
-  int head[RS], pos[RS];
-  int64_t qrow[RS];
-  const int wr0 = row0 + wave * WROWS, wr1 = min(wr0 + WROWS, rows);
-#pragma unroll
-  for (int i = 0; i < RS; ++i) {
-    const int row = wr0 + 32 * i + col;
-    live[i] = row < rows;
-    const int tok = live[i] ? row / group : 0;
-    head[i] = h0 + (live[i] ? row - tok * group : 0);
-    qrow[i] = q.start + tok;
-    pos[i] = live[i] && q.ctx > 0 ? first_pos + tok : -1;
-  }
+  // This lane's row.
+  const int wr0 = row0 + wave * 32, wr1 = min(wr0 + 32, rows);
+  const int row = wr0 + col;
+  const bool live = row < rows;
+  const int tok = live ? row / group : 0;
+  const int head = h0 + (live ? row - tok * group : 0);
+  const int64_t qrow = q.start + tok;
+  const int pos = live && q.ctx > 0 ? first_pos + tok : -1;
   // Positions of the wavefront's rows (uniform): none where w_min > w_max.
   const bool w_any = wr0 < wr1 && q.ctx > 0;
   const int w_min = w_any ? first_pos + wr0 / group : 0, w_max = w_any ? first_pos + (wr1 - 1) / group : -1;
@@ -288,31 +289,27 @@ __global__ __launch_bounds__(kExtendThreads, RS == 1 ? 2 : 1) void extend_kernel
   const int v0 = min(split * per, ntiles), v1 = min(v0 + per, ntiles);
   auto tile_start = [&](int v) { return (v < lead ? v : base_tile + v - lead) * kExtendTile; };
 
-  uint4 qf[RS][KSTEPS];
+  uint4 qf[KSTEPS];
   const uint32_t sign = p.scale_log2 < 0.f ? 0x80008000u : 0u;  // (a negative scale goes into the queries)
   const float scale = fmaxf(__builtin_fabsf(p.scale_log2), 0x1p-120f);
-#pragma unroll
-  for (int i = 0; i < RS; ++i) {
-    const QS* src = static_cast<const QS*>(p.q) + qrow[i] * p.q_stride + (int64_t)head[i] * D;
+  {
+    const QS* src = static_cast<const QS*>(p.q) + qrow * p.q_stride + (int64_t)head * D;
 #pragma unroll
     for (int j = 0; j < KSTEPS; ++j) {
       const int d = 16 * j + 8 * half;
-      const uint4 x = live[i] && d < D ? *reinterpret_cast<const uint4*>(src + d) : make_uint4(0, 0, 0, 0);
-      qf[i][j] = make_uint4(x.x ^ sign, x.y ^ sign, x.z ^ sign, x.w ^ sign);
+      const uint4 x = live && d < D ? *reinterpret_cast<const uint4*>(src + d) : make_uint4(0, 0, 0, 0);
+      qf[j] = make_uint4(x.x ^ sign, x.y ^ sign, x.z ^ sign, x.w ^ sign);
     }
   }
-  f32x16 o[RS][DT];
-  float m[RS], l[RS];
+  f32x16 o[DT];
+  float m, l;
   auto reset = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < RS; ++i) {
+    for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[i][dt][r] = 0.f;
-      m[i] = kNoScore;
-      l[i] = 0.f;
-    }
+      for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
+    m = kNoScore;
+    l = 0.f;
   };
   reset();
 
@@ -321,55 +318,75 @@ __global__ __launch_bounds__(kExtendThreads, RS == 1 ? 2 : 1) void extend_kernel
   const CS* kc = static_cast<const CS*>(p.k_cache) + (int64_t)kvh * p.k_head_stride;
   const CS* vc = static_cast<const CS*>(p.v_cache) + (int64_t)kvh * p.v_head_stride;
 
-  // The block of this lane's token of tile v, -1 past the context, outside the
-  // pool or past the last tile.
+  // The block of 8-token group lane % 8 of tile v, -1 past the context, outside
+  // the pool or past the last tile.
   auto load_bid = [&](int v) __attribute__((always_inline)) {
     int32_t bid = -1;
     if (v < v1) {
-      const int t = tile_start(v) + lane;
+      const int t = tile_start(v) + 8 * (lane & 7);
       if (t < q.ctx) bid = table[t >> shift];
     }
     return bid >= 0 && (int64_t)bid < p.num_blocks ? bid : -1;
   };
+  // Wavefront w stages token group w of K: a load is four chunks (FP8: four of
+  // 16) of 16 tokens.  A missing block's tokens are masked: any block will do.
+  constexpr int KL = F8 ? (D / 16 + 3) / 4 : (DK + 3) / 4;
+  constexpr int X = 16 / Elem<CT>::kBytes;
+  const int k_chunk = lane >> 4, k_tok = lane & 15;
   // FP8: a tile's codes on their way to LDS.
-  constexpr int FK = F8 ? (KU / 2 + 3) / 4 : 1, FV = F8 ? (VU + 3) / 4 : 1;
+  constexpr int FK = F8 ? KL : 1, FV = F8 ? (VU + 3) / 4 : 1;
   uint4 fk[FK] = {};
   uint2 fv[FV] = {};
-  // Issues the loads of the tile at t0, whose tokens' blocks are bid.
+  // Issues the loads of the tile at t0, whose groups' blocks are bid.
   auto stage = [&](auto k, int t0, int32_t bid) __attribute__((always_inline)) {
-    const int kt = t0 + k_token(lane);  // the token that this lane stages of K
-    const int kb = __shfl(bid, k_token(lane));
-    const CS* kp = kc + (int64_t)max(kb, 0) * p.k_block_stride;
-    if constexpr (!F8) {
+    auto load_k = [&](const CS* base, int at) __attribute__((always_inline)) {  // at: this lane's token in the block
 #pragma unroll
-      for (int j = 0; j < (KU + 3) / 4; ++j) {
-        const int c = 4 * j + wave;
-        if (KU % 4 != 0 && c >= KU) continue;
-        const CS* src = kp + (c * 8 * bs + (kt & (bs - 1)) * 8);
-        const bool have = kb >= 0 && (D % 16 == 0 || c * 8 < D);
-        load_to_lds(have ? (const void*)src : (const void*)&kNothing, k_image(k) + c * 64);
+      for (int j = 0; j < KL; ++j) {
+        const CS* src = base + 4 * j * X * bs + (k_chunk * bs + at) * X;
+        if constexpr (F8) {
+          fk[j] = make_uint4(0, 0, 0, 0);
+          if ((D / 16) % 4 == 0 || 4 * j + k_chunk < D / 16) fk[j] = *reinterpret_cast<const uint4*>(src);
+        } else {
+          // (The image of a head size that 16 does not divide ends in a chunk of
+          // zeros, that of one that 32 does not in half a load.)
+          const bool have = D % 32 == 0 || (4 * j + k_chunk) * 8 < D;
+          if (D % 32 == 0 || 4 * j + k_chunk < DK)
+            load_to_lds(have ? (const void*)src : (const void*)&kNothing, k_image(k) + wave * KG + 64 * j);
+        }
       }
+    };
+    const int kt = (t0 + 16 * wave) & (bs - 1);
+    if (bs >= 16) {
+      const int b = max(__builtin_amdgcn_readlane(bid, 2 * wave), 0);
+      load_k(kc + (int64_t)b * p.k_block_stride + kt * X, k_tok);
     } else {
-#pragma unroll
-      for (int j = 0; j < FK; ++j) {
-        const int c = 4 * j + wave;
-        fk[j] = make_uint4(0, 0, 0, 0);
-        if (kb >= 0 && c * 16 < D) fk[j] = *reinterpret_cast<const uint4*>(kp + (c * 16 * bs + (kt & (bs - 1)) * 16));
-      }
+      const int b = max(__shfl(bid, 2 * wave + (k_tok >> 3)), 0);
+      load_k(kc + (int64_t)b * p.k_block_stride, k_tok & 7);
     }
 #pragma unroll
     for (int j = 0; j < (VU + 3) / 4; ++j) {
       const int u0 = (4 * j + wave) * 64;
       if (VU % 4 != 0 && u0 >= 8 * DV) continue;
-      const int u = u0 + lane, tg = u / DV, d = u - tg * DV;
-      const int vb = __shfl(bid, 8 * tg);
-      const CS* src = vc + (int64_t)max(vb, 0) * p.v_block_stride + (d * bs + ((t0 + 8 * tg) & (bs - 1)));
-      const bool have = vb >= 0 && (D % 32 == 0 || d < D);
-      if constexpr (!F8) {
-        load_to_lds(have ? (const void*)src : (const void*)&kNothing, v_image(k) + u0);
+      auto load_v = [&](const CS* src, bool have) __attribute__((always_inline)) {
+        if constexpr (!F8) {
+          load_to_lds(have ? (const void*)src : (const void*)&kNothing, v_image(k) + u0);
+        } else {
+          fv[j] = make_uint2(0, 0);
+          if (have) fv[j] = *reinterpret_cast<const uint2*>(src);
+        }
+      };
+      if constexpr (DV % 64 == 0) {
+        const int tg = u0 / DV, d = u0 % DV + lane;
+        const int b = __builtin_amdgcn_readlane(bid, tg);
+        const CS* base = vc + (int64_t)b * p.v_block_stride + ((t0 + 8 * tg) & (bs - 1));
+        if (b >= 0)
+          load_v(base + d * bs, D % 64 == 0 || d < D);
+        else
+          load_v(nullptr, false);
       } else {
-        fv[j] = make_uint2(0, 0);
-        if (have) fv[j] = *reinterpret_cast<const uint2*>(src);
+        const int u = u0 + lane, tg = u / DV, d = u - tg * DV;
+        const int b = __shfl(bid, tg);
+        load_v(vc + (int64_t)max(b, 0) * p.v_block_stride + (d * bs + ((t0 + 8 * tg) & (bs - 1))), b >= 0 && d < D);
       }
     }
   };
@@ -384,10 +401,11 @@ __global__ __launch_bounds__(kExtendThreads, RS == 1 ? 2 : 1) void extend_kernel
       auto write = [&](bool special) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < FK; ++j) {
-          const int c = 4 * j + wave;
-          if (2 * c < DK) {
-            k_image(k)[2 * c * 64 + lane] = decode8<QT>(make_uint2(fk[j].x, fk[j].y), special);
-            k_image(k)[(2 * c + 1) * 64 + lane] = decode8<QT>(make_uint2(fk[j].z, fk[j].w), special);
+          const int c = 4 * j + k_chunk;
+          if ((D / 16) % 4 == 0 || c < D / 16) {
+            uint4* dst = k_image(k) + wave * KG + 2 * c * 16 + k_tok;
+            dst[0] = decode8<QT>(make_uint2(fk[j].x, fk[j].y), special);
+            dst[16] = decode8<QT>(make_uint2(fk[j].z, fk[j].w), special);
           }
         }
 #pragma unroll
@@ -409,86 +427,72 @@ __global__ __launch_bounds__(kExtendThreads, RS == 1 ? 2 : 1) void extend_kernel
     asm volatile("s_barrier" ::: "memory");
   };
 
+  // Bit r: the block of token 32 sub + 16 half + r of the tile is in the pool.
+  auto held = [&](uint32_t ok, int sub) {
+    const uint32_t g = ok >> (4 * sub + 2 * half);
+    return (g & 1u ? 0xffu : 0u) | (g & 2u ? 0xff00u : 0u);
+  };
   // The tile at t0, in image k.  whole: every row of the wavefront sees all of it.
   // CAREFUL: what a row does not see is kept out of its products.
-  auto attend = [&](auto k, auto careful, bool whole, int t0, uint64_t ok_tokens) __attribute__((always_inline)) {
+  auto attend = [&](auto k, auto careful, bool whole, int t0, uint32_t ok) __attribute__((always_inline)) {
     constexpr bool CAREFUL = decltype(careful)::value;
-    const uint4* ki = k_image(k);
-    const uint4* vi = v_image(k);
-    f32x16 s[RS][2];
+    // (K: group (col / 4) % 2 of a pair, its token 4 (col / 8) + col % 4.)
+    const uint4* ki = k_image(k) + ((col >> 2) & 1) * KG + half * 16 + 4 * (col >> 3) + (col & 3);
+    const uint4* vi = v_image(k) + 2 * half * DV + col;
+    f32x16 s[2];
 #pragma unroll
     for (int sub = 0; sub < 2; ++sub) {
 #pragma unroll
-      for (int i = 0; i < RS; ++i)
+      for (int r = 0; r < 16; ++r) s[sub][r] = 0.f;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[i][sub][r] = 0.f;
-#pragma unroll
-      for (int j = 0; j < KSTEPS; ++j) {
-        const uint4 kf = ki[(2 * j + half) * 64 + 32 * sub + col];
-#pragma unroll
-        for (int i = 0; i < RS; ++i) s[i][sub] = mma32<QT>(kf, qf[i][j], s[i][sub]);
-      }
+      for (int j = 0; j < KSTEPS; ++j) s[sub] = mma32<QT>(ki[2 * sub * KG + 32 * j], qf[j], s[sub]);
     }
     if (!whole) {
 #pragma unroll
       for (int sub = 0; sub < 2; ++sub) {
-        const int a = t0 + 32 * sub + 16 * half;  // token of register 0
+        const uint32_t sees = seen16(pos, t0 + 32 * sub + 16 * half, window, sinks) & held(ok, sub);
 #pragma unroll
-        for (int i = 0; i < RS; ++i) {
-          const uint32_t sees = seen16(pos[i], a, window, sinks) & (uint32_t)(ok_tokens >> (32 * sub + 16 * half));
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[i][sub][r] = sees >> r & 1u ? s[i][sub][r] : kNoScore;
-        }
+        for (int r = 0; r < 16; ++r) s[sub][r] = sees >> r & 1u ? s[sub][r] : kNoScore;
       }
     }
-    float ref[RS];
+    float mt = kNoScore;
 #pragma unroll
-    for (int i = 0; i < RS; ++i) {
-      float mt = kNoScore;
+    for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
-      for (int sub = 0; sub < 2; ++sub)
+      for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[sub][r]);
+    mt = fmaxf(xchg32_max(mt), m);
+    if (__any(mt * scale > m * scale + kExtendSlack || (m == kNoScore && mt != kNoScore))) {
+      const float alpha = mt == kNoScore ? 1.f : __builtin_amdgcn_exp2f((m - mt) * scale);
+      m = mt;
+      l *= alpha;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[i][sub][r]);
-      mt = fmaxf(xchg32_max(mt), m[i]);
-      if (__any(mt * scale > m[i] * scale + kExtendSlack || (m[i] == kNoScore && mt != kNoScore))) {
-        const float alpha = mt == kNoScore ? 1.f : __builtin_amdgcn_exp2f((m[i] - mt) * scale);
-        m[i] = mt;
-        l[i] *= alpha;
+      for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) o[i][dt][r] *= alpha;
-      }
-      // (A row that has seen nothing keeps a finite reference point: no inf - inf.)
-      ref[i] = m[i] == kNoScore ? 0.f : m[i] * scale;
+        for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
     }
-    uint32_t w[RS][2][8];
+    // (A row that has seen nothing keeps a finite reference point: no inf - inf.)
+    const float ref = m == kNoScore ? 0.f : m * scale;
+    uint32_t w[2][8];
     auto exponentials = [&](int sub) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < RS; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; r += 2) {
-          const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][sub][r], scale, -ref[i]));
-          const float b = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][sub][r + 1], scale, -ref[i]));
-          l[i] += a + b;
-          w[i][sub][r / 2] = pack_weights<QT>(a, b);
-        }
+      for (int r = 0; r < 16; r += 2) {
+        const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[sub][r], scale, -ref));
+        const float b = __builtin_amdgcn_exp2f(__builtin_fmaf(s[sub][r + 1], scale, -ref));
+        l += a + b;
+        w[sub][r / 2] = pack_weights<QT>(a, b);
+      }
     };
     auto v_piece = [&](int dt, int sub, int k8) {  // tokens 32 sub + 16 half + 8 k8 ..+7 of dimension 32 dt + col
-      return vi[(4 * sub + 2 * half + k8) * DV + 32 * dt + col];
+      return vi[(4 * sub + k8) * DV + 32 * dt];
     };
-    auto weights = [&](int i, int sub, int k8) {
-      return make_uint4(w[i][sub][4 * k8], w[i][sub][4 * k8 + 1], w[i][sub][4 * k8 + 2], w[i][sub][4 * k8 + 3]);
+    auto weights = [&](int sub, int k8) {
+      return make_uint4(w[sub][4 * k8], w[sub][4 * k8 + 1], w[sub][4 * k8 + 2], w[sub][4 * k8 + 3]);
     };
     auto products = [&](int sub) __attribute__((always_inline)) {
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int k8 = 0; k8 < 2; ++k8) {
-          const uint4 vf = v_piece(dt, sub, k8);
-#pragma unroll
-          for (int i = 0; i < RS; ++i) o[i][dt] = mma32<QT>(vf, weights(i, sub, k8), o[i][dt]);
-        }
+        for (int k8 = 0; k8 < 2; ++k8) o[dt] = mma32<QT>(v_piece(dt, sub, k8), weights(sub, k8), o[dt]);
     };
     exponentials(0);
     if constexpr (!CAREFUL) {
@@ -507,13 +511,10 @@ __global__ __launch_bounds__(kExtendThreads, RS == 1 ? 2 : 1) void extend_kernel
           for (int sub = 0; sub < 2; ++sub) {
             const uint32_t keep = seen16(at, t0 + 32 * sub + 16 * half, window, sinks);
             const uint4 va = keep8(v_piece(dt, sub, 0), keep), vb = keep8(v_piece(dt, sub, 1), keep >> 8);
+            f32x16 n = mma32<QT>(va, weights(sub, 0), o[dt]);
+            n = mma32<QT>(vb, weights(sub, 1), n);
 #pragma unroll
-            for (int i = 0; i < RS; ++i) {
-              f32x16 n = mma32<QT>(va, weights(i, sub, 0), o[i][dt]);
-              n = mma32<QT>(vb, weights(i, sub, 1), n);
-#pragma unroll
-              for (int r = 0; r < 16; ++r) o[i][dt][r] = pos[i] == at ? n[r] : o[i][dt][r];
-            }
+            for (int r = 0; r < 16; ++r) o[dt][r] = pos == at ? n[r] : o[dt][r];
           }
     }
     if (!CAREFUL && !whole) {
@@ -533,12 +534,13 @@ __global__ __launch_bounds__(kExtendThreads, RS == 1 ? 2 : 1) void extend_kernel
       if (__any(sum != 0.f)) s_again = 1;
     }
   };
-  auto consume = [&](auto k, auto careful, int t0, uint64_t ok_tokens) __attribute__((always_inline)) {
+  auto consume = [&](auto k, auto careful, int t0, uint32_t ok) __attribute__((always_inline)) {
     // Whether any of the wavefront's rows sees a token of the tile, and whether all see all.
     if (w_max < t0 || !(t0 < sinks || t0 + kExtendTile > w_min - window + 1)) return;
-    const bool whole = t0 + kExtendTile - 1 <= w_min && (t0 > w_max - window || t0 + kExtendTile <= sinks) &&
-                       ok_tokens == ~0ull && wr0 + WROWS <= rows;
-    attend(k, careful, whole, t0, ok_tokens);
+    // (Lanes without a row compute on zero queries and store nothing.)
+    const bool whole =
+        t0 + kExtendTile - 1 <= w_min && (t0 > w_max - window || t0 + kExtendTile <= sinks) && ok == 0xffu;
+    attend(k, careful, whole, t0, ok);
   };
 
   // Takes the tokens past the context out of the last tile's image of V (K's are
@@ -553,7 +555,7 @@ __global__ __launch_bounds__(kExtendThreads, RS == 1 ? 2 : 1) void extend_kernel
   // looked up.
   if (v0 < v1) {
     int32_t bid = load_bid(v0), next = load_bid(v0 + 1);
-    uint64_t ok_tokens = __ballot(bid >= 0);
+    uint32_t ok = (uint32_t)__ballot(bid >= 0) & 0xffu;
     stage(I0{}, tile_start(v0), bid);
     finish_stage(I0{});
     auto step = [&](auto k, int v) __attribute__((always_inline)) {
@@ -561,12 +563,12 @@ __global__ __launch_bounds__(kExtendThreads, RS == 1 ? 2 : 1) void extend_kernel
       const int t0 = tile_start(v);
       meet();  // tile v has landed, tile v - 1 has been read
       trim(k, t0);
-      const uint64_t ok_next = __ballot(next >= 0);
+      const uint32_t ok_next = (uint32_t)__ballot(next >= 0) & 0xffu;
       if (v + 1 < v1) stage(KN{}, tile_start(v + 1), next);
       next = load_bid(v + 2);
-      consume(k, std::false_type{}, t0, ok_tokens);
+      consume(k, std::false_type{}, t0, ok);
       if (v + 1 < v1) finish_stage(KN{});
-      ok_tokens = ok_next;
+      ok = ok_next;
     };
     for (int v = v0; v < v1; v += 2) {
       step(I0{}, v);
@@ -580,50 +582,46 @@ __global__ __launch_bounds__(kExtendThreads, RS == 1 ? 2 : 1) void extend_kernel
       for (int v = v0; v < v1; ++v) {
         const int t0 = tile_start(v);
         bid = load_bid(v);
-        ok_tokens = __ballot(bid >= 0);
+        ok = (uint32_t)__ballot(bid >= 0) & 0xffu;
         meet();
         stage(I0{}, t0, bid);
         finish_stage(I0{});
         meet();
         trim(I0{}, t0);
-        consume(I0{}, std::true_type{}, t0, ok_tokens);
+        consume(I0{}, std::true_type{}, t0, ok);
       }
     }
   }
 
+  l = xchg32_sum(l);
+  if (!live) return;
+  if (p.splits == 1) {
+    const float inv = l > 0.f ? p.v_scale / l : l == 0.f ? 0.f : l;  // (NaN stays NaN)
+    QS* out = static_cast<QS*>(p.out) + (qrow * p.num_heads + head) * D;
 #pragma unroll
-  for (int i = 0; i < RS; ++i) {
-    const float sum = xchg32_sum(l[i]);
-    if (!live[i]) continue;
-    if (p.splits == 1) {
-      const float inv = sum > 0.f ? p.v_scale / sum : sum == 0.f ? 0.f : sum;  // (NaN stays NaN)
-      QS* out = static_cast<QS*>(p.out) + (qrow[i] * p.num_heads + head[i]) * D;
+    for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-          const int d = 32 * dt + 2 * r + 4 * half;
-          if (D % 32 != 0 && d >= D) continue;
-          uint2 x;
-          x.x = pack2(from_f32<QT>(o[i][dt][r] * inv), from_f32<QT>(o[i][dt][r + 1] * inv));
-          x.y = pack2(from_f32<QT>(o[i][dt][r + 2] * inv), from_f32<QT>(o[i][dt][r + 3] * inv));
-          *reinterpret_cast<uint2*>(out + d) = x;
-        }
-    } else {
-      const int64_t at = (qrow[i] * p.num_heads + head[i]) * p.splits + split;
-      float* wo = p.ws_o + at * D;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-          const int d = 32 * dt + 2 * r + 4 * half;
-          if (D % 32 != 0 && d >= D) continue;
-          *reinterpret_cast<float4*>(wo + d) =
-              make_float4(o[i][dt][r], o[i][dt][r + 1], o[i][dt][r + 2], o[i][dt][r + 3]);
-        }
-      if (half == 0) *reinterpret_cast<float2*>(p.ws_ml + at * 2) = make_float2(m[i] * scale, sum);
-    }
+      for (int r = 0; r < 16; r += 4) {
+        const int d = 32 * dt + 2 * r + 4 * half;
+        if (D % 32 != 0 && d >= D) continue;
+        uint2 x;
+        x.x = pack2(from_f32<QT>(o[dt][r] * inv), from_f32<QT>(o[dt][r + 1] * inv));
+        x.y = pack2(from_f32<QT>(o[dt][r + 2] * inv), from_f32<QT>(o[dt][r + 3] * inv));
+        *reinterpret_cast<uint2*>(out + d) = x;
+      }
+    return;
   }
+  const int64_t at = (qrow * p.num_heads + head) * p.splits + split;
+  float* wo = p.ws_o + at * D;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int d = 32 * dt + 2 * r + 4 * half;
+      if (D % 32 != 0 && d >= D) continue;
+      *reinterpret_cast<float4*>(wo + d) = make_float4(o[dt][r], o[dt][r + 1], o[dt][r + 2], o[dt][r + 3]);
+    }
+  if (half == 0) *reinterpret_cast<float2*>(p.ws_ml + at * 2) = make_float2(m * scale, l);
 }
 
 // The outputs of a call whose row tiles are split: one wavefront per query row.
@@ -658,17 +656,25 @@ __global__ __launch_bounds__(256) void extend_merge_kernel(ExtendParams p) {
 }
 
 // ---------------------------------------------------------------------------
-// One new token per sequence: one workgroup per (sequence, up to 16 heads of a
-// KV head, split), four wavefronts that take tiles of 32 tokens in turn, K and
-// V from the cache straight into the matrix units' registers.
+// Few query rows per sequence (decodes, drafted tokens): one workgroup per
+// (sequence, 16 rows of a KV head, part of the length), four wavefronts that take
+// tiles of 32 tokens in turn, K and V from the cache straight into the matrix
+// units' registers.
 //
 // Row i of score product u (of two) is token 8 (i / 4) + 4 u + i % 4, so that
 // the registers of both products in lane group g are tokens 8 g ..+7.
+//
+// ONE: a sequence has one token, whose heads all see the same keys.
+//
+// Bound: HBM reads of K and V.  128 sequences, window 4000, fp16: 141 us, 5.3 TB/s;
+// 64 sequences, window 1024, FP8: 32 us, 4.2 TB/s; one sequence, window 4096:
+// 11 us, of which the reads take 4 and the launch, the chain context length ->
+// block -> tile, and the merge of the parts the rest.
 // ---------------------------------------------------------------------------
 constexpr int kWindowTile = 32;
 
-template <class QT, class CT, int D>
-__global__ __launch_bounds__(256, 2) void window_decode_kernel(ExtendParams p) {
+template <class QT, class CT, int D, bool ONE>
+__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void extend_few_kernel(ExtendParams p) {
   using QS = typename Elem<QT>::storage;
   using CS = typename Elem<CT>::storage;
   constexpr bool F8 = std::is_same<CT, FP8>::value;
@@ -685,50 +691,69 @@ __global__ __launch_bounds__(256, 2) void window_decode_kernel(ExtendParams p) {
   const int unit = blockIdx.x % p.units;
   const int seq = blockIdx.x / p.units;
   const int split = blockIdx.y;
-  const int kvh = unit / p.slices;
-  const int g0 = (unit - kvh * p.slices) * 16;
-  const int nh = min(16, p.group - g0), h0 = kvh * p.group + g0;
+  const int kvh = unit / p.slices, slice = unit - kvh * p.slices;
+  const int group = p.group, h0 = kvh * group;
   if (seq == p.num_seqs) {
     // Rows behind the last sequence become zeros.
     const int last = min(max(p.query_start_loc[p.num_seqs], 0), p.num_tokens);
-    if (split == 0) zero_tokens<QT, 256>(p, D, last, p.num_tokens, h0, nh);
+    if (split == 0 && slice == 0) zero_tokens<QT, 256>(p, D, last, p.num_tokens, h0, group);
     return;
   }
   const ExtendSeq q = extend_seq(p, seq);
   if (q.count == 0) return;
   if (q.ctx == 0) {
-    if (split == 0) zero_tokens<QT, 256>(p, D, q.start, q.start + q.count, h0, nh);
+    if (split == 0 && slice == 0) zero_tokens<QT, 256>(p, D, q.start, q.start + q.count, h0, group);
     return;
   }
-  const int pos = q.ctx - 1;
-  const int lo = p.window > 0 ? max(0, q.ctx - p.window) : 0;
-  const int sinks = p.window > 0 ? min(p.sinks, lo) : 0;
-  const int lead = (sinks + kWindowTile - 1) / kWindowTile;
+  // Row row0 + c, c < nr, is head (row0 + c) % group of token (row0 + c) / group;
+  // this lane's is c = col.
+  const int row0 = 16 * slice, nr = min(16, q.count * group - row0);
+  if (nr <= 0) return;
+  const int first_pos = q.ctx - q.count;
+  const int pmin = first_pos + row0 / group, pmax = first_pos + (row0 + nr - 1) / group;  // (uniform)
+  const bool live = col < nr;
+  const int mine = row0 + min(col, nr - 1), token = mine / group;
+  const int pos = first_pos + token;
+  auto row_of = [&](int c) {  // of the output and of the states
+    const int tok = (row0 + c) / group;
+    return ((int64_t)q.start + tok) * p.num_heads + h0 + (row0 + c - tok * group);
+  };
+  if (pmax < 0) {
+    if (split == 0)
+      for (int i = tid; i < nr * D; i += 256) static_cast<QS*>(p.out)[row_of(i / D) * D + i % D] = 0;
+    return;
+  }
+  const int window = p.window > 0 ? p.window : p.max_seq_len;
+  const int sinks = p.window > 0 ? p.sinks : 0;
+  const int lo = max(0, max(pmin, 0) - window + 1);
+  const int lead = (min(sinks, lo) + kWindowTile - 1) / kWindowTile;
   const int base_tile = max(lo / kWindowTile, lead);
-  const int ntiles = lead + pos / kWindowTile + 1 - base_tile;
+  const int ntiles = lead + max(0, pmax / kWindowTile + 1 - base_tile);
   // Parts of one length for all sequences, that of the longest cut in p.splits.
   const int per = p.part_tiles;
-  const int parts = (ntiles + per - 1) / per;
+  const int parts = max((ntiles + per - 1) / per, 1);
   const int v0 = split * per, v1 = min(v0 + per, ntiles);
   if (split >= parts) return;
 
   uint4 qf[KSTEPS];
   {
-    const QS* src = static_cast<const QS*>(p.q) + q.start * p.q_stride + (int64_t)(h0 + min(col, nh - 1)) * D;
+    const QS* src =
+        static_cast<const QS*>(p.q) + (q.start + token) * p.q_stride + (int64_t)(h0 + (mine - token * group)) * D;
 #pragma unroll
     for (int j = 0; j < KSTEPS; ++j) {
       const int d = F8 ? 64 * (j / 2) + 16 * g + 8 * (j & 1) : 32 * j + 8 * g;
-      qf[j] = col < nh && d < D ? *reinterpret_cast<const uint4*>(src + d) : make_uint4(0, 0, 0, 0);
+      qf[j] = live && d < D ? *reinterpret_cast<const uint4*>(src + d) : make_uint4(0, 0, 0, 0);
     }
   }
-  f32x4 o[DT];
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt) o[dt] = {0.f, 0.f, 0.f, 0.f};
-  float m = kNoScore, l = 0.f;
   const int shift = p.block_shift, bs = 1 << shift;
   const int32_t* table = p.block_tables + (int64_t)seq * p.max_blocks_per_seq;
   const CS* kc = static_cast<const CS*>(p.k_cache) + (int64_t)kvh * p.k_head_stride;
   const CS* vc = static_cast<const CS*>(p.v_cache) + (int64_t)kvh * p.v_head_stride;
+
+  f32x4 o[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) o[dt] = {0.f, 0.f, 0.f, 0.f};
+  float m = kNoScore, l = 0.f;
 
   // A tile's blocks (of this lane's K row and of its V pieces), and its K and V.
   struct Blocks {
@@ -796,14 +821,8 @@ __global__ __launch_bounds__(256, 2) void window_decode_kernel(ExtendParams p) {
         }
       }
     }
-    // Bit i: token tv + i is seen (by every row alike).
-    uint32_t sees = 0xffu;
-    if (!(tv >= lo && tv + 8 <= q.ctx && b.v >= 0)) {
-      sees = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (b.v >= 0 && tv + i < q.ctx && (tv + i >= lo || tv + i < sinks)) sees |= 1u << i;
-    }
+    // Bit r: this lane's row sees token tv + r.
+    const uint32_t sees = b.v >= 0 ? seen16(pos, tv, window, sinks) & 0xffu : 0u;
     float mt = m;
 #pragma unroll
     for (int u = 0; u < 2; ++u)
@@ -827,8 +846,12 @@ __global__ __launch_bounds__(256, 2) void window_decode_kernel(ExtendParams p) {
         w[2 * u + r / 2] = pack_weights<QT>(a, c);
       }
     const uint4 wf = make_uint4(w[0], w[1], w[2], w[3]);
-    // What a token that is not seen holds must not matter.
-    const bool hidden = __any(sees != 0xffu);
+    // What a token that a row does not see holds must not matter (a weight of 0
+    // times inf or NaN is NaN): it is taken out of V, and where the rows see
+    // different tokens, at the few tiles where a row's keys begin or end, one query
+    // position at a time; the others' rows keep their sums.
+    const int t0 = tile_start(v);
+    const bool one = ONE || (t0 + kWindowTile - 1 <= pmin && (t0 > pmax - window || t0 + kWindowTile <= sinks));
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       uint4 y;
@@ -836,10 +859,17 @@ __global__ __launch_bounds__(256, 2) void window_decode_kernel(ExtendParams p) {
         y = decode8<QT>(x.v[dt], special);
       else
         y = x.v[dt];
-      if (hidden) y = keep8(y, sees);
 #pragma unroll
       for (int r = 0; r < 4; ++r) o[dt][r] *= alpha;
-      o[dt] = Mma<QT>::k32(y, wf, o[dt]);
+      if (one) {
+        o[dt] = Mma<QT>::k32(keep8(y, sees), wf, o[dt]);
+        continue;
+      }
+      for (int at = pmin; at <= pmax; ++at) {
+        const f32x4 n = Mma<QT>::k32(keep8(y, b.v >= 0 ? seen16(at, tv, window, sinks) : 0u), wf, o[dt]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[dt][r] = pos == at ? n[r] : o[dt][r];
+      }
     }
   };
   // Each wavefront takes every fourth tile.  While one is attended, the next one
@@ -872,34 +902,38 @@ __global__ __launch_bounds__(256, 2) void window_decode_kernel(ExtendParams p) {
     }
   }
 
-  // The wavefronts' states: column col is head h0 + col.
+  // The wavefronts' states: column col is row row0 + col.
   l = column_sum(l);
   if (g == 0) s_m[wave][col] = m, s_l[wave][col] = l;
   __syncthreads();
   float M = kNoScore, L = 0.f;
 #pragma unroll
   for (int w = 0; w < 4; ++w) M = fmaxf(M, s_m[w][col]);
-  const float ref = M == kNoScore ? 0.f : M;
+  {
+    const float ref = M == kNoScore ? 0.f : M;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) L += s_l[w][col] * __builtin_amdgcn_exp2f(s_m[w][col] - ref);
-  const float f = __builtin_amdgcn_exp2f(m - ref);
+    for (int w = 0; w < 4; ++w) L += s_l[w][col] * __builtin_amdgcn_exp2f(s_m[w][col] - ref);
+    const float f = __builtin_amdgcn_exp2f(m - ref);
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
+    for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) s_o[wave][4 * dt + r][lane] = o[dt][r] * f;
+      for (int r = 0; r < 4; ++r) s_o[wave][dt * 4 + r][lane] = o[dt][r] * f;
+  }
   __syncthreads();
   // Wavefront w sums the 16-dimension tiles w, w + 4, ...
   const float inv = L > 0.f ? p.v_scale / L : L == 0.f ? 0.f : L;
-  const int64_t row0 = (int64_t)q.start * p.num_heads + h0, row = row0 + col;
+  const int64_t row = row_of(min(col, nr - 1));
 #pragma unroll
   for (int k = 0; k < (DT + 3) / 4; ++k) {
     const int dt = 4 * k + wave;
     const int d = 16 * dt + 4 * g;
-    if (dt >= DT || col >= nh || d >= D) continue;
+    if (dt >= DT || !live || d >= D) continue;
     float x[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      x[r] = s_o[0][4 * dt + r][lane] + s_o[1][4 * dt + r][lane] + s_o[2][4 * dt + r][lane] + s_o[3][4 * dt + r][lane];
+    for (int r = 0; r < 4; ++r) {
+      const int at = dt * 4 + r;
+      x[r] = s_o[0][at][lane] + s_o[1][at][lane] + s_o[2][at][lane] + s_o[3][at][lane];
+    }
     if (parts == 1) {
       uint2 y;
       y.x = pack2(from_f32<QT>(x[0] * inv), from_f32<QT>(x[1] * inv));
@@ -911,8 +945,8 @@ __global__ __launch_bounds__(256, 2) void window_decode_kernel(ExtendParams p) {
       store_agent(to + 2, x[2], x[3]);
     }
   }
+  if (parts > 1 && wave == 0 && g == 0 && live) store_agent(p.ws_ml + (row * p.splits + split) * 2, M, L);
   if (parts == 1) return;
-  if (wave == 0 && g == 0 && col < nh) store_agent(p.ws_ml + (row * p.splits + split) * 2, M, L);
   // The workgroup whose part is the last to arrive merges all, in their order.
   wait_agent_stores();
   __syncthreads();
@@ -920,17 +954,18 @@ __global__ __launch_bounds__(256, 2) void window_decode_kernel(ExtendParams p) {
   __syncthreads();
   if (!s_last) return;
   // (The states lie in what was the wavefronts' outputs.)
-  static_assert(sizeof(s_o) >= 16 * kWindowMaxSplits * sizeof(float2), "room for every state");
+  static_assert(sizeof(s_o) >= 16 * kFewMaxSplits * sizeof(float2), "room for every state");
   float2* s_ml = reinterpret_cast<float2*>(&s_o[0][0][0]);
-  for (int i = tid; i < nh * parts; i += 256) {
-    const int h = i / parts;
-    s_ml[i] = load_agent(p.ws_ml + ((row0 + h) * p.splits + (i - h * parts)) * 2);
+  for (int i = tid; i < nr * parts; i += 256) {
+    const int c = i / parts;
+    s_ml[i] = load_agent(p.ws_ml + (row_of(c) * p.splits + (i - c * parts)) * 2);
   }
   __syncthreads();
-  for (int i = tid; i < nh * (D / 2); i += 256) {
-    const int h = i / (D / 2), d = 2 * (i - h * (D / 2));
-    const float2* state = s_ml + h * parts;
-    const float* from = p.ws_o + (row0 + h) * p.splits * D + d;
+  for (int i = tid; i < nr * (D / 2); i += 256) {
+    const int c = i / (D / 2), d = 2 * (i - c * (D / 2));
+    const int64_t r = row_of(c);
+    const float2* state = s_ml + c * parts;
+    const float* from = p.ws_o + r * p.splits * D + d;
     float mm = kNoScore;
     for (int s = 0; s < parts; ++s) mm = fmaxf(mm, state[s].x);
     const float rf = mm == kNoScore ? 0.f : mm;
@@ -950,21 +985,24 @@ __global__ __launch_bounds__(256, 2) void window_decode_kernel(ExtendParams p) {
       }
     }
     const float iv = ll > 0.f ? p.v_scale / ll : ll == 0.f ? 0.f : ll;
-    *reinterpret_cast<uint32_t*>(static_cast<QS*>(p.out) + (row0 + h) * D + d) =
+    *reinterpret_cast<uint32_t*>(static_cast<QS*>(p.out) + r * D + d) =
         pack2(from_f32<QT>(x * iv), from_f32<QT>(y * iv));
   }
 }
 
 template <class QT, class CT, int D>
 hipError_t launch_extend_d(const ExtendParams& p, hipStream_t stream) {
-  if (p.max_query_len == 1) {
+  if (p.part_tiles > 0) {
     const int seqs = p.num_seqs + (p.query_start_loc != nullptr ? 1 : 0);
-    hipLaunchKernelGGL((window_decode_kernel<QT, CT, D>), dim3((unsigned)(seqs * p.units), (unsigned)p.splits),
-                       dim3(256), 0, stream, p);
+    const dim3 grid((unsigned)(seqs * p.units), (unsigned)p.splits);
+    if (p.max_query_len == 1)
+      hipLaunchKernelGGL((extend_few_kernel<QT, CT, D, true>), grid, dim3(256), 0, stream, p);
+    else
+      hipLaunchKernelGGL((extend_few_kernel<QT, CT, D, false>), grid, dim3(256), 0, stream, p);
     return hipGetLastError();
   }
   const int64_t items = extend_items(p.num_tokens, p.num_seqs, p.group);
-  hipLaunchKernelGGL((extend_kernel<QT, CT, D, 1>), dim3((unsigned)(items * p.num_kv_heads), (unsigned)p.splits),
+  hipLaunchKernelGGL((extend_kernel<QT, CT, D>), dim3((unsigned)(items * p.num_kv_heads), (unsigned)p.splits),
                      dim3(kExtendThreads), 0, stream, p);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.splits == 1) return e;

@@ -583,38 +583,41 @@ int norm_rope_launch(const pkv::NormRopeParams& p, void* stream) {
 
 constexpr int32_t kExtendMaxSeq = 1 << 30;
 
-// Most 32-token tiles of keys that one sequence's new token attends to.
-int64_t window_tiles(int64_t max_seq_len, int64_t window, int64_t num_sinks) {
-  if (window == 0 || window >= max_seq_len) return ceil_div(max_seq_len, 32);
-  return std::min(ceil_div(max_seq_len, 32), ceil_div(window - 1, 32) + 1 + ceil_div(num_sinks, 32));
-}
-
-// Parts along the keys: of a decode's (sequence, KV head) items, part_tiles (the
-// longest item cut evenly, no part shorter than kPartTiles) and the most parts of
-// an item; of row tiles, as many as make the launch fill the chip.  A decode is
-// cut to two workgroups per CU, which is what the registers let stay resident:
-// four a CU measured 39.3 against 31.8 us (64 sequences, window 1024, FP8) and
-// 155 against 148 us (128 sequences, window 4000); parts of 4 tiles 13.9 against
-// 12.0 us, of 16 tiles 12.5 (one sequence, window 4096).
-constexpr int64_t kPartTiles = 8, kDecodeGroups = 512;
-struct ExtendSplit {
-  int64_t splits, part_tiles;
+// How a call is cut.  At most kFewRows rows per KV head and sequence, or single
+// tokens: workgroups of 16 rows, each (sequence, KV head, slice)'s keys in parts of
+// part_tiles 32-token tiles, the longest one's cut evenly and no part shorter than
+// kPartTiles.  Otherwise (part_tiles 0) row tiles, their keys in as many parts as
+// make the launch fill the chip.
+//
+// Few rows against row tiles (4 heads per KV head, bf16, 1 sequence of 16000, 16 and
+// 64 sequences of up to 4000 tokens): 8 rows 27/38/128 against 34/58/179 us; 20 rows,
+// two slices that read the keys twice, 38/61/182 against 31/53/170 us.  32 rows in
+// one slice do not help either (one workgroup per CU): 55/63/167 us.
+//
+// Few rows are cut to two workgroups per CU, which is what the registers let stay
+// resident: four a CU measured 39.3 against 31.8 us (64 sequences, window 1024,
+// FP8) and 155 against 148 us (128 sequences, window 4000); parts of 4 tiles 13.9
+// against 12.0 us, of 16 tiles 12.5 (one sequence, window 4096).
+constexpr int64_t kFewRows = 16, kPartTiles = 8, kFewGroups = 512;
+struct ExtendCut {
+  int64_t splits, part_tiles, slices;
 };
-ExtendSplit extend_split(int64_t num_tokens, int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads,
-                         int64_t max_seq_len, int64_t max_query_len, int64_t window, int64_t num_sinks) {
+ExtendCut extend_cut(int64_t num_tokens, int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads,
+                     int64_t max_seq_len, int64_t max_query_len, int64_t window, int64_t num_sinks) {
   const int64_t group = num_heads / num_kv_heads;
-  if (max_query_len == 1) {
-    const int64_t tiles = window_tiles(max_seq_len, window, num_sinks);
-    const int64_t items = num_seqs * num_kv_heads * ((group + 15) / 16);
-    if (items == 0 || items * 4 > pkv::kCounterBytes) return {1, tiles};
-    const int64_t most = std::min<int64_t>(ceil_div(kDecodeGroups, items), pkv::kWindowMaxSplits);
+  const int64_t span = window > 0 ? std::min(max_seq_len, window + max_query_len + num_sinks) : max_seq_len;
+  if (max_query_len == 1 || max_query_len * group <= kFewRows) {
+    const int64_t slices = ceil_div(max_query_len * group, 16), items = num_seqs * num_kv_heads * slices;
+    // (The window and the sinks each end inside a tile.)
+    const int64_t tiles = span == max_seq_len ? ceil_div(span, 32) : ceil_div(span, 32) + 2;
+    if (items == 0 || items * 4 > pkv::kCounterBytes) return {1, tiles, slices};
+    const int64_t most = std::min<int64_t>(ceil_div(kFewGroups, items), pkv::kFewMaxSplits);
     const int64_t part = std::max(ceil_div(tiles, most), kPartTiles);
-    return {ceil_div(tiles, part), part};
+    return {ceil_div(tiles, part), part, slices};
   }
-  const int64_t span = window > 0 ? std::min(max_seq_len, window + num_sinks + max_query_len) : max_seq_len;
-  const int64_t items = (ceil_div(num_tokens * group, pkv::kExtendRows)) * num_kv_heads;
-  if (items == 0) return {1, 0};
-  return {std::max<int64_t>(1, std::min(512 / items, ceil_div(span, 64 * 8))), 0};
+  const int64_t items = ceil_div(num_tokens * group, pkv::kExtendRows) * num_kv_heads;
+  if (items == 0) return {1, 0, 0};
+  return {std::max<int64_t>(1, std::min(512 / items, ceil_div(span, 64 * 8))), 0, 0};
 }
 
 struct ExtendWorkspace {
@@ -796,8 +799,8 @@ size_t pkv_paged_attention_extend_workspace_size(int32_t num_tokens, int32_t num
       head_size <= 0 || max_seq_len <= 0 || max_seq_len > kExtendMaxSeq || max_query_len <= 0 || window < 0 ||
       num_sinks < 0)
     return 0;
-  const int64_t splits = extend_split(num_tokens, num_seqs, num_heads, num_kv_heads, max_seq_len, max_query_len,
-                                      window, num_sinks).splits;
+  const int64_t splits = extend_cut(num_tokens, num_seqs, num_heads, num_kv_heads, max_seq_len, max_query_len,
+                                    window, num_sinks).splits;
   return extend_workspace(num_tokens, num_heads, head_size, splits).total;
 }
 
@@ -832,11 +835,11 @@ int pkv_paged_attention_extend(void* out, const void* query, const void* key_cac
   if (fp8 && !(std::isfinite(k_scale) && std::isfinite(v_scale) && k_scale != 0.f && v_scale != 0.f))
     return fail(PKV_ERR_INVALID, "k_scale and v_scale must be finite and nonzero for FP8 caches");
   if (num_blocks <= 0) return fail(PKV_ERR_INVALID, "num_blocks must be positive");
-  const ExtendSplit cut = extend_split(num_tokens, num_seqs, num_heads, num_kv_heads, max_seq_len, max_query_len,
-                                       window, num_sinks);
+  const ExtendCut cut = extend_cut(num_tokens, num_seqs, num_heads, num_kv_heads, max_seq_len, max_query_len,
+                                   window, num_sinks);
   const int64_t splits = cut.splits;
-  const int32_t group = num_heads / num_kv_heads, slices = (group + 15) / 16;
-  const int64_t groups = max_query_len == 1 ? ((int64_t)num_seqs + 1) * num_kv_heads * slices
+  const int32_t group = num_heads / num_kv_heads;
+  const int64_t groups = cut.part_tiles > 0 ? ((int64_t)num_seqs + 1) * num_kv_heads * cut.slices
                                             : pkv::extend_items(num_tokens, num_seqs, group) * num_kv_heads;
   // (HIP bounds a launch to 2^32 work-items; rows of a sequence are counted in 32 bits.)
   if (groups * splits * 256 >= ((int64_t)1 << 32) || (int64_t)num_tokens * num_heads >= ((int64_t)1 << 30))
@@ -881,8 +884,8 @@ int pkv_paged_attention_extend(void* out, const void* query, const void* key_cac
   p.num_heads = num_heads;
   p.num_kv_heads = num_kv_heads;
   p.group = group;
-  p.slices = slices;
-  p.units = num_kv_heads * slices;
+  p.slices = (int32_t)cut.slices;
+  p.units = (int32_t)(num_kv_heads * cut.slices);
   p.max_blocks_per_seq = max_num_blocks_per_seq;
   p.max_seq_len = max_seq_len;
   p.max_query_len = max_query_len;

@@ -289,7 +289,7 @@ struct ExtendParams {
   const int32_t* query_start_loc;  // [num_seqs + 1], null: one token per sequence
   float* ws_ml;                    // [num_tokens, Hq, splits, 2]: (max, sum) per split, log2 domain
   float* ws_o;                     // [num_tokens, Hq, splits, D]: outputs before the division by the sum
-  int32_t* counters;               // one token per sequence: arrivals per (sequence, unit), zero between launches
+  int32_t* counters;               // few rows: arrivals per (sequence, unit), zero between launches
   int64_t num_blocks;
   int64_t q_stride;
   int64_t k_block_stride, k_head_stride;
@@ -297,17 +297,18 @@ struct ExtendParams {
   float scale_log2;                // scale * log2(e) (FP8 caches: times k_scale)
   float v_scale;                   // 1 but for FP8 caches
   int32_t num_tokens, num_seqs, num_heads, num_kv_heads;
-  int32_t group, slices, units;    // as in DecodeParams
+  int32_t group;                   // num_heads / num_kv_heads
+  int32_t slices, units;           // few rows: 16-row slices per KV head, num_kv_heads * slices
   int32_t max_blocks_per_seq, max_seq_len, max_query_len;
   int32_t window, sinks;           // window 0: the whole context
   int32_t block_shift;             // log2(block_size)
   int32_t splits;                  // the most parts of a row
-  int32_t part_tiles;              // one token per sequence: 32-token tiles of a part
+  int32_t part_tiles;              // few rows: 32-token tiles of a part; 0: row tiles
 };
 // Row tiles (of kExtendRows) that num_tokens query tokens of num_seqs
 // sequences can make, and at least one more.
 constexpr int kExtendRows = 128;
-constexpr int kWindowMaxSplits = 64;  // parts of a decode's length (their states meet in LDS)
+constexpr int kFewMaxSplits = 64;  // parts of few rows' lengths (their states meet in LDS)
 constexpr int64_t extend_items(int64_t num_tokens, int64_t num_seqs, int64_t group) {
   return (num_tokens * group + kExtendRows - 1) / kExtendRows + std::min(num_seqs, num_tokens) + 1;
 }

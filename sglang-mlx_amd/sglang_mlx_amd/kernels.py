@@ -282,15 +282,17 @@ def paged_attention_extend(
             n query rows of a sequence are its context's last n tokens
         query_start_loc: [num_seqs + 1], each sequence's first query row, and
             the number of rows; output rows behind it are zero
-        max_query_len: at least the most query rows of one sequence
+        max_query_len: at least the most query rows of one sequence; the
+            closer, the better the kernel fits (one for a few rows per sequence,
+            one for many)
         window, num_sinks: with a window > 0 a query sees the ``window`` last
             tokens up to its own, and the context's first ``num_sinks``
         The others as ``paged_attention_window``.
 
     Returns:
         [num_tokens, num_heads, head_size]; a row that sees no token (context 0
-        or beyond max_seq_len, more rows than max_query_len or than tokens) is
-        zero.
+        or beyond max_seq_len, a sequence of more than max_query_len rows, rows
+        before the context's first token) is zero.
     """
     return _ext.paged_attention_extend(query, key_cache, value_cache, block_tables, context_lens, query_start_loc,
                                        num_kv_heads, scale, block_size, max_seq_len, max_query_len, window, num_sinks,

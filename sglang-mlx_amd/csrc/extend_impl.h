@@ -183,7 +183,7 @@ __device__ __forceinline__ void load_to_lds(const void* src, uint4* dst) {
 }
 
 template <class QT, class CT, int D>
-__global__ __launch_bounds__(kExtendThreads, 2) void extend_kernel(ExtendParams p) {
+__global__ __launch_bounds__(kExtendThreads, D <= 128 ? 2 : 1) void extend_kernel(ExtendParams p) {
   using QS = typename Elem<QT>::storage;
   using CS = typename Elem<CT>::storage;
   constexpr bool F8 = std::is_same<CT, FP8>::value;

@@ -894,6 +894,11 @@ int pkv_paged_attention_extend(void* out, const void* query, const void* key_cac
   p.block_shift = block_size == 8 ? 3 : block_size == 16 ? 4 : 5;
   p.splits = (int32_t)splits;
   p.part_tiles = (int32_t)cut.part_tiles;
+  // Split row tiles take two launches, between which no other call's may come: one
+  // from another thread on the same stream would have the same workspace.
+  static std::mutex pair;
+  std::unique_lock<std::mutex> both(pair, std::defer_lock);
+  if (p.part_tiles == 0 && p.splits > 1) both.lock();
   clear_pending_error();
   const hipStream_t s = static_cast<hipStream_t>(stream);
   hipError_t e;

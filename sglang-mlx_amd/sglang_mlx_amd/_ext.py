@@ -101,8 +101,9 @@ def _done(result) -> bool:
 # Decode scratch, one buffer per (device, stream).  Its first
 # PKV_COUNTER_BYTES are arrival counters that start at zero (cleared when the
 # buffer is made) and that every call leaves at zero; the rest is read only
-# where the same launch wrote it.  So calls ordered on one stream share it
-# whatever their shapes.
+# where the same launch wrote it, or the launch before it, where the library
+# lets no other call come between the two.  So calls ordered on one stream share
+# it whatever their shapes.
 #
 # HIP graphs: a call captured on a stream that has its buffer already uses that
 # buffer, so an outgrown buffer is kept for the graphs that hold its address
@@ -491,6 +492,8 @@ def build_step_tables(request_blocks, rows, context_lens, query_lens, new_blocks
         raise ValueError("max_blocks and block_size must be positive")
     if num_tokens < 0:
         raise ValueError("num_tokens must be non-negative")
+    if max(num_tokens, block_size) >= 1 << 31:
+        raise ValueError("num_tokens and block_size must be below 2^31")
     R, W = request_blocks.shape
     B = rows.shape[0]
     if B > _lib.PKV_MAX_STEP_SEQS:
@@ -712,6 +715,9 @@ def _new_token_attention(op, query, key_cache, value_cache, block_tables, contex
         raise ValueError(f"Unsupported query/cache dtype pair for paged_attention: {query.dtype}/{key_cache.dtype}")
     if max_seq_len > 1 << 30:
         raise ValueError("max_seq_len must be at most 2^30")
+    # (Beyond the context, larger ones see no more; the C entry takes 32 bits.)
+    window, num_sinks = min(window, max_seq_len), min(num_sinks, max_seq_len)
+    max_query_len = min(max_query_len, 2**31 - 1)
     if fp8 and not all(math.isfinite(v) and v != 0.0 for v in (k_scale, v_scale)):
         raise ValueError("k_scale and v_scale must be finite and nonzero for FP8 caches")
     _check_index(block_tables)

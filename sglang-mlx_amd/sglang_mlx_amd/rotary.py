@@ -64,6 +64,8 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | N
     if kind == "linear":
         return freq / factor, 1.0
     if kind == "yarn":
+        if base <= 1:
+            raise ValueError("rotary scaling 'yarn' needs a base above 1")
         length = _number(rule, "original_max_position")
 
         def pair_of(turns):  # the (real) pair index that makes so many turns within `length` tokens

@@ -9,6 +9,8 @@ sum of weights take relatively, twice; the exponential, sums over T keys and the
 splits' factors add at most (T + 64) 2^-23 sum p |v|.  The expected values
 themselves are exact to 2^-50."""
 
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -365,3 +367,34 @@ def test_captured_replays():
     graphs[0].replay()
     torch.cuda.synchronize()
     a.check(outs[0], 2000, 4)
+
+
+def test_two_threads_on_one_stream():
+    # Both calls split their row tiles and use the stream's one scratch.
+    batches = [Batch(24, [5000], [40], (8, 2)), Batch(25, [4000, 1000], [33, 17], (8, 2))]
+    want = [b.extend() for b in batches]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def run(i):
+        for _ in range(100):
+            got[i].append(batches[i].extend())
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert [len(g) for g in got] == [100, 100]
+    assert all(o.equal(w) for g, w in zip(got, want) for o in g)
+
+
+def test_windows_beyond_32_bits_see_the_whole_context():
+    b = Batch(26, [300, 20], [1, 1], (8, 2))
+    whole = b.window(300)
+    assert b.window((1 << 32) + 5).equal(whole) and b.window(10 ** 20, 10 ** 20).equal(whole)
+    e = Batch(27, [300, 90], [33, 9], (8, 2))
+    whole = e.extend()
+    for kw in (dict(window=(1 << 32) + 5), dict(window=300, sinks=(1 << 32) + 1), dict(max_query_len=(1 << 32) + 2)):
+        assert e.extend(**kw).equal(whole)

@@ -35,6 +35,8 @@ def tables_args(**kw):
     (dict(request_blocks=torch.zeros(4, 0, dtype=I32)), ValueError, "must be positive"),
     (dict(block_size=0), ValueError, "must be positive"),
     (dict(num_tokens=-1), ValueError, "non-negative"),
+    (dict(num_tokens=(1 << 32) + 4), ValueError, "below 2"),
+    (dict(block_size=(1 << 32) + 16), ValueError, "below 2"),
     (dict(query_lens=torch.zeros(2)), ValueError, "integer dtype"),
     (dict(rows=[0, 1]), TypeError, "Expected torch.Tensor"),
     (dict(rows=torch.zeros(4097, dtype=I32), context_lens=torch.zeros(4097, dtype=I32),
@@ -311,6 +313,7 @@ def test_rotary_scalings():
     ((4, 8, 1e4, {"type": "other"}), "Unknown rotary scaling"), ((4, 8, 1e4, {"type": "linear"}), "needs 'factor'"),
     ((4, 8, 1e4, {"type": "linear", "factor": -1}), "must be positive"),
     ((4, 2, 1e4, {"type": "ntk", "factor": 2}), "above 2"),
+    ((4, 8, 1.0, {"type": "yarn", "factor": 2, "original_max_position": 8}), "above 1"),
     ((4, 8, 1e4, {"type": "llama3", "factor": 2, "low_freq_factor": 4, "high_freq_factor": 1,
                   "original_max_position": 8}), "must exceed"),
 ])

@@ -157,8 +157,9 @@ __device__ __forceinline__ void zero_tokens(const ExtendParams& p, int D, int64_
 // 8192 new tokens on 8192, 32 heads of 128, bf16, take 1.75 ms, 943 TFLOP/s of the
 // 1381 that a large matrix product reaches.  Matrix units busy 42 % and vector units
 // 50 % of the time; 32-token tiles in four stages with the softmax of one beside the
-// products of the next came to 952 TFLOP/s.  Cuts of the workgroup: 128 rows let two
-// workgroups share a CU, so that one computes while the other waits.
+// products of the next came to 952 TFLOP/s.  128 rows let two workgroups share a CU
+// (three at head sizes up to 64, none above 128), so that one computes while another
+// waits.
 // ---------------------------------------------------------------------------
 constexpr int kExtendTile = 64;
 constexpr int kExtendThreads = 256;
@@ -183,7 +184,7 @@ __device__ __forceinline__ void load_to_lds(const void* src, uint4* dst) {
 }
 
 template <class QT, class CT, int D>
-__global__ __launch_bounds__(kExtendThreads, D <= 128 ? 2 : 1) void extend_kernel(ExtendParams p) {
+__global__ __launch_bounds__(kExtendThreads, D <= 64 ? 3 : D <= 128 ? 2 : 1) void extend_kernel(ExtendParams p) {
   using QS = typename Elem<QT>::storage;
   using CS = typename Elem<CT>::storage;
   constexpr bool F8 = std::is_same<CT, FP8>::value;
@@ -1002,8 +1003,15 @@ hipError_t launch_extend_d(const ExtendParams& p, hipStream_t stream) {
     return hipGetLastError();
   }
   const int64_t items = extend_items(p.num_tokens, p.num_seqs, p.group);
+  // Head sizes up to 64 let three workgroups share a CU, which hides more of a tile's
+  // softmax (13 prompts of up to 1700 tokens, window 1024, FP8: 178 us, with two 206).
+  // A launch of no more than two per CU asks for shared memory that a third would
+  // not have, so that it spreads over the chip (4 sequences, 100 tokens on 7900: 61
+  // us, else 75).
+  const int64_t full = ((int64_t)p.num_tokens * p.group + kExtendRows - 1) / kExtendRows * p.num_kv_heads * p.splits;
+  const unsigned lds = D <= 64 && full <= 512 ? 40960 : 0;
   hipLaunchKernelGGL((extend_kernel<QT, CT, D>), dim3((unsigned)(items * p.num_kv_heads), (unsigned)p.splits),
-                     dim3(kExtendThreads), 0, stream, p);
+                     dim3(kExtendThreads), lds, stream, p);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.splits == 1) return e;
   const int64_t rows = (int64_t)p.num_tokens * p.num_heads;

@@ -146,9 +146,9 @@ __device__ __forceinline__ void zero_tokens(const ExtendParams& p, int D, int64_
 // 110 of 243 instructions a tile on them.
 //
 // Row rho of a 32-token score product is token 16 (rho / 4 % 2) + 4 (rho / 8) +
-// rho % 4, so that register r of half h is token 16 h + r.  K's groups lie 64
-// bytes further apart than they are long: eight lanes' reads, four tokens of
-// either group, then touch different banks.
+// rho % 4, so that register r of half h is token 16 h + r.  Reads of both images
+// meet no bank twice: counted conflicts are 0, where K's groups 64 or 128 bytes
+// further apart than they are long took half as many LDS cycles again.
 //
 // Tiles that every row of a wavefront sees in full take no mask; a wavefront
 // skips tiles that none of its rows sees.
@@ -192,7 +192,7 @@ __global__ __launch_bounds__(kExtendThreads, D <= 64 ? 3 : D <= 128 ? 2 : 1) voi
   constexpr int DT = (D + 31) / 32;      // 32-dimension tiles of the output
   constexpr int DK = KSTEPS * 2;         // 8-dimension chunks staged
   constexpr int DV = DT * 32;            // dimensions of V staged
-  constexpr int KG = DK * 16 + 4;        // 16-byte pieces from one token group of K's image to the next
+  constexpr int KG = DK * 16;            // 16-byte pieces from one token group of K's image to the next
   constexpr int VU = DV / 8;             // 64-lane loads of a tile of V
   // Two stages, arrays of their own: the compiler then knows that the loads in
   // flight do not touch what is read.

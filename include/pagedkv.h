@@ -489,7 +489,8 @@ size_t pkv_paged_attention_extend_workspace_size(int32_t num_tokens,
  * below 0, every block of its tokens outside [0, num_blocks) (such tokens are
  * masked out), context 0 or beyond max_seq_len, or more than max_query_len
  * query rows in its sequence.  What a token that a row does not see holds,
- * infinities and NaN included, does not reach the row.
+ * infinities and NaN included, does not reach the row.  A row all of whose
+ * scores are minus infinity is zero too.
  *
  * query          : [num_tokens, num_heads, head_size], row stride q_stride.
  * out            : [num_tokens, num_heads, head_size] contiguous; rows from

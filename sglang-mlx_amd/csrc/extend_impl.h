@@ -1008,7 +1008,9 @@ hipError_t launch_extend_d(const ExtendParams& p, hipStream_t stream) {
   // A launch of no more than two per CU asks for shared memory that a third would
   // not have, so that it spreads over the chip (4 sequences, 100 tokens on 7900: 61
   // us, else 75).
-  const int64_t full = ((int64_t)p.num_tokens * p.group + kExtendRows - 1) / kExtendRows * p.num_kv_heads * p.splits;
+  const int64_t tiles = std::max(((int64_t)p.num_tokens * p.group + kExtendRows - 1) / kExtendRows,
+                                 (int64_t)std::min(p.num_seqs, p.num_tokens));
+  const int64_t full = tiles * p.num_kv_heads * p.splits;
   const unsigned lds = D <= 64 && full <= 512 ? 40960 : 0;
   hipLaunchKernelGGL((extend_kernel<QT, CT, D>), dim3((unsigned)(items * p.num_kv_heads), (unsigned)p.splits),
                      dim3(kExtendThreads), lds, stream, p);

@@ -615,7 +615,11 @@ ExtendCut extend_cut(int64_t num_tokens, int64_t num_seqs, int64_t num_heads, in
     const int64_t part = std::max(ceil_div(tiles, most), kPartTiles);
     return {ceil_div(tiles, part), part, slices};
   }
-  const int64_t items = ceil_div(num_tokens * group, pkv::kExtendRows) * num_kv_heads;
+  // (Short ones fill a tile for each sequence.  Split as if their rows shared tiles,
+  // 16 sequences of up to 4000 tokens with 16 new ones took 63 instead of 56 us, 64
+  // with 5 170 instead of 162.)
+  const int64_t tiles = std::max(ceil_div(num_tokens * group, pkv::kExtendRows), std::min(num_seqs, num_tokens));
+  const int64_t items = tiles * num_kv_heads;
   if (items == 0) return {1, 0, 0};
   return {std::max<int64_t>(1, std::min(512 / items, ceil_div(span, 64 * 8))), 0, 0};
 }

@@ -18,7 +18,10 @@
  *   - Launches are asynchronous on `stream` (a hipStream_t passed as void*;
  *     NULL = the legacy default stream).  Nothing synchronises.
  *   - The library allocates no device memory.  Output buffers and the
- *     attention workspace belong to the caller.
+ *     attention workspace belong to the caller.  Calls on one stream, of any
+ *     entry point and from any thread, may share a workspace: the launches of a
+ *     call with one stay together.  Calls that may overlap on the GPU (other
+ *     streams, other graphs) need workspaces of their own.
  *   - Strides are in elements, not bytes.
  *   - Block tables, context lengths and slot mappings are 32-bit integers.
  */

@@ -111,6 +111,17 @@ int resolve_partition(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
   return PKV_OK;
 }
 
+// Held over a call's launches by every call that writes a workspace.  Threads
+// that share a stream share its workspace, and some calls are two launches, the
+// second of which reads what the first left there: no launch of another call may
+// come between them.  One lock per workspace (a few may share one), so that a
+// full queue of one stream keeps no other waiting.
+std::mutex& launches_of(const void* workspace) {
+  static std::mutex locks[64];
+  const uint64_t mixed = (reinterpret_cast<uintptr_t>(workspace) >> 4) * 0x9E3779B97F4A7C15ull;
+  return locks[mixed >> 58];
+}
+
 }  // namespace
 
 static_assert(PKV_COUNTER_BYTES == pkv::kCounterBytes, "the header's counter region is the kernels'");
@@ -469,6 +480,7 @@ int paged_attention_impl(void* out, const void* query, const void* key_cache, co
   bool ok = true;
   hipError_t e = hipErrorInvalidValue;
   const hipStream_t s = static_cast<hipStream_t>(stream);
+  std::lock_guard<std::mutex> together(launches_of(workspace));
   clear_pending_error();
   if (cascade) {
     pkv::CascadeParams c;
@@ -898,11 +910,7 @@ int pkv_paged_attention_extend(void* out, const void* query, const void* key_cac
   p.block_shift = block_size == 8 ? 3 : block_size == 16 ? 4 : 5;
   p.splits = (int32_t)splits;
   p.part_tiles = (int32_t)cut.part_tiles;
-  // Split row tiles take two launches, between which no other call's may come: one
-  // from another thread on the same stream would have the same workspace.
-  static std::mutex pair;
-  std::unique_lock<std::mutex> both(pair, std::defer_lock);
-  if (p.part_tiles == 0 && p.splits > 1) both.lock();
+  std::lock_guard<std::mutex> together(launches_of(workspace));
   clear_pending_error();
   const hipStream_t s = static_cast<hipStream_t>(stream);
   hipError_t e;

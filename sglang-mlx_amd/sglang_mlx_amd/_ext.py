@@ -101,9 +101,9 @@ def _done(result) -> bool:
 # Decode scratch, one buffer per (device, stream).  Its first
 # PKV_COUNTER_BYTES are arrival counters that start at zero (cleared when the
 # buffer is made) and that every call leaves at zero; the rest is read only
-# where the same launch wrote it, or the launch before it, where the library
-# lets no other call come between the two.  So calls ordered on one stream share
-# it whatever their shapes.
+# where the same call wrote it, in one launch or in two, and the library lets no
+# other call with this buffer launch between the two.  So calls on one stream,
+# from any thread, share it whatever their shapes.
 #
 # HIP graphs: a call captured on a stream that has its buffer already uses that
 # buffer, so an outgrown buffer is kept for the graphs that hold its address

@@ -94,8 +94,10 @@ __global__ __launch_bounds__(kThreads) void step_tables_kernel(StepTablesParams 
   if ((int)blockIdx.x < token_groups) {
     if (blockIdx.x == 0)
       for (int s = tid; s <= p.num_seqs; s += kThreads) p.query_start_loc[s] = s_tok[s];
-    const int t1 = (int)min((int64_t)p.num_tokens, ((int64_t)blockIdx.x + 1) * kTokensPerGroup);
-    for (int t = blockIdx.x * kTokensPerGroup + tid; t < t1; t += kThreads) {
+    // (Counted from the group's first token: num_tokens may be 2^31 - 1.)
+    const int t0 = blockIdx.x * kTokensPerGroup, count = min(kTokensPerGroup, p.num_tokens - t0);
+    for (int i = tid; i < count; i += kThreads) {
+      const int t = t0 + i;
       int32_t slot = -1, pos = 0;
       if (t < s_tok[p.num_seqs]) {
         int lo = 0, hi = p.num_seqs;  // s_tok[lo] <= t < s_tok[hi]
@@ -119,7 +121,7 @@ __global__ __launch_bounds__(kThreads) void step_tables_kernel(StepTablesParams 
   }
   const int s = (int)blockIdx.x - token_groups;
   const Seq q = load_seq(p, s);
-  for (int b = tid; b < p.max_blocks; b += kThreads) {
+  for (int64_t b = tid; b < p.max_blocks; b += kThreads) {
     int32_t id = -1;
     if (b < q.have) {
       id = p.request_blocks[(int64_t)q.row * p.max_blocks + b];

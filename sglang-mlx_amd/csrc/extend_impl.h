@@ -120,15 +120,19 @@ __device__ __forceinline__ ExtendSeq extend_seq(const ExtendParams& p, int s) {
   return q;
 }
 
-// Zeroes rows [r0, r1) of the output's tokens, the heads of one KV head
-// (slice), by all threads of the workgroup.
+// Zeroes tokens [t0, t1) of the output, heads [h0, h0 + nh), by all threads of the
+// workgroup, 16 bytes a lane.
 template <class QT, int NT>
 __device__ __forceinline__ void zero_tokens(const ExtendParams& p, int D, int64_t t0, int64_t t1, int h0, int nh) {
   using QS = typename Elem<QT>::storage;
-  const int per = nh * D;
-  for (int64_t i = threadIdx.x; i < (t1 - t0) * per; i += NT) {
-    const int64_t t = i / per;
-    static_cast<QS*>(p.out)[((t0 + t) * p.num_heads + h0) * D + (i - t * per)] = 0;
+  const int per = nh * (D / 8);  // pieces of a token
+  const int tokens = NT / per, rest = NT - tokens * per;
+  int64_t t = t0 + (int)threadIdx.x / per;
+  int piece = (int)threadIdx.x % per;
+  for (; t < t1; t += tokens) {
+    *reinterpret_cast<uint4*>(static_cast<QS*>(p.out) + (t * p.num_heads + h0) * D + 8 * piece) = make_uint4(0, 0, 0, 0);
+    piece += rest;
+    if (piece >= per) piece -= per, ++t;
   }
 }
 
@@ -251,8 +255,9 @@ __global__ __launch_bounds__(kExtendThreads, D <= 64 ? 3 : D <= 128 ? 2 : 1) voi
     const int tiles = s_seq[2];
     if (split != 0) return;
     const int last = p.query_start_loc ? min(max(p.query_start_loc[p.num_seqs], 0), p.num_tokens) : p.num_seqs;
-    for (int64_t t = last + (item - tiles); t < p.num_tokens; t += items - tiles)
-      zero_tokens<QT, kExtendThreads>(p, D, t, t + 1, h0, group);
+    const int share = (p.num_tokens - last + items - tiles - 1) / (items - tiles);
+    const int64_t t0 = last + (int64_t)(item - tiles) * share;
+    zero_tokens<QT, kExtendThreads>(p, D, t0, min(t0 + share, (int64_t)p.num_tokens), h0, group);
     return;
   }
   const int z = __builtin_amdgcn_readfirstlane(s_seq[1]);
@@ -694,10 +699,13 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void extend_few_kernel(Exten
   const int split = blockIdx.y;
   const int kvh = unit / p.slices, slice = unit - kvh * p.slices;
   const int group = p.group, h0 = kvh * group;
-  if (seq == p.num_seqs) {
+  if (seq >= p.num_seqs) {
     // Rows behind the last sequence become zeros.
     const int last = min(max(p.query_start_loc[p.num_seqs], 0), p.num_tokens);
-    if (split == 0 && slice == 0) zero_tokens<QT, 256>(p, D, last, p.num_tokens, h0, group);
+    const int groups = (gridDim.x - p.num_seqs * p.units) * gridDim.y;
+    const int share = (p.num_tokens - last + groups - 1) / groups;
+    const int64_t t0 = last + (int64_t)((blockIdx.x - p.num_seqs * p.units) * gridDim.y + split) * share;
+    zero_tokens<QT, 256>(p, D, t0, min(t0 + share, (int64_t)p.num_tokens), 0, p.num_heads);
     return;
   }
   const ExtendSeq q = extend_seq(p, seq);
@@ -994,8 +1002,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void extend_few_kernel(Exten
 template <class QT, class CT, int D>
 hipError_t launch_extend_d(const ExtendParams& p, hipStream_t stream) {
   if (p.part_tiles > 0) {
-    const int seqs = p.num_seqs + (p.query_start_loc != nullptr ? 1 : 0);
-    const dim3 grid((unsigned)(seqs * p.units), (unsigned)p.splits);
+    const int64_t tail = p.query_start_loc != nullptr ? extend_tail_groups(p.num_tokens, p.num_heads, D, p.splits) : 0;
+    const dim3 grid((unsigned)((int64_t)p.num_seqs * p.units + tail), (unsigned)p.splits);
     if (p.max_query_len == 1)
       hipLaunchKernelGGL((extend_few_kernel<QT, CT, D, true>), grid, dim3(256), 0, stream, p);
     else

@@ -855,7 +855,8 @@ int pkv_paged_attention_extend(void* out, const void* query, const void* key_cac
                                    window, num_sinks);
   const int64_t splits = cut.splits;
   const int32_t group = num_heads / num_kv_heads;
-  const int64_t groups = cut.part_tiles > 0 ? ((int64_t)num_seqs + 1) * num_kv_heads * cut.slices
+  const int64_t groups = cut.part_tiles > 0 ? (int64_t)num_seqs * num_kv_heads * cut.slices +
+                                                  pkv::extend_tail_groups(num_tokens, num_heads, head_size, splits)
                                             : pkv::extend_items(num_tokens, num_seqs, group) * num_kv_heads;
   // (HIP bounds a launch to 2^32 work-items; rows of a sequence are counted in 32 bits.)
   if (groups * splits * 256 >= ((int64_t)1 << 32) || (int64_t)num_tokens * num_heads >= ((int64_t)1 << 30))

@@ -312,6 +312,12 @@ constexpr int kFewMaxSplits = 64;  // parts of few rows' lengths (their states m
 constexpr int64_t extend_items(int64_t num_tokens, int64_t num_seqs, int64_t group) {
   return (num_tokens * group + kExtendRows - 1) / kExtendRows + std::min(num_seqs, num_tokens) + 1;
 }
+// Few rows: workgroups, for each part of the length, that zero the rows behind the
+// last sequence (64 KB of output each if all rows are; a padded batch's are most).
+constexpr int64_t extend_tail_groups(int64_t num_tokens, int64_t num_heads, int64_t head_size, int64_t splits) {
+  const int64_t groups = (num_tokens * num_heads * head_size * 2 + 65535) / 65536;
+  return std::max<int64_t>((groups + splits - 1) / splits, 1);
+}
 // Defined in extend_impl.h, instantiated per (query, cache) pair in extend_<q>_<cache>.hip.
 template <class QT, class CT>
 hipError_t launch_extend_typed(const ExtendParams& p, int head_size, hipStream_t stream);

@@ -48,9 +48,9 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | N
         raise ValueError("rotary_dim must be even and at least 2")
     if not (math.isfinite(base) and base > 0):
         raise ValueError("base must be positive")
-    rule = dict(scaling) if scaling is not None else {"type": None}
+    rule = dict(scaling) if scaling is not None else {}
     kind = rule.get("type")
-    if kind not in (None, "linear", "ntk", "yarn", "llama3"):
+    if scaling is not None and kind not in ("linear", "ntk", "yarn", "llama3"):
         raise ValueError(f"Unknown rotary scaling {kind!r}")
     i = torch.arange(0, rotary_dim, 2, dtype=torch.float64)
     if kind == "ntk":

@@ -322,6 +322,13 @@ def test_rotary_refusals(args, msg):
         rotary_table(*args)
 
 
+def test_rotary_scaling_without_a_type_is_refused():
+    # (A rule under another name for its type must not become an unscaled table.)
+    for rule in ({}, {"factor": 8.0}, {"type": None, "factor": 8.0}, {"rope_type": "linear", "factor": 8.0}):
+        with pytest.raises(ValueError, match="Unknown rotary scaling None"):
+            rotary_table(4, 8, 1e4, rule)
+
+
 # ---- the host side of RequestBlocks ---------------------------------------------------
 
 

@@ -506,8 +506,8 @@ size_t pkv_paged_attention_extend_workspace_size(int32_t num_tokens,
  *                  then not used.
  * The other arguments as pkv_paged_attention's with PKV_LAYOUT_PAGED5D;
  * (q_dtype, cache_dtype): (BF16, BF16), (F16, F16), (BF16 | F16, FP8_E4M3);
- * max_seq_len is at most 2^30.  V's base and strides are 16-byte aligned (FP8:
- * 8-byte).
+ * max_seq_len is at most 2^30; scale (FP8: times k_scale) is finite.  V's base
+ * and strides are 16-byte aligned (FP8: 8-byte).
  * Launches: with single tokens (max_query_len 1), or few rows per KV head
  * (max_query_len * num_heads / num_kv_heads at most 16), one kernel, a workgroup
  * per (sequence, 16 rows of a KV head, part of the length), whose last arrival

@@ -850,6 +850,8 @@ int pkv_paged_attention_extend(void* out, const void* query, const void* key_cac
     return fail(PKV_ERR_UNSUPPORTED, "FP8 caches are read in the paged layout with head_size a multiple of 16");
   if (fp8 && !(std::isfinite(k_scale) && std::isfinite(v_scale) && k_scale != 0.f && v_scale != 0.f))
     return fail(PKV_ERR_INVALID, "k_scale and v_scale must be finite and nonzero for FP8 caches");
+  const float scale_log2 = scale * 1.4426950408889634f * (fp8 ? k_scale : 1.f);
+  if (!std::isfinite(scale_log2)) return fail(PKV_ERR_INVALID, "scale must be finite (with k_scale for FP8 caches)");
   if (num_blocks <= 0) return fail(PKV_ERR_INVALID, "num_blocks must be positive");
   const ExtendCut cut = extend_cut(num_tokens, num_seqs, num_heads, num_kv_heads, max_seq_len, max_query_len,
                                    window, num_sinks);
@@ -894,7 +896,7 @@ int pkv_paged_attention_extend(void* out, const void* query, const void* key_cac
   p.k_head_stride = k_head_stride;
   p.v_block_stride = v_block_stride;
   p.v_head_stride = v_head_stride;
-  p.scale_log2 = scale * 1.4426950408889634f * (fp8 ? k_scale : 1.f);
+  p.scale_log2 = scale_log2;
   p.v_scale = fp8 ? v_scale : 1.f;
   p.num_tokens = num_tokens;
   p.num_seqs = num_seqs;

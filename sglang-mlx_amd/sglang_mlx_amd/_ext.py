@@ -690,7 +690,7 @@ def _new_token_attention(op, query, key_cache, value_cache, block_tables, contex
     _tensor(query_start_loc, allow_none=True)
     num_kv_heads, block_size, max_seq_len = int(num_kv_heads), int(block_size), int(max_seq_len)
     max_query_len, window, num_sinks = int(max_query_len), int(window), int(num_sinks)
-    k_scale, v_scale = float(k_scale), float(v_scale)
+    scale, k_scale, v_scale = float(scale), float(k_scale), float(v_scale)
     if query.dim() != 3:
         raise ValueError("query must have shape [num_tokens, num_heads, head_size]")
     if block_tables.dim() != 2 or context_lens.dim() != 1:
@@ -704,6 +704,8 @@ def _new_token_attention(op, query, key_cache, value_cache, block_tables, contex
         raise ValueError("max_query_len must be positive")
     if window < 0 or num_sinks < 0:
         raise ValueError("window and num_sinks must be non-negative")
+    if not math.isfinite(scale):
+        raise ValueError("scale must be finite")
     # (The decode's checks, with a query row for each of its sequences.)
     qc, cc, layout = _check_paged_attention(query[:1].expand(B, -1, -1) if query.shape[0] else query.new_empty(
         (B,) + query.shape[1:]), key_cache, value_cache, block_tables, context_lens, num_kv_heads, block_size,
@@ -741,7 +743,7 @@ def _new_token_attention(op, query, key_cache, value_cache, block_tables, contex
         st = lib.pkv_paged_attention_extend(
             out.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), bt.data_ptr(),
             lens.data_ptr(), _ptr(start), N, B, Hq, num_kv_heads, D, block_size, bt.shape[1], max_seq_len,
-            max_query_len, window, num_sinks, key_cache.shape[0], float(scale), q_stride, key_cache.stride(0),
+            max_query_len, window, num_sinks, key_cache.shape[0], scale, q_stride, key_cache.stride(0),
             key_cache.stride(1), value_cache.stride(0), value_cache.stride(1), ws.data_ptr(), ws.numel(), qc, cc,
             k_scale, v_scale, stream)
     _lib.check(st)

@@ -221,6 +221,23 @@ def test_extend_abi_refusals():
         assert size(*bad) == 0
 
 
+def test_attention_refuses_a_scale_that_is_not_finite():
+    for scale in (math.nan, math.inf, -math.inf):
+        for extend, call in ((False, kernels.paged_attention_window), (True, kernels.paged_attention_extend)):
+            with pytest.raises(ValueError, match="scale must be finite"):
+                call(**attn_args(extend, scale=scale))
+    lib = _lib.lib()
+    args = lambda scale, cd, k_scale: (P, P, P, P, P, P, P, 5, 2, 8, 2, 128, 16, 4, 64, 3, 0, 0, 10, scale, 1024, 4096,  # noqa: E731
+                                       2048, 4096, 2048, None, 0, _lib.PKV_BF16, cd, k_scale, 1.0, None)
+    for scale, cd, k_scale in ((math.nan, _lib.PKV_BF16, 1.0), (math.inf, _lib.PKV_BF16, 1.0),
+                               (3e38, _lib.PKV_BF16, 1.0), (1e30, _lib.PKV_FP8_E4M3, 1e30)):
+        assert lib.pkv_paged_attention_extend(*args(scale, cd, k_scale)) == 1
+        assert b"scale must be finite" in lib.pkv_last_error()
+    # (An FP8 scale does not count for other caches; the next check is the workspace's.)
+    assert lib.pkv_paged_attention_extend(*args(1e30, _lib.PKV_BF16, 1e30)) == 1
+    assert b"workspace" in lib.pkv_last_error()
+
+
 def test_norm_rope_abi_refusals():
     lib = _lib.lib()
     base = dict(qo=P, q=P, k=P, v=P, pos=P, cs=P, qw=None, kw=None, kc=P, vc=P, slots=P, N=3, Hq=8, Hkv=2, D=64,

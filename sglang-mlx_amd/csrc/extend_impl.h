@@ -166,13 +166,14 @@ __device__ __forceinline__ void zero_tokens(const ExtendParams& p, int D, int64_
 // Tiles that every row of a wavefront sees in full take no mask; a wavefront
 // skips tiles that none of its rows sees.
 //
-// Bound: the matrix units, which a tile's softmax and its barrier keep waiting:
-// 8192 new tokens on 8192, 32 heads of 128, bf16, take 1.75 ms, 943 TFLOP/s of the
-// 1381 that a large matrix product reaches.  Matrix units busy 42 % and vector units
-// 50 % of the time; 32-token tiles in four stages with the softmax of one beside the
-// products of the next came to 952 TFLOP/s.  128 rows let two workgroups share a CU
-// (three at head sizes up to 64, none above 128), so that one computes while another
-// waits.
+// Bound: neither unit, but their order: a wavefront's products wait for its softmax,
+// and all for the tile's barrier.  8192 new tokens on 8192, 32 heads of 128, bf16,
+// take 1.70 - 1.76 ms, 940 - 970 TFLOP/s of the 1381 that a large matrix product
+// reaches, the matrix units busy 43 % and the vector units 42 % of the time; 32-token
+// tiles in four stages with the softmax of one beside the products of the next came
+// to 952 TFLOP/s.  128 rows let two workgroups share a CU (three at head sizes up to
+// 64, none above 128), so that one computes while another waits.  At head size 64 the
+// third costs spills, 40 bytes a lane (FP8 caches 56), and still pays (launch_extend_d).
 // ---------------------------------------------------------------------------
 constexpr int kExtendTile = 64;
 constexpr int kExtendThreads = 256;

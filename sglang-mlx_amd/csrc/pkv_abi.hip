@@ -607,9 +607,12 @@ constexpr int32_t kExtendMaxSeq = 1 << 30;
 // one slice do not help either (one workgroup per CU): 55/63/167 us.
 //
 // Few rows are cut to two workgroups per CU, which is what the registers let stay
-// resident: four a CU measured 39.3 against 31.8 us (64 sequences, window 1024,
-// FP8) and 155 against 148 us (128 sequences, window 4000); parts of 4 tiles 13.9
-// against 12.0 us, of 16 tiles 12.5 (one sequence, window 4096).
+// resident up to head size 128: four a CU measured 39.3 against 31.8 us (64 sequences,
+// window 1024, FP8) and 155 against 148 us (128 sequences, window 4000); parts of 4
+// tiles 13.9 against 12.0 us, of 16 tiles 12.5 (one sequence, window 4096).  All of
+// that is head size 128.  At 192 and 256, where one workgroup stays resident (two of
+// single tokens over 16-bit caches of 192), the same cut is kept and no other was
+// measured: 4.3 TB/s (32 sequences, window 1024, bf16; at 128 4.7), FP8 3.0 and 3.4.
 constexpr int64_t kFewRows = 16, kPartTiles = 8, kFewGroups = 512;
 struct ExtendCut {
   int64_t splits, part_tiles, slices;

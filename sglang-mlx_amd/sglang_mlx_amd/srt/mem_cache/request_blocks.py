@@ -6,6 +6,11 @@ table; a step copies its request rows, lengths and new block ids (a few words a
 sequence, one copy) and ``kernels.build_step_tables`` makes the step's block
 tables, slots and positions from them.  The host keeps what it needs to allocate
 and free: each request's blocks and token count.
+
+A request only grows: the tokens of a step stay in its context until it is
+closed.  Drafted tokens that a verification refuses cannot be taken back here; a
+caller that drafts keeps its own tables (``kernels.build_step_tables`` takes any
+lengths).
 """
 
 from __future__ import annotations

@@ -579,6 +579,150 @@ int pkv_convert_fp8(void* dst, const void* src, int64_t num_elements,
                     void* stream);
 
 /*
+ * Append to paged caches of E4M3 codes that have a scale for each block and head.
+ * No counterpart in the reference, whose conversion takes one scale for a call
+ * (convert_fp8.metal:33-35).
+ *
+ * scales: [num_blocks, num_kv_heads, 2] float32, of K and of V: a code c of the
+ * block and head stands for c * scale.  Sequence s brings the tokens of rows
+ * [start_loc[s], start_loc[s + 1]), n of them, its context's last tokens: row i
+ * goes to position context_lens[s] - n + i (nowhere below 0), in block
+ * block_tables[s][position / block_size].  For each block that receives tokens,
+ * each head, and K and V apart:
+ *   a      = the largest |x| of the new tokens in the block, of those x that are
+ *            finite;
+ *   scale  = the least power of two, at least 2^-126, with a / scale <= 240; at
+ *            least the block's scale where the block holds earlier tokens of the
+ *            context (new tokens at its offset 0 begin a block anew);
+ *   codes  = x / scale, rounded to nearest even (subnormals too); inf and NaN
+ *            become the codes of inf and NaN;
+ * and where that scale is larger than the block's, the codes of its earlier
+ * tokens c become c * (block's scale / scale), rounded the same way.
+ * Nothing else of the caches and scales changes.  Sequences of a call write
+ * different blocks; a block id outside [0, num_blocks) drops its tokens, and so
+ * does a context beyond max_num_blocks_per_seq * block_size, rows behind the last
+ * sequence go nowhere.  The scale of a block that holds earlier tokens is finite
+ * and positive.
+ *
+ * key, value: [num_tokens, num_kv_heads, head_size] of type dtype (F32, F16 or
+ * BF16), row strides key_stride and value_stride, the inner two dimensions
+ * contiguous, rows 16-byte aligned.  Caches: PKV_LAYOUT_PAGED5D of PKV_FP8_E4M3
+ * codes (x = 16), contiguous, 16-byte aligned.  head_size in
+ * {32,64,80,96,112,128,192,256}, block_size in {8,16,32}.  One launch.
+ */
+int pkv_quantize_and_cache(const void* key, const void* value, void* key_cache,
+                           void* value_cache, float* scales,
+                           const int32_t* block_tables,
+                           const int32_t* context_lens,
+                           const int32_t* start_loc, int32_t num_tokens,
+                           int32_t num_seqs, int32_t num_kv_heads,
+                           int32_t head_size, int32_t block_size,
+                           int32_t max_num_blocks_per_seq, int64_t num_blocks,
+                           int64_t key_stride, int64_t value_stride,
+                           int32_t dtype, void* stream);
+
+/*
+ * The way back: tokens 0, 1, ... of sequence s into rows [start_loc[s],
+ * start_loc[s + 1]) of key_out and value_out, code * scale rounded once to dtype
+ * (F32, F16 or BF16).  Rows without a block (its id outside [0, num_blocks), past
+ * max_num_blocks_per_seq * block_size tokens) and rows behind the last sequence
+ * are zero; start_loc[0] is 0.  key_out, value_out: [num_tokens, num_kv_heads,
+ * head_size], contiguous, 16-byte aligned.  The others as for
+ * pkv_quantize_and_cache.  One launch.
+ */
+int pkv_dequantize_cache(void* key_out, void* value_out, const void* key_cache,
+                         const void* value_cache, const float* scales,
+                         const int32_t* block_tables, const int32_t* start_loc,
+                         int32_t num_tokens, int32_t num_seqs,
+                         int32_t num_kv_heads, int32_t head_size,
+                         int32_t block_size, int32_t max_num_blocks_per_seq,
+                         int64_t num_blocks, int32_t dtype, void* stream);
+
+/*
+ * Workspace bytes that pkv_paged_attention_scaled needs: PKV_COUNTER_BYTES of
+ * arrival counters (as pkv_paged_attention's, with which a workspace may be
+ * shared), then the states of items' pieces.  0 for invalid sizes.
+ */
+size_t pkv_paged_attention_scaled_workspace_size(int32_t num_seqs,
+                                                 int32_t num_heads,
+                                                 int32_t num_kv_heads,
+                                                 int32_t head_size,
+                                                 int32_t max_seq_len,
+                                                 int32_t max_query_len,
+                                                 int32_t window,
+                                                 int32_t num_sinks);
+
+/*
+ * Attention of single and drafted tokens over caches with a scale for each block
+ * and head.  Rules, rows, masks and arguments as pkv_paged_attention_extend over
+ * FP8 caches, with K = decode(code) * scales[block][head][0] and V = decode(code)
+ * * scales[block][head][1] in the place of k_scale and v_scale (scales as
+ * pkv_quantize_and_cache writes them, or any others that are finite and not
+ * negative).  Made for few rows: every 16 rows (query tokens * num_heads /
+ * num_kv_heads) of a sequence read its keys once; for a prompt's many rows,
+ * pkv_dequantize_cache and pkv_prompt_attention take less.
+ * num_seqs * num_kv_heads * ceil(rows / 16) * (max_seq_len / 32 + 4) stays below
+ * 2^31.  One launch.
+ */
+int pkv_paged_attention_scaled(
+    void* out, const void* query, const void* key_cache, const void* value_cache,
+    const float* scales, const int32_t* block_tables,
+    const int32_t* context_lens, const int32_t* query_start_loc,
+    int32_t num_tokens, int32_t num_seqs, int32_t num_heads,
+    int32_t num_kv_heads, int32_t head_size, int32_t block_size,
+    int32_t max_num_blocks_per_seq, int32_t max_seq_len, int32_t max_query_len,
+    int32_t window, int32_t num_sinks, int64_t num_blocks, float scale,
+    int64_t q_stride, int64_t k_block_stride, int64_t k_head_stride,
+    int64_t v_block_stride, int64_t v_head_stride, void* workspace,
+    size_t workspace_bytes, int32_t q_dtype, void* stream);
+
+/*
+ * Workspace bytes that pkv_prompt_attention needs for these sizes (as
+ * pkv_paged_attention's, with which a workspace may be shared).  0 for invalid
+ * sizes.
+ */
+size_t pkv_prompt_attention_workspace_size(int32_t num_tokens, int32_t num_seqs,
+                                           int32_t num_heads,
+                                           int32_t num_kv_heads,
+                                           int32_t head_size,
+                                           int32_t max_query_len,
+                                           int32_t max_key_len, int32_t window,
+                                           int32_t num_sinks);
+
+/*
+ * Causal attention of packed prompts over their keys and values as rows.  No
+ * counterpart in the reference (whose prefill calls MLX).
+ *
+ * Sequence s has query rows [query_start_loc[s], query_start_loc[s + 1]), n of
+ * them, and key rows [key_start_loc[s], key_start_loc[s + 1]), c of them; its
+ * queries are its last n tokens: row i sits at position p = c - n + i and attends
+ * to its key rows t <= p, with a window (window > 0) to those of them with t > p -
+ * window or t < num_sinks:
+ *   out = sum_t softmax_t(scale * q . k_t) v_t,
+ * GQA as in pkv_paged_attention.  Rows that see no key and rows behind the last
+ * sequence are zero.  What a row does not see does not reach it, inf and NaN
+ * included.
+ * query [num_tokens, num_heads, head_size], key, value [num_keys, num_kv_heads,
+ * head_size], all of type dtype (BF16 or F16), row strides q_stride, k_stride and
+ * v_stride, the inner two dimensions contiguous, rows 16-byte aligned.  out:
+ * contiguous, 16-byte aligned.  key_start_loc may be NULL: query_start_loc (with
+ * num_keys = num_tokens).  max_query_len, max_key_len: the most rows of a
+ * sequence; they choose how the work is cut, not the result.
+ * head_size in {32,64,80,96,112,120,128,192,256}.  One launch, or two where few
+ * rows meet many keys.
+ */
+int pkv_prompt_attention(void* out, const void* query, const void* key,
+                         const void* value, const int32_t* query_start_loc,
+                         const int32_t* key_start_loc, int32_t num_tokens,
+                         int32_t num_keys, int32_t num_seqs, int32_t num_heads,
+                         int32_t num_kv_heads, int32_t head_size,
+                         int32_t max_query_len, int32_t max_key_len,
+                         int32_t window, int32_t num_sinks, float scale,
+                         int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                         void* workspace, size_t workspace_bytes, int32_t dtype,
+                         void* stream);
+
+/*
  * LDS bytes available to one workgroup on a device.
  * Replaces get_max_shared_memory_per_block_device_attribute
  * (mlx_device.cpp:16-20, bindings.cpp:130-133).

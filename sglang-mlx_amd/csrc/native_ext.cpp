@@ -21,9 +21,11 @@
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <pybind11/pybind11.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <limits>
@@ -525,6 +527,228 @@ PyObject* new_token_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// Paged caches of E4M3 codes with a scale for each block and head, [nb, H, D / 16, bs, 16]
+// and [nb, H, D, bs], scales [nb, H, 2]; whole: contiguous, else within a (block, head).
+bool scaled_cache(const Tensor& kc, const Tensor& vc, const Tensor& sc, const c10::Device& dev, bool whole) {
+  if (!usable(kc, dev) || !usable(vc, dev) || !usable(sc, dev) || kc.dim() != 5 || vc.dim() != 4 || sc.dim() != 3 ||
+      kc.scalar_type() != at::kByte || vc.scalar_type() != at::kByte || sc.scalar_type() != at::kFloat)
+    return false;
+  const int64_t nb = kc.size(0), H = kc.size(1), D = kc.size(2) * 16, bs = kc.size(3);
+  if (nb == 0 || H == 0 || D == 0 || kc.size(4) != 16 || vc.size(0) != nb || vc.size(1) != H || vc.size(2) != D ||
+      vc.size(3) != bs || sc.size(0) != nb || sc.size(1) != H || sc.size(2) != 2 || !sc.is_contiguous())
+    return false;
+  if (whole) return kc.is_contiguous() && vc.is_contiguous();
+  return kc.stride(2) == bs * 16 && kc.stride(3) == 16 && kc.stride(4) == 1 && vc.stride(2) == bs && vc.stride(3) == 1;
+}
+float* floats(const Tensor& t) { return static_cast<float*>(t.data_ptr()); }
+
+// (key, value, key_cache, value_cache, kv_scales, block_tables, context_lens, query_start_loc)
+PyObject* quantize_and_cache(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 8) Py_RETURN_NONE;
+  for (int i = 0; i < 8; ++i)
+    if (!plain(a[i])) Py_RETURN_NONE;
+  if (transformed()) Py_RETURN_NONE;
+  const Tensor key = THPVariable_Unpack(a[0]), value = THPVariable_Unpack(a[1]), kc = THPVariable_Unpack(a[2]),
+               vc = THPVariable_Unpack(a[3]), sc = THPVariable_Unpack(a[4]), bt = THPVariable_Unpack(a[5]),
+               lens = THPVariable_Unpack(a[6]), start = THPVariable_Unpack(a[7]);
+  const c10::Device dev = key.device();
+  if (!dev.is_cuda() || !usable(key, dev) || !usable(value, dev) || !usable(bt, dev) || !usable(lens, dev) ||
+      !usable(start, dev) || !scaled_cache(kc, vc, sc, dev, true))
+    Py_RETURN_NONE;
+  if (key.dim() != 3 || value.sizes() != key.sizes() || value.scalar_type() != key.scalar_type() ||
+      !i32_contiguous(bt, 2) || !i32_contiguous(lens, 1) || !i32_contiguous(start, 1))
+    Py_RETURN_NONE;
+  const int64_t N = key.size(0), H = key.size(1), D = key.size(2), B = lens.size(0);
+  const int64_t limit = std::numeric_limits<int32_t>::max();
+  const int code = code_of(key, false);
+  int64_t ks, vs;
+  if (N == 0 || N > limit || B == 0 || B >= limit || bt.size(0) != B || bt.size(1) == 0 || bt.size(1) > limit ||
+      start.size(0) != B + 1 || code < 0 || kc.size(1) != H || vc.size(2) != D ||
+      !aligned_rows(key, bytes_of(code), ks) || !aligned_rows(value, bytes_of(code), vs))
+    Py_RETURN_NONE;
+  const OnDevice on(dev);
+  int st;
+  {
+    pybind11::gil_scoped_release release;
+    st = pkv_quantize_and_cache(key.data_ptr(), value.data_ptr(), kc.data_ptr(), vc.data_ptr(), floats(sc), ints(bt),
+                                ints(lens), ints(start), (int32_t)N, (int32_t)B, (int32_t)H, (int32_t)D,
+                                (int32_t)kc.size(3), (int32_t)bt.size(1), kc.size(0), ks, vs, code,
+                                c10::hip::getCurrentHIPStream(dev.index()).stream());
+  }
+  if (st != PKV_OK) return PyLong_FromLong(st);
+  PyObject* out = PyList_New(3);
+  if (out == nullptr) return nullptr;
+  for (int i = 0; i < 3; ++i) {
+    Py_INCREF(a[2 + i]);
+    PyList_SET_ITEM(out, i, a[2 + i]);
+  }
+  return out;
+  END_HANDLE_TH_ERRORS
+}
+
+// (key_cache, value_cache, kv_scales, block_tables, start_loc, num_tokens, dtype)
+PyObject* dequantize_cache(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 7) Py_RETURN_NONE;
+  for (int i = 0; i < 5; ++i)
+    if (!plain(a[i])) Py_RETURN_NONE;
+  int64_t N;
+  if (!as_int(a[5], N) || !THPDtype_Check(a[6]) || transformed()) Py_RETURN_NONE;
+  const at::ScalarType type = reinterpret_cast<THPDtype*>(a[6])->scalar_type;
+  const int code = type == at::kFloat ? PKV_F32 : type == at::kHalf ? PKV_F16 : type == at::kBFloat16 ? PKV_BF16 : -1;
+  const Tensor kc = THPVariable_Unpack(a[0]), vc = THPVariable_Unpack(a[1]), sc = THPVariable_Unpack(a[2]),
+               bt = THPVariable_Unpack(a[3]), start = THPVariable_Unpack(a[4]);
+  const c10::Device dev = kc.device();
+  if (!dev.is_cuda() || code < 0 || !usable(bt, dev) || !usable(start, dev) || !scaled_cache(kc, vc, sc, dev, true) ||
+      !i32_contiguous(bt, 2) || !i32_contiguous(start, 1))
+    Py_RETURN_NONE;
+  const int64_t B = bt.size(0), H = kc.size(1), D = vc.size(2), limit = std::numeric_limits<int32_t>::max();
+  if (N <= 0 || B == 0 || B >= limit || bt.size(1) == 0 || bt.size(1) > limit || start.size(0) != B + 1)
+    Py_RETURN_NONE;
+  const OnDevice on(dev);
+  Tensor k, v;
+  int st;
+  {
+    pybind11::gil_scoped_release release;
+    k = at::empty({N, H, D}, kc.options().dtype(type));
+    v = at::empty({N, H, D}, kc.options().dtype(type));
+    st = pkv_dequantize_cache(k.data_ptr(), v.data_ptr(), kc.data_ptr(), vc.data_ptr(), floats(sc), ints(bt),
+                              ints(start), (int32_t)N, (int32_t)B, (int32_t)H, (int32_t)D, (int32_t)kc.size(3),
+                              (int32_t)bt.size(1), kc.size(0), code,
+                              c10::hip::getCurrentHIPStream(dev.index()).stream());
+  }
+  if (st != PKV_OK) return PyLong_FromLong(st);
+  return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(k)), THPVariable_Wrap(std::move(v)));
+  END_HANDLE_TH_ERRORS
+}
+
+// (scratch buffers by (device index, stream), query, key_cache, value_cache,
+// kv_scales, block_tables, context_lens, query_start_loc or None, num_kv_heads,
+// scale, block_size, max_seq_len, max_query_len, window, num_sinks)
+PyObject* paged_attention_scaled(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 15 || !PyDict_CheckExact(a[0])) Py_RETURN_NONE;
+  for (int i = 1; i < 7; ++i)
+    if (!plain(a[i])) Py_RETURN_NONE;
+  int64_t Hkv, bs, max_seq, max_query, window, sinks;
+  double scale;
+  if (!as_int(a[8], Hkv) || !as_double(a[9], scale) || !as_int(a[10], bs) || !as_int(a[11], max_seq) ||
+      !as_int(a[12], max_query) || !as_int(a[13], window) || !as_int(a[14], sinks) || transformed())
+    Py_RETURN_NONE;
+  const Tensor q = THPVariable_Unpack(a[1]), kc = THPVariable_Unpack(a[2]), vc = THPVariable_Unpack(a[3]),
+               sc = THPVariable_Unpack(a[4]), bt = THPVariable_Unpack(a[5]), lens = THPVariable_Unpack(a[6]);
+  const c10::Device dev = q.device();
+  if (!dev.is_cuda() || !usable(q, dev) || !usable(bt, dev) || !usable(lens, dev) ||
+      !scaled_cache(kc, vc, sc, dev, false) || q.dim() != 3 || !i32_contiguous(bt, 2) || !i32_contiguous(lens, 1))
+    Py_RETURN_NONE;
+  const int64_t N = q.size(0), B = lens.size(0), Hq = q.size(1), D = q.size(2);
+  Tensor start;
+  if (a[7] != Py_None) {
+    if (!plain(a[7])) Py_RETURN_NONE;
+    start = THPVariable_Unpack(a[7]);
+    if (!usable(start, dev) || !i32_contiguous(start, 1) || start.size(0) != B + 1) Py_RETURN_NONE;
+  } else if (N != B || max_query != 1) {
+    Py_RETURN_NONE;
+  }
+  const int64_t limit = std::numeric_limits<int32_t>::max();
+  const int qc = code_of(q, false);
+  int64_t qs;
+  if (N == 0 || N > limit || B == 0 || bt.size(0) != B || bt.size(1) > limit || Hkv <= 0 || Hq == 0 ||
+      Hq % Hkv != 0 || bs <= 0 || max_seq <= 0 || max_query <= 0 || window < 0 || sinks < 0 ||
+      max_seq > bt.size(1) * bs || kc.size(1) != Hkv || vc.size(2) != D || kc.size(3) != bs ||
+      (qc != PKV_BF16 && qc != PKV_F16) || !aligned_rows(q, 2, qs))
+    Py_RETURN_NONE;
+  max_query = std::min(max_query, N);
+  const size_t need = pkv_paged_attention_scaled_workspace_size((int32_t)B, (int32_t)Hq, (int32_t)Hkv, (int32_t)D,
+                                                                (int32_t)max_seq, (int32_t)max_query, (int32_t)window,
+                                                                (int32_t)sinks);
+  if (need == 0) Py_RETURN_NONE;
+  const auto stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+  Tensor ws;
+  if (!find_scratch(a[0], dev, stream, need, ws)) return nullptr;
+  if (!ws.defined()) Py_RETURN_NONE;
+  const OnDevice on(dev);
+  Tensor out;
+  int st;
+  {
+    pybind11::gil_scoped_release release;
+    out = at::empty({N, Hq, D}, q.options());
+    st = pkv_paged_attention_scaled(
+        out.data_ptr(), q.data_ptr(), kc.data_ptr(), vc.data_ptr(), floats(sc), ints(bt), ints(lens),
+        start.defined() ? ints(start) : nullptr, (int32_t)N, (int32_t)B, (int32_t)Hq, (int32_t)Hkv, (int32_t)D,
+        (int32_t)bs, (int32_t)bt.size(1), (int32_t)max_seq, (int32_t)max_query, (int32_t)window, (int32_t)sinks,
+        kc.size(0), (float)scale, qs, kc.stride(0), kc.stride(1), vc.stride(0), vc.stride(1), ws.data_ptr(),
+        (size_t)ws.numel(), qc, stream);
+  }
+  if (st != PKV_OK) return PyLong_FromLong(st);
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// (scratch buffers by (device index, stream), query, key, value, query_start_loc,
+// scale, max_query_len, key_start_loc or None, max_key_len or None, window, num_sinks)
+PyObject* prompt_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 11 || !PyDict_CheckExact(a[0])) Py_RETURN_NONE;
+  for (int i = 1; i < 5; ++i)
+    if (!plain(a[i])) Py_RETURN_NONE;
+  int64_t max_query, max_key, window, sinks;
+  double scale;
+  if (!as_double(a[5], scale) || !as_int(a[6], max_query) || !as_int(a[9], window) || !as_int(a[10], sinks) ||
+      transformed())
+    Py_RETURN_NONE;
+  const Tensor q = THPVariable_Unpack(a[1]), k = THPVariable_Unpack(a[2]), v = THPVariable_Unpack(a[3]),
+               start = THPVariable_Unpack(a[4]);
+  const c10::Device dev = q.device();
+  if (!dev.is_cuda() || !usable(q, dev) || !usable(k, dev) || !usable(v, dev) || !usable(start, dev) ||
+      q.dim() != 3 || k.dim() != 3 || v.sizes() != k.sizes() || !i32_contiguous(start, 1))
+    Py_RETURN_NONE;
+  const int64_t N = q.size(0), Hq = q.size(1), D = q.size(2), T = k.size(0), H = k.size(1), B = start.size(0) - 1;
+  Tensor key_start;
+  if (a[7] != Py_None) {
+    if (!plain(a[7]) || !as_int(a[8], max_key)) Py_RETURN_NONE;
+    key_start = THPVariable_Unpack(a[7]);
+    if (!usable(key_start, dev) || !i32_contiguous(key_start, 1) || key_start.size(0) != B + 1) Py_RETURN_NONE;
+  } else {
+    if (T != N || a[8] != Py_None) Py_RETURN_NONE;
+    max_key = max_query;
+  }
+  const int64_t limit = 1 << 30;
+  const int code = code_of(q, false);
+  int64_t qs, ks, vs;
+  if (N == 0 || N > limit || T == 0 || T > limit || B <= 0 || Hq == 0 || H == 0 || Hq % H != 0 || k.size(2) != D ||
+      (code != PKV_BF16 && code != PKV_F16) || k.scalar_type() != q.scalar_type() ||
+      v.scalar_type() != q.scalar_type() || max_query <= 0 || max_key <= 0 || window < 0 || sinks < 0 ||
+      !aligned_rows(q, 2, qs) || !aligned_rows(k, 2, ks) || !aligned_rows(v, 2, vs))
+    Py_RETURN_NONE;
+  max_query = std::min(max_query, N);
+  max_key = std::min(max_key, T);
+  const size_t need = pkv_prompt_attention_workspace_size((int32_t)N, (int32_t)B, (int32_t)Hq, (int32_t)H, (int32_t)D,
+                                                          (int32_t)max_query, (int32_t)max_key, (int32_t)window,
+                                                          (int32_t)sinks);
+  if (need == 0) Py_RETURN_NONE;
+  const auto stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+  Tensor ws;
+  if (!find_scratch(a[0], dev, stream, need, ws)) return nullptr;
+  if (!ws.defined()) Py_RETURN_NONE;
+  const OnDevice on(dev);
+  Tensor out;
+  int st;
+  {
+    pybind11::gil_scoped_release release;
+    out = at::empty({N, Hq, D}, q.options());
+    st = pkv_prompt_attention(out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), ints(start),
+                              key_start.defined() ? ints(key_start) : nullptr, (int32_t)N, (int32_t)T, (int32_t)B,
+                              (int32_t)Hq, (int32_t)H, (int32_t)D, (int32_t)max_query, (int32_t)max_key,
+                              (int32_t)window, (int32_t)sinks, (float)scale, qs, ks, vs, ws.data_ptr(),
+                              (size_t)ws.numel(), code, stream);
+  }
+  if (st != PKV_OK) return PyLong_FromLong(st);
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
 // (stream handle) -> a number that names the HIP graph capture under way on
 // the stream, 0 if there is none.
 PyObject* capture_id(PyObject*, PyObject* handle) {
@@ -550,6 +774,10 @@ PyMethodDef methods[] = {
     {"qk_norm_rope", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(qk_norm_rope)), METH_FASTCALL, nullptr},
     {"qk_norm_rope_and_cache", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(qk_norm_rope_and_cache)), METH_FASTCALL, nullptr},
     {"new_token_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(new_token_attention)), METH_FASTCALL, nullptr},
+    {"quantize_and_cache", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(quantize_and_cache)), METH_FASTCALL, nullptr},
+    {"dequantize_cache", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(dequantize_cache)), METH_FASTCALL, nullptr},
+    {"paged_attention_scaled", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(paged_attention_scaled)), METH_FASTCALL, nullptr},
+    {"prompt_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(prompt_attention)), METH_FASTCALL, nullptr},
     {"capture_id", capture_id, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

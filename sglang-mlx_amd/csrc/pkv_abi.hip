@@ -650,6 +650,86 @@ ExtendWorkspace extend_workspace(int64_t num_tokens, int64_t num_heads, int64_t 
   return w;
 }
 
+// ---- caches with a scale for each block and head ---------------------------------
+
+// What store and read share of their checks; fills p's sizes.
+int scaled_cache_args(pkv::ScaledCacheParams& p, const void* key_cache, const void* value_cache, const float* scales,
+                      const int32_t* block_tables, const int32_t* start_loc, int32_t num_tokens, int32_t num_seqs,
+                      int32_t num_kv_heads, int32_t head_size, int32_t block_size, int32_t max_num_blocks_per_seq,
+                      int64_t num_blocks, int32_t dtype) {
+  if (num_tokens < 0 || num_seqs < 0)
+    return fail(PKV_ERR_INVALID, "num_tokens and num_seqs must be non-negative");
+  if (num_kv_heads <= 0) return fail(PKV_ERR_INVALID, "num_kv_heads must be positive");
+  if (!valid_dtype(dtype)) return fail(PKV_ERR_INVALID, "Unsupported dtype");
+  if (!valid_head_size(head_size) || head_size % 16 != 0 || !valid_block_size(block_size))
+    return fail(PKV_ERR_UNSUPPORTED, "Unsupported head_size/block_size for FP8 caches");
+  if (max_num_blocks_per_seq <= 0) return fail(PKV_ERR_INVALID, "max_num_blocks_per_seq must be positive");
+  if (num_blocks <= 0 || num_blocks > INT32_MAX) return fail(PKV_ERR_INVALID, "num_blocks must be in [1, 2^31)");
+  p.k_cache = const_cast<void*>(key_cache);
+  p.v_cache = const_cast<void*>(value_cache);
+  p.scales = const_cast<float*>(scales);
+  p.block_tables = block_tables;
+  p.start_loc = start_loc;
+  p.num_blocks = num_blocks;
+  p.num_tokens = num_tokens;
+  p.num_seqs = num_seqs;
+  p.num_heads = num_kv_heads;
+  p.head_size = head_size;
+  p.block_shift = block_size == 8 ? 3 : block_size == 16 ? 4 : 5;
+  p.max_blocks_per_seq = max_num_blocks_per_seq;
+  p.dtype = dtype;
+  // (HIP bounds a launch to 2^32 work-items.)
+  if (pkv::scaled_cache_groups(p) * 256 >= ((int64_t)1 << 32))
+    return fail(PKV_ERR_UNSUPPORTED, "num_tokens * num_kv_heads exceeds the launch grid limit");
+  if (num_tokens == 0) return PKV_OK;
+  if (!key_cache || !value_cache || !scales || !start_loc || (num_seqs > 0 && !block_tables))
+    return fail(PKV_ERR_INVALID, "null buffer");
+  if (!aligned16(key_cache) || !aligned16(value_cache) || (reinterpret_cast<uintptr_t>(scales) & 7u) != 0)
+    return fail(PKV_ERR_INVALID, "caches must be 16-byte aligned, scales 8-byte");
+  return PKV_OK;
+}
+int scaled_cache_launch(const pkv::ScaledCacheParams& p, const char* where, void* stream) {
+  clear_pending_error();
+  const hipError_t e = pkv::launch_scaled_cache(p, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, where);
+  return PKV_OK;
+}
+
+// How pkv_paged_attention_scaled is cut: workgroups for the most tiles that its sizes
+// allow, each at least kScaledLeast long, and at most those that stay resident.
+struct ScaledCut {
+  int64_t slices, tiles, workgroups;  // tiles: of all items, each with its start (a bound)
+};
+ScaledCut scaled_cut(int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads, int64_t max_seq_len,
+                     int64_t max_query_len, int64_t window, int64_t num_sinks) {
+  const int64_t slices = ceil_div(max_query_len * (num_heads / num_kv_heads), 16);
+  // (The window and the sinks each end inside a tile.)
+  int64_t tiles = ceil_div(max_seq_len, 32);
+  if (window > 0) tiles = std::min(tiles, ceil_div(window + max_query_len, 32) + ceil_div(num_sinks, 32) + 2);
+  const int64_t all = num_seqs * num_kv_heads * slices * (tiles + pkv::kScaledStart);
+  return {slices, all,
+          std::min<int64_t>(pkv::kScaledWorkgroups, std::max<int64_t>(ceil_div(all, pkv::kScaledLeast), 1))};
+}
+struct ScaledWorkspace {
+  size_t ml_bytes, total;
+};
+ScaledWorkspace scaled_workspace(const ScaledCut& cut, int64_t head_size) {
+  const size_t rows = (size_t)cut.workgroups * 2 * 16;
+  return {rows * 4 * sizeof(float),
+          (size_t)pkv::kCounterBytes + rows * 4 * sizeof(float) + rows * head_size * sizeof(float)};
+}
+
+// Parts of the keys of pkv_prompt_attention's row tiles: as many as make the launch fill
+// the chip, none shorter than 8 tiles of 64 keys (pkv_paged_attention_extend's rule).
+int64_t prompt_splits(int64_t num_tokens, int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads,
+                      int64_t max_query_len, int64_t max_key_len, int64_t window, int64_t num_sinks) {
+  const int64_t group = num_heads / num_kv_heads;
+  const int64_t span = window > 0 ? std::min(max_key_len, window + max_query_len + num_sinks) : max_key_len;
+  const int64_t tiles = std::max(ceil_div(num_tokens * group, pkv::kExtendRows), std::min(num_seqs, num_tokens));
+  if (tiles == 0) return 1;
+  return std::max<int64_t>(1, std::min(512 / (tiles * num_kv_heads), ceil_div(span, 64 * 8)));
+}
+
 }  // namespace
 
 extern "C" {
@@ -927,6 +1007,243 @@ int pkv_paged_attention_extend(void* out, const void* query, const void* key_cac
     e = q_dtype == PKV_BF16 ? pkv::launch_extend_typed<pkv::BF16, pkv::BF16>(p, head_size, s)
                             : pkv::launch_extend_typed<pkv::F16, pkv::F16>(p, head_size, s);
   if (e != hipSuccess) return hip_fail(e, "paged_attention_extend launch");
+  return PKV_OK;
+}
+
+int pkv_quantize_and_cache(const void* key, const void* value, void* key_cache, void* value_cache, float* scales,
+                           const int32_t* block_tables, const int32_t* context_lens, const int32_t* start_loc,
+                           int32_t num_tokens, int32_t num_seqs, int32_t num_kv_heads, int32_t head_size,
+                           int32_t block_size, int32_t max_num_blocks_per_seq, int64_t num_blocks, int64_t key_stride,
+                           int64_t value_stride, int32_t dtype, void* stream) {
+  pkv::ScaledCacheParams p = {};
+  const int st = scaled_cache_args(p, key_cache, value_cache, scales, block_tables, start_loc, num_tokens, num_seqs,
+                                   num_kv_heads, head_size, block_size, max_num_blocks_per_seq, num_blocks, dtype);
+  if (st != PKV_OK || num_tokens == 0 || num_seqs == 0) return st;
+  if (!key || !value || !context_lens) return fail(PKV_ERR_INVALID, "null buffer");
+  const int64_t row = (int64_t)num_kv_heads * head_size, eb = elem_bytes(dtype);
+  if (key_stride < row || value_stride < row || !aligned16(key) || !aligned16(value) || (key_stride * eb) % 16 != 0 ||
+      (value_stride * eb) % 16 != 0)
+    return fail(PKV_ERR_INVALID, "key and value rows must be 16-byte aligned, num_kv_heads * head_size long");
+  p.key = key;
+  p.value = value;
+  p.context_lens = context_lens;
+  p.key_stride = key_stride;
+  p.value_stride = value_stride;
+  return scaled_cache_launch(p, "quantize_and_cache launch", stream);
+}
+
+int pkv_dequantize_cache(void* key_out, void* value_out, const void* key_cache, const void* value_cache,
+                         const float* scales, const int32_t* block_tables, const int32_t* start_loc,
+                         int32_t num_tokens, int32_t num_seqs, int32_t num_kv_heads, int32_t head_size,
+                         int32_t block_size, int32_t max_num_blocks_per_seq, int64_t num_blocks, int32_t dtype,
+                         void* stream) {
+  pkv::ScaledCacheParams p = {};
+  p.key_out = key_out;
+  p.value_out = value_out;
+  if (num_tokens > 0 && (!key_out || !value_out)) return fail(PKV_ERR_INVALID, "null buffer");
+  if (!aligned16(key_out) || !aligned16(value_out))
+    return fail(PKV_ERR_INVALID, "key_out and value_out must be 16-byte aligned");
+  const int st = scaled_cache_args(p, key_cache, value_cache, scales, block_tables, start_loc, num_tokens, num_seqs,
+                                   num_kv_heads, head_size, block_size, max_num_blocks_per_seq, num_blocks, dtype);
+  if (st != PKV_OK || num_tokens == 0) return st;
+  return scaled_cache_launch(p, "dequantize_cache launch", stream);
+}
+
+size_t pkv_paged_attention_scaled_workspace_size(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
+                                                 int32_t head_size, int32_t max_seq_len, int32_t max_query_len,
+                                                 int32_t window, int32_t num_sinks) {
+  if (num_seqs < 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 || head_size <= 0 ||
+      max_seq_len <= 0 || max_seq_len > kExtendMaxSeq || max_query_len <= 0 || window < 0 || num_sinks < 0)
+    return 0;
+  return scaled_workspace(scaled_cut(num_seqs, num_heads, num_kv_heads, max_seq_len, max_query_len, window, num_sinks),
+                          head_size).total;
+}
+
+int pkv_paged_attention_scaled(void* out, const void* query, const void* key_cache, const void* value_cache,
+                               const float* scales, const int32_t* block_tables, const int32_t* context_lens,
+                               const int32_t* query_start_loc, int32_t num_tokens, int32_t num_seqs, int32_t num_heads,
+                               int32_t num_kv_heads, int32_t head_size, int32_t block_size,
+                               int32_t max_num_blocks_per_seq, int32_t max_seq_len, int32_t max_query_len,
+                               int32_t window, int32_t num_sinks, int64_t num_blocks, float scale, int64_t q_stride,
+                               int64_t k_block_stride, int64_t k_head_stride, int64_t v_block_stride,
+                               int64_t v_head_stride, void* workspace, size_t workspace_bytes, int32_t q_dtype,
+                               void* stream) {
+  if (num_tokens < 0 || num_seqs < 0)
+    return fail(PKV_ERR_INVALID, "num_tokens and num_seqs must be non-negative");
+  if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0)
+    return fail(PKV_ERR_INVALID, "num_heads must be divisible by num_kv_heads");
+  if (max_seq_len <= 0) return fail(PKV_ERR_INVALID, "max_seq_len must be positive");
+  if (max_seq_len > kExtendMaxSeq) return fail(PKV_ERR_UNSUPPORTED, "max_seq_len must be at most 2^30");
+  if (max_query_len <= 0) return fail(PKV_ERR_INVALID, "max_query_len must be positive");
+  if (window < 0 || num_sinks < 0) return fail(PKV_ERR_INVALID, "window and num_sinks must be non-negative");
+  if (query_start_loc == nullptr && (num_tokens != num_seqs || max_query_len != 1))
+    return fail(PKV_ERR_INVALID, "without query_start_loc a call has one token per sequence");
+  if (!valid_head_size(head_size) || head_size % 16 != 0 || !valid_block_size(block_size))
+    return fail(PKV_ERR_UNSUPPORTED, "Unsupported head_size/block_size for FP8 caches");
+  if (max_num_blocks_per_seq <= 0 || (int64_t)max_seq_len > (int64_t)max_num_blocks_per_seq * block_size)
+    return fail(PKV_ERR_INVALID, "max_seq_len exceeds block table capacity");
+  if (q_dtype != PKV_BF16 && q_dtype != PKV_F16)
+    return fail(PKV_ERR_UNSUPPORTED, "Unsupported query dtype for paged_attention_scaled");
+  const float scale_log2 = scale * 1.4426950408889634f;
+  if (!std::isfinite(scale_log2)) return fail(PKV_ERR_INVALID, "scale must be finite");
+  if (num_blocks <= 0) return fail(PKV_ERR_INVALID, "num_blocks must be positive");
+  max_query_len = std::min(max_query_len, std::max(num_tokens, 1));  // (no sequence has more rows)
+  const ScaledCut cut =
+      scaled_cut(num_seqs, num_heads, num_kv_heads, max_seq_len, max_query_len, window, num_sinks);
+  // (Tiles and query rows are counted in 32 bits; HIP bounds a launch to 2^32 work-items.)
+  if (cut.tiles >= ((int64_t)1 << 31) - pkv::kScaledLeast * pkv::kScaledWorkgroups ||
+      (int64_t)num_tokens * num_heads >= ((int64_t)1 << 30) ||
+      (cut.workgroups + pkv::extend_tail_groups(num_tokens, num_heads, head_size, 1)) * 256 >= ((int64_t)1 << 32))
+    return fail(PKV_ERR_UNSUPPORTED, "num_seqs * num_heads * max_seq_len exceeds what a launch counts");
+  if (num_tokens == 0) return PKV_OK;
+  if (!out || !query || !key_cache || !value_cache || !scales || (num_seqs > 0 && (!block_tables || !context_lens)))
+    return fail(PKV_ERR_INVALID, "null buffer");
+  if (!aligned16(out)) return fail(PKV_ERR_INVALID, "out must be 16-byte aligned");
+  if (!aligned16(query) || (q_stride * 2) % 16 != 0 || q_stride < (int64_t)num_heads * head_size)
+    return fail(PKV_ERR_INVALID, "query rows must be 16-byte aligned with stride >= num_heads * head_size");
+  if (!aligned16(key_cache) || k_block_stride % 16 != 0 || k_head_stride % 16 != 0 ||
+      (reinterpret_cast<uintptr_t>(value_cache) % 8) != 0 || v_block_stride % 8 != 0 || v_head_stride % 8 != 0 ||
+      (reinterpret_cast<uintptr_t>(scales) % 8) != 0)
+    return fail(PKV_ERR_INVALID, "cache or scale bases or strides are not aligned for vector loads");
+  const ScaledWorkspace w = scaled_workspace(cut, head_size);
+  if (workspace == nullptr || workspace_bytes < w.total)
+    return fail(PKV_ERR_INVALID, "workspace is smaller than pkv_paged_attention_scaled_workspace_size()");
+  if (!aligned16(workspace)) return fail(PKV_ERR_INVALID, "workspace must be 16-byte aligned");
+  char* ws = static_cast<char*>(workspace);
+  pkv::ScaledAttentionParams p = {};
+  p.out = out;
+  p.q = query;
+  p.k_cache = key_cache;
+  p.v_cache = value_cache;
+  p.scales = scales;
+  p.block_tables = block_tables;
+  p.context_lens = context_lens;
+  p.query_start_loc = query_start_loc;
+  p.counters = reinterpret_cast<int32_t*>(ws);
+  p.ws_ml = reinterpret_cast<float*>(ws + pkv::kCounterBytes);
+  p.ws_o = reinterpret_cast<float*>(ws + pkv::kCounterBytes + w.ml_bytes);
+  p.num_blocks = num_blocks;
+  p.q_stride = q_stride;
+  p.k_block_stride = k_block_stride;
+  p.k_head_stride = k_head_stride;
+  p.v_block_stride = v_block_stride;
+  p.v_head_stride = v_head_stride;
+  p.scale_log2 = scale_log2;
+  p.num_tokens = num_tokens;
+  p.num_seqs = num_seqs;
+  p.num_heads = num_heads;
+  p.num_kv_heads = num_kv_heads;
+  p.group = num_heads / num_kv_heads;
+  p.slices = (int32_t)cut.slices;
+  p.units = (int32_t)(num_kv_heads * cut.slices);
+  p.max_blocks_per_seq = max_num_blocks_per_seq;
+  p.max_seq_len = max_seq_len;
+  p.max_query_len = max_query_len;
+  p.window = std::min(window, max_seq_len);  // (a longer one sees no more)
+  p.sinks = std::min(num_sinks, max_seq_len);
+  p.workgroups = (int32_t)cut.workgroups;
+  std::lock_guard<std::mutex> together(launches_of(workspace));
+  clear_pending_error();
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  hipError_t e;
+  if (q_dtype == PKV_BF16)
+    e = block_size == 8    ? pkv::launch_scaled_attention<pkv::BF16, 8>(p, head_size, s)
+        : block_size == 16 ? pkv::launch_scaled_attention<pkv::BF16, 16>(p, head_size, s)
+                           : pkv::launch_scaled_attention<pkv::BF16, 32>(p, head_size, s);
+  else
+    e = block_size == 8    ? pkv::launch_scaled_attention<pkv::F16, 8>(p, head_size, s)
+        : block_size == 16 ? pkv::launch_scaled_attention<pkv::F16, 16>(p, head_size, s)
+                           : pkv::launch_scaled_attention<pkv::F16, 32>(p, head_size, s);
+  if (e != hipSuccess) return hip_fail(e, "paged_attention_scaled launch");
+  return PKV_OK;
+}
+
+size_t pkv_prompt_attention_workspace_size(int32_t num_tokens, int32_t num_seqs, int32_t num_heads,
+                                           int32_t num_kv_heads, int32_t head_size, int32_t max_query_len,
+                                           int32_t max_key_len, int32_t window, int32_t num_sinks) {
+  if (num_tokens < 0 || num_seqs < 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 ||
+      head_size <= 0 || max_query_len <= 0 || max_key_len <= 0 || window < 0 || num_sinks < 0)
+    return 0;
+  return extend_workspace(num_tokens, num_heads, head_size,
+                          prompt_splits(num_tokens, num_seqs, num_heads, num_kv_heads, max_query_len, max_key_len,
+                                        window, num_sinks))
+      .total;
+}
+
+int pkv_prompt_attention(void* out, const void* query, const void* key, const void* value,
+                         const int32_t* query_start_loc, const int32_t* key_start_loc, int32_t num_tokens,
+                         int32_t num_keys, int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
+                         int32_t head_size, int32_t max_query_len, int32_t max_key_len, int32_t window,
+                         int32_t num_sinks, float scale, int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                         void* workspace, size_t workspace_bytes, int32_t dtype, void* stream) {
+  if (num_tokens < 0 || num_keys < 0 || num_seqs < 0)
+    return fail(PKV_ERR_INVALID, "num_tokens, num_keys and num_seqs must be non-negative");
+  if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0)
+    return fail(PKV_ERR_INVALID, "num_heads must be divisible by num_kv_heads");
+  if (max_query_len <= 0 || max_key_len <= 0)
+    return fail(PKV_ERR_INVALID, "max_query_len and max_key_len must be positive");
+  if (num_keys > kExtendMaxSeq) return fail(PKV_ERR_UNSUPPORTED, "num_keys must be at most 2^30");
+  if (window < 0 || num_sinks < 0) return fail(PKV_ERR_INVALID, "window and num_sinks must be non-negative");
+  if (key_start_loc == nullptr && num_keys != num_tokens)
+    return fail(PKV_ERR_INVALID, "without key_start_loc there are as many keys as queries");
+  if (!valid_head_size(head_size)) return fail(PKV_ERR_UNSUPPORTED, "Unsupported head_size for prompt_attention");
+  if (dtype != PKV_BF16 && dtype != PKV_F16)
+    return fail(PKV_ERR_UNSUPPORTED, "Unsupported dtype for prompt_attention");
+  const float scale_log2 = scale * 1.4426950408889634f;
+  if (!std::isfinite(scale_log2)) return fail(PKV_ERR_INVALID, "scale must be finite");
+  const int64_t row = (int64_t)num_kv_heads * head_size;
+  if (q_stride < (int64_t)num_heads * head_size || k_stride < row || v_stride < row)
+    return fail(PKV_ERR_INVALID, "query/key/value row stride is smaller than a row");
+  // (The kernel's offsets within 16 rows of keys are 32-bit.)
+  if (k_stride > (int64_t)1 << 26 || v_stride > (int64_t)1 << 26)
+    return fail(PKV_ERR_UNSUPPORTED, "key/value row stride must be at most 2^26 elements");
+  const int32_t group = num_heads / num_kv_heads;
+  const int64_t splits = prompt_splits(num_tokens, num_seqs, num_heads, num_kv_heads, max_query_len, max_key_len,
+                                       window, num_sinks);
+  // (HIP bounds a launch to 2^32 work-items; rows of a sequence are counted in 32 bits.)
+  if (pkv::extend_items(num_tokens, num_seqs, group) * num_kv_heads * splits * 256 >= ((int64_t)1 << 32) ||
+      (int64_t)num_tokens * num_heads >= ((int64_t)1 << 30))
+    return fail(PKV_ERR_UNSUPPORTED, "num_tokens * num_heads exceeds the launch grid limit");
+  if (num_tokens == 0) return PKV_OK;
+  if (!out || !query || (num_keys > 0 && (!key || !value)) || !query_start_loc)
+    return fail(PKV_ERR_INVALID, "null buffer");
+  if (!aligned16(out) || !aligned16(query) || !aligned16(key) || !aligned16(value) || q_stride % 8 != 0 ||
+      k_stride % 8 != 0 || v_stride % 8 != 0)
+    return fail(PKV_ERR_INVALID, "out and the rows of query, key and value must be 16-byte aligned");
+  const ExtendWorkspace w = extend_workspace(num_tokens, num_heads, head_size, splits);
+  if (workspace == nullptr || workspace_bytes < w.total)
+    return fail(PKV_ERR_INVALID, "workspace is smaller than pkv_prompt_attention_workspace_size()");
+  if (!aligned16(workspace)) return fail(PKV_ERR_INVALID, "workspace must be 16-byte aligned");
+  char* ws = static_cast<char*>(workspace);
+  pkv::PromptParams p = {};
+  p.out = out;
+  p.q = query;
+  p.k_cache = key;
+  p.v_cache = value;
+  p.query_start_loc = query_start_loc;
+  p.key_start_loc = key_start_loc ? key_start_loc : query_start_loc;
+  p.ws_ml = reinterpret_cast<float*>(ws + pkv::kCounterBytes);
+  p.ws_o = reinterpret_cast<float*>(ws + pkv::kCounterBytes + w.ml_bytes);
+  p.q_stride = q_stride;
+  p.k_stride = k_stride;
+  p.v_stride = v_stride;
+  p.scale_log2 = scale_log2;
+  p.v_scale = 1.f;
+  p.num_tokens = num_tokens;
+  p.num_keys = num_keys;
+  p.num_seqs = num_seqs;
+  p.num_heads = num_heads;
+  p.num_kv_heads = num_kv_heads;
+  p.group = group;
+  p.window = std::min(window, kExtendMaxSeq);  // (a longer one sees no more)
+  p.sinks = std::min(num_sinks, kExtendMaxSeq);
+  p.splits = (int32_t)splits;
+  std::lock_guard<std::mutex> together(launches_of(workspace));
+  clear_pending_error();
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const hipError_t e = dtype == PKV_BF16 ? pkv::launch_prompt<pkv::BF16>(p, head_size, s)
+                                         : pkv::launch_prompt<pkv::F16>(p, head_size, s);
+  if (e != hipSuccess) return hip_fail(e, "prompt_attention launch");
   return PKV_OK;
 }
 

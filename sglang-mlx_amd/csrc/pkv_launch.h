@@ -322,6 +322,59 @@ constexpr int64_t extend_tail_groups(int64_t num_tokens, int64_t num_heads, int6
 template <class QT, class CT>
 hipError_t launch_extend_typed(const ExtendParams& p, int head_size, hipStream_t stream);
 
+// Caches with a scale for each block and head (scaled_cache.hip; the rules of
+// pkv_quantize_and_cache and pkv_dequantize_cache).
+struct ScaledCacheParams {
+  const void* key;              // store: [num_tokens, H, D], row strides in elements
+  const void* value;
+  void* key_out;                // read: [num_tokens, H, D], contiguous (null: store)
+  void* value_out;
+  void* k_cache;                // paged 5-D, contiguous
+  void* v_cache;
+  float* scales;                // [num_blocks, H, 2]: K's, V's
+  const int32_t* block_tables;
+  const int32_t* context_lens;  // store
+  const int32_t* start_loc;     // [num_seqs + 1]
+  int64_t key_stride, value_stride;
+  int64_t num_blocks;
+  int32_t num_tokens, num_seqs, num_heads, head_size, block_shift, max_blocks_per_seq;
+  int32_t dtype;                // of the rows
+};
+// Workgroups of a call: a wavefront for K and one for V of every head and block that
+// its tokens can touch.
+inline int64_t scaled_cache_groups(const ScaledCacheParams& p) {
+  const int64_t per = p.key_out != nullptr ? 1 : 2;  // (the search in scaled_cache.hip)
+  const int64_t items = ((int64_t)p.num_tokens >> p.block_shift) + per * ((int64_t)p.num_seqs + 1);
+  return (items * p.num_heads * 2 + 3) / 4;
+}
+hipError_t launch_scaled_cache(const ScaledCacheParams& p, hipStream_t stream);
+
+// Attention of single and drafted tokens over caches with a scale for each block and
+// head (scaled_attention_impl.h; the rules of pkv_paged_attention_scaled).  Pieces'
+// states: per workgroup two slots of 16 rows, (max, sum, exponent) in ws_ml, outputs in
+// ws_o, and one arrival counter.
+struct ScaledAttentionParams : ExtendParams {
+  const float* scales;   // [num_blocks, H, 2]: K's, V's
+  int32_t workgroups;
+};
+constexpr int kScaledStart = 4;    // what an item's start costs, in tiles
+constexpr int kScaledLeast = 8;    // the least span of a workgroup, in tiles
+constexpr int kScaledWorkgroups = 768;
+constexpr int kNoExponent = -300;  // below the exponent of every scale
+// (one block size a file, scaled_attention_<q>_<block size>.hip)
+template <class QT, int BS>
+hipError_t launch_scaled_attention(const ScaledAttentionParams& p, int head_size, hipStream_t stream);
+
+// Attention of packed prompts over their keys and values as rows (prompt_impl.h; the
+// rules of pkv_prompt_attention): k_cache and v_cache are the first rows.
+struct PromptParams : ExtendParams {
+  const int32_t* key_start_loc;  // [num_seqs + 1]
+  int64_t k_stride, v_stride;    // of rows, in elements
+  int32_t num_keys;
+};
+template <class QT>
+hipError_t launch_prompt(const PromptParams& p, int head_size, hipStream_t stream);
+
 struct F32;
 struct F16;
 struct BF16;

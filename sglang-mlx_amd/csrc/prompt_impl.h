@@ -1,0 +1,450 @@
+// Causal attention of packed prompts over their keys and values as rows, [tokens, heads,
+// head_size], the whole of a sequence or a sliding window and its first tokens.
+//
+// Sequence s brings n query tokens, the last n of its c key tokens: query i sits at
+// position p = c - n + i and sees the keys t <= p, of them only those with t > p - window
+// or t < sinks where there is a window.  A query row is one (token, head); the rows of the
+// heads that share a KV head are attended together, row r of a sequence being head
+// r % group of token r / group, so that they share the tiles of K and V.
+//
+// S^T = K Q^T and O^T = V^T P^T, as in extend_impl.h: a query row is a column of every
+// matrix, its maximum and sum are one register a lane, and the weights leave the first
+// product in the lanes where the second takes them.  K and V rows lie in LDS as they lie in
+// memory; the second product wants 8 tokens of a dimension in a lane, which the transposing
+// LDS read gives: of 16 lanes, lanes 4 k ..+3 name 16 elements of row k, and lane i
+// receives element i of the rows 0 .. 3.
+#pragma once
+
+#include "extend_impl.h"
+
+namespace pkv {
+
+constexpr int kPromptTile = 64;
+constexpr int kPromptThreads = 256;
+
+// 16-byte chunk c of row r of an image with ROW chunks a row sits at chunk
+// c ^ prompt_swizzle(r).  Reads meet no bank twice: 16 rows at one chunk (K) and 4 rows of
+// 4 chunks (V) both take the 256 bytes of all banks once.
+template <int ROW> __device__ __forceinline__ constexpr int prompt_swizzle(int r) {
+  return ROW >= 16 ? ((r & 3) << 2) | ((r >> 2) & 3) : ROW == 8 ? (((r >> 1) & 1) << 2) | ((r >> 2) & 3) : (r >> 2) & 3;
+}
+
+struct PromptSeq {
+  int start, count;  // query rows
+  int key, ctx;      // key rows
+};
+__device__ __forceinline__ PromptSeq prompt_seq(const PromptParams& p, int s) {
+  PromptSeq q;
+  q.start = min(max(p.query_start_loc[s], 0), p.num_tokens);
+  q.count = min(max(p.query_start_loc[s + 1], q.start), p.num_tokens) - q.start;
+  q.key = min(max(p.key_start_loc[s], 0), p.num_keys);
+  q.ctx = min(max(p.key_start_loc[s + 1], q.key), p.num_keys) - q.key;
+  return q;
+}
+
+// Bit i of 32: a query at position pos sees token a + i.
+__device__ __forceinline__ uint32_t seen32(int pos, int a, int window, int sinks) {
+  auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };
+  return below(pos + 1 - a) & (~below(pos - window + 1 - a) | below(sinks - a));
+}
+
+template <class QT, int D>
+__global__ __launch_bounds__(kPromptThreads, D <= 128 ? 2 : 1) void prompt_kernel(PromptParams p) {
+  using QS = typename Elem<QT>::storage;
+  constexpr int KSTEPS = (D + 15) / 16;  // score products per 32 tokens
+  constexpr int DT = (D + 31) / 32;      // 32-dimension tiles of the output
+  constexpr int ROW = D <= 32 ? 4 : D <= 64 ? 8 : D <= 128 ? 16 : 32;
+  constexpr int IMG = kPromptTile * ROW;
+  constexpr int LOADS = ROW / 4;  // 64-lane loads of a wavefront's 16 rows
+  // Arrays of their own: the compiler then knows that the loads in flight do not touch
+  // what is read.
+  __shared__ uint4 s_k0[IMG], s_k1[IMG], s_v0[IMG], s_v1[IMG];
+  __shared__ int s_seq[3], s_again;
+  using I0 = std::integral_constant<int, 0>;
+  using I1 = std::integral_constant<int, 1>;
+  auto k_image = [&](auto k) __attribute__((always_inline)) -> uint4* {
+    if constexpr (decltype(k)::value == 0) return s_k0;
+    else return s_k1;
+  };
+  auto v_image = [&](auto k) __attribute__((always_inline)) -> uint4* {
+    if constexpr (decltype(k)::value == 0) return s_v0;
+    else return s_v1;
+  };
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  const int kvh = blockIdx.x % p.num_kv_heads;
+  const int item = blockIdx.x / p.num_kv_heads;
+  const int items = gridDim.x / p.num_kv_heads;
+  const int split = blockIdx.y;
+  const int group = p.group, h0 = kvh * group;
+
+  // The workgroup's sequence and row tile: tiles of the sequences lie end to end, a
+  // sequence's last tile (the longest) first.
+  if (wave == 0) {
+    int base = 0, found = -1, z = 0;
+    for (int s0 = 0; s0 < p.num_seqs; s0 += 64) {
+      const int s = s0 + lane;
+      int tiles = 0;
+      if (s < p.num_seqs) tiles = (prompt_seq(p, s).count * group + kExtendRows - 1) / kExtendRows;
+      int sum = tiles;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int a = __shfl_up(sum, d);
+        if (lane >= d) sum += a;
+      }
+      const uint64_t past = __ballot(base + sum > item);
+      if (past) {
+        const int w = __builtin_ctzll(past);
+        found = s0 + w;
+        z = base + __shfl(sum, w) - 1 - item;  // counted from the sequence's first tile
+        break;
+      }
+      base += __shfl(sum, 63);
+    }
+    if (lane == 0) s_seq[0] = found, s_seq[1] = z, s_seq[2] = base, s_again = 0;
+  }
+  __syncthreads();
+  const int seq = __builtin_amdgcn_readfirstlane(s_seq[0]);
+  if (seq < 0) {
+    // Past the last tile: rows behind the last sequence become zeros.
+    const int tiles = s_seq[2];
+    if (split != 0) return;
+    const int last = min(max(p.query_start_loc[p.num_seqs], 0), p.num_tokens);
+    const int share = (p.num_tokens - last + items - tiles - 1) / (items - tiles);
+    const int64_t t0 = last + (int64_t)(item - tiles) * share;
+    zero_tokens<QT, kPromptThreads>(p, D, t0, min(t0 + share, (int64_t)p.num_tokens), h0, group);
+    return;
+  }
+  const int z = __builtin_amdgcn_readfirstlane(s_seq[1]);
+  const PromptSeq q = prompt_seq(p, seq);
+  const int first_pos = q.ctx - q.count;  // position of the sequence's first query token
+  const int rows = q.count * group;
+  const int row0 = z * kExtendRows;
+  const int row_end = min(row0 + kExtendRows, rows);
+  // Positions of the workgroup's rows; tokens before position 0 see nothing.
+  const int pmin = first_pos + row0 / group, pmax = first_pos + (row_end - 1) / group;
+
+  // This lane's row.
+  const int wr0 = row0 + wave * 32, wr1 = min(wr0 + 32, rows);
+  const int row = wr0 + col;
+  const bool live = row < rows;
+  const int tok = live ? row / group : 0;
+  const int head = h0 + (live ? row - tok * group : 0);
+  const int64_t qrow = q.start + tok;
+  const int pos = live ? first_pos + tok : -1;
+  // Positions of the wavefront's rows (uniform): none where w_min > w_max.
+  const bool w_any = wr0 < wr1;
+  const int w_min = w_any ? first_pos + wr0 / group : 0, w_max = w_any ? first_pos + (wr1 - 1) / group : -1;
+
+  // The tiles to visit: those of the sinks, then those of the window.
+  const int window = p.window > 0 ? p.window : 1 << 30;
+  const int sinks = p.window > 0 ? p.sinks : 0;
+  int lead = 0, base_tile = 0, ntiles = 0;
+  if (pmax >= 0) {
+    const int lo = max(0, max(pmin, 0) - window + 1);
+    lead = (min(sinks, lo) + kPromptTile - 1) / kPromptTile;
+    base_tile = max(lo / kPromptTile, lead);
+    ntiles = lead + max(0, pmax / kPromptTile + 1 - base_tile);
+  }
+  const int per = (ntiles + p.splits - 1) / p.splits;
+  const int v0 = min(split * per, ntiles), v1 = min(v0 + per, ntiles);
+  auto tile_start = [&](int v) { return (v < lead ? v : base_tile + v - lead) * kPromptTile; };
+
+  uint4 qf[KSTEPS];
+  const uint32_t sign = p.scale_log2 < 0.f ? 0x80008000u : 0u;  // (a negative scale goes into the queries)
+  const float scale = fmaxf(__builtin_fabsf(p.scale_log2), 0x1p-120f);
+  {
+    const QS* src = static_cast<const QS*>(p.q) + qrow * p.q_stride + (int64_t)head * D;
+#pragma unroll
+    for (int j = 0; j < KSTEPS; ++j) {
+      const int d = 16 * j + 8 * half;
+      const uint4 x = live && d < D ? *reinterpret_cast<const uint4*>(src + d) : make_uint4(0, 0, 0, 0);
+      qf[j] = make_uint4(x.x ^ sign, x.y ^ sign, x.z ^ sign, x.w ^ sign);
+    }
+  }
+  f32x16 o[DT];
+  float m, l;
+  auto reset = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
+    m = kNoScore;
+    l = 0.f;
+  };
+  reset();
+
+  // A wavefront stages rows 16 wave ..+15 of a tile of K or V, 16 bytes a lane; what
+  // lies behind the sequence, or behind a row, is zeros.
+  const char* k_rows = static_cast<const char*>(p.k_cache) + (q.key * p.k_stride + (int64_t)kvh * D) * 2;
+  const char* v_rows = static_cast<const char*>(p.v_cache) + (q.key * p.v_stride + (int64_t)kvh * D) * 2;
+  auto stage = [&](uint4* image, const char* rows_of, int64_t stride, int t0) __attribute__((always_inline)) {
+    const int r0 = 16 * wave;
+    const char* base = rows_of + (t0 + r0) * stride * 2;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int r = (64 * i + lane) / ROW, at = lane % ROW;  // (r0 does not change the swizzle)
+      const int c = at ^ prompt_swizzle<ROW>(r);
+      const char* src = base + (uint32_t)r * (uint32_t)(stride * 2) + 16 * c;
+      const bool have = t0 + r0 + r < q.ctx && (D == 8 * ROW || 8 * c < D);
+      load_to_lds(have ? (const void*)src : (const void*)&kNothing, image + r0 * ROW + 64 * i);
+    }
+  };
+  auto stage_k = [&](auto k, int v) __attribute__((always_inline)) {
+    if (v < v1) stage(k_image(k), k_rows, p.k_stride, tile_start(v));
+  };
+  auto stage_v = [&](auto k, int v) __attribute__((always_inline)) {
+    if (v < v1) stage(v_image(k), v_rows, p.v_stride, tile_start(v));
+  };
+  // The workgroup meets at a bare s_barrier, each wavefront's own loads and LDS accesses
+  // awaited before.
+  auto meet = [] __attribute__((always_inline)) {
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+    asm volatile("s_barrier" ::: "memory");
+  };
+
+  // S^T of the tile in image k: register r of sub is token 32 sub + r % 4 + 8 (r / 4) + 4 half.
+  const int k_swizzle = half ^ prompt_swizzle<ROW>(col);
+  auto scores = [&](auto k, f32x16 (&s)[2]) __attribute__((always_inline)) {
+    const uint4* ki = k_image(k) + col * ROW;
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[sub][r] = 0.f;
+#pragma unroll
+    for (int j = 0; j < KSTEPS; ++j)
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub)
+        s[sub] = mma32<QT>(ki[32 * sub * ROW + ((2 * j) ^ k_swizzle)], qf[j], s[sub]);
+  };
+  // Tokens 32 sub + 16 st + 8 i + 4 half ..+3, i = 0 and 1, of dimension 32 dt + col.
+  const int v_row = 4 * half + (lane % 16) / 4;
+  auto v_piece = [&](auto k, int dt, int sub, int st) __attribute__((always_inline)) {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    uint2 x[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = v_row + 8 * i, c = 4 * dt + 2 * ((lane / 16) % 2) + (lane % 4) / 2;
+      const uint4* chunk = v_image(k) + (32 * sub + 16 * st + r) * ROW + (c ^ prompt_swizzle<ROW>(r));
+      const char* at = reinterpret_cast<const char*>(chunk) + 8 * (lane & 1);
+      x[i] = __builtin_bit_cast(
+          uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at));
+    }
+    return make_uint4(x[0].x, x[0].y, x[1].x, x[1].y);
+  };
+  // Bits of a lane's 8 tokens of (sub, st) among the 32 of sub.
+  auto lane_bits = [&](uint32_t seen, int st) {
+    const uint32_t a = seen >> (16 * st + 4 * half);
+    return (a & 0xfu) | ((a >> 4) & 0xf0u);
+  };
+  auto mask = [&](f32x16 (&s)[2], int t0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub) {
+      const uint32_t sees = seen32(pos, t0 + 32 * sub, window, sinks) >> (4 * half);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[sub][r] = sees >> ((r & 3) + 8 * (r >> 2)) & 1u ? s[sub][r] : kNoScore;
+    }
+  };
+  // Moves the rows' reference points where the scores pass them by the slack.
+  auto refer = [&](const f32x16 (&s)[2]) __attribute__((always_inline)) {
+    float mt = kNoScore;
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[sub][r]);
+    mt = fmaxf(xchg32_max(mt), m);
+    if (__any(mt * scale > m * scale + kExtendSlack<QT> || (m == kNoScore && mt != kNoScore))) {
+      const float alpha = mt == kNoScore ? 1.f : __builtin_amdgcn_exp2f((m - mt) * scale);
+      m = mt;
+      l *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
+    }
+  };
+  auto weigh = [&](const f32x16 (&s)[2], uint32_t (&w)[2][8]) __attribute__((always_inline)) {
+    // (A row that has seen nothing keeps a finite reference point: no inf - inf.)
+    const float ref = (m == kNoScore ? 0.f : m * scale) - weight_shift<QT>(kExtendSlack<QT>);
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) {
+        const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[sub][r], scale, -ref));
+        const float b = __builtin_amdgcn_exp2f(__builtin_fmaf(s[sub][r + 1], scale, -ref));
+        l += a + b;
+        w[sub][r / 2] = pack_weights<QT>(a, b);
+      }
+  };
+  auto weights = [&](const uint32_t (&w)[2][8], int sub, int st) {
+    return make_uint4(w[sub][4 * st], w[sub][4 * st + 1], w[sub][4 * st + 2], w[sub][4 * st + 3]);
+  };
+  auto products = [&](auto k, const uint32_t (&w)[2][8]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+      for (int st = 0; st < 2; ++st)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[dt] = mma32<QT>(v_piece(k, dt, sub, st), weights(w, sub, st), o[dt]);
+  };
+  // A token that some rows do not see must not reach them, whatever its value, but a
+  // weight of 0 times inf or NaN is NaN.  A product with zeros tells whether a partly
+  // seen tile has such a value: the rows are then done again, with care.
+  auto test = [&](auto k) __attribute__((always_inline)) {
+    f32x16 zero;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) zero[r] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) zero = mma32<QT>(v_piece(k, dt, j >> 1, j & 1), make_uint4(0, 0, 0, 0), zero);
+    float sum = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sum += zero[r];
+    if (__any(sum != 0.f)) s_again = 1;
+  };
+  // One query position at a time, with the tokens that it does not see taken out of V;
+  // the other positions' rows keep their sums.
+  auto careful_products = [&](const uint32_t (&w)[2][8], int t0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll 1
+      for (int at = w_min; at <= w_max; ++at)
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub) {
+          const uint32_t keep = seen32(at, t0 + 32 * sub, window, sinks);
+          f32x16 n = o[dt];
+#pragma unroll
+          for (int st = 0; st < 2; ++st)
+            n = mma32<QT>(keep8(v_piece(I0{}, dt, sub, st), lane_bits(keep, st)), weights(w, sub, st), n);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[dt][r] = pos == at ? n[r] : o[dt][r];
+        }
+  };
+  // Whether any of the wavefront's rows sees a token of the tile, and whether all see all.
+  auto some_see = [&](int t0) { return w_max >= t0 && (t0 < sinks || t0 + kPromptTile > w_min - window + 1); };
+  auto all_see = [&](int t0) {
+    return t0 + kPromptTile - 1 <= w_min && (t0 > w_max - window || t0 + kPromptTile <= sinks);
+  };
+
+  // Tile v's weights and second product go beside tile v + 1's scores, while V of tile
+  // v + 1 and K of tile v + 2 load.
+  if (v0 < v1) {
+    f32x16 s[2];
+    stage_k(I0{}, v0);
+    stage_v(I0{}, v0);
+    stage_k(I1{}, v0 + 1);
+    meet();
+    auto ready = [&](auto k, int v) __attribute__((always_inline)) {
+      // Scores of tile v, in image k.
+      const int t0 = tile_start(v);
+      if (!some_see(t0)) return;
+      scores(k, s);
+      if (!all_see(t0)) mask(s, t0);
+    };
+    ready(I0{}, v0);
+    auto step = [&](auto k, int v) __attribute__((always_inline)) {
+      using KN = std::integral_constant<int, decltype(k)::value ^ 1>;
+      const int t0 = tile_start(v);
+      const bool seen = some_see(t0);
+      uint32_t w[2][8];
+      if (seen) {
+        refer(s);
+        weigh(s, w);
+      }
+      meet();  // V of tile v and K of tile v + 1 have landed; K of tile v and V of tile v - 1 have been read
+      stage_k(k, v + 2);
+      stage_v(KN{}, v + 1);
+      if (v + 1 < v1) ready(KN{}, v + 1);
+      if (seen) {
+        products(k, w);
+        if (!all_see(t0)) test(k);
+      }
+    };
+    for (int v = v0; v < v1; v += 2) {
+      step(I0{}, v);
+      if (v + 1 >= v1) break;
+      step(I1{}, v + 1);
+    }
+    meet();
+    if (__builtin_expect(s_again, 0)) {
+      reset();
+#pragma unroll 1
+      for (int v = v0; v < v1; ++v) {
+        const int t0 = tile_start(v);
+        meet();
+        stage_k(I0{}, v);
+        stage_v(I0{}, v);
+        meet();
+        if (!some_see(t0)) continue;
+        uint32_t w[2][8];
+        scores(I0{}, s);
+        mask(s, t0);
+        refer(s);
+        weigh(s, w);
+        careful_products(w, t0);
+      }
+    }
+  }
+
+  l = xchg32_sum(l);
+  if (!live) return;
+  if (p.splits == 1) {
+    const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;  // (NaN stays NaN)
+    QS* out = static_cast<QS*>(p.out) + (qrow * p.num_heads + head) * D;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int d = 32 * dt + 2 * r + 4 * half;
+        if (D % 32 != 0 && d >= D) continue;
+        uint2 x;
+        x.x = pack2(from_f32<QT>(o[dt][r] * inv), from_f32<QT>(o[dt][r + 1] * inv));
+        x.y = pack2(from_f32<QT>(o[dt][r + 2] * inv), from_f32<QT>(o[dt][r + 3] * inv));
+        *reinterpret_cast<uint2*>(out + d) = x;
+      }
+    return;
+  }
+  const int64_t at = (qrow * p.num_heads + head) * p.splits + split;
+  float* wo = p.ws_o + at * D;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int d = 32 * dt + 2 * r + 4 * half;
+      if (D % 32 != 0 && d >= D) continue;
+      *reinterpret_cast<float4*>(wo + d) = make_float4(o[dt][r], o[dt][r + 1], o[dt][r + 2], o[dt][r + 3]);
+    }
+  if (half == 0) *reinterpret_cast<float2*>(p.ws_ml + at * 2) = make_float2(m * scale, l);
+}
+
+template <class QT, int D> hipError_t launch_prompt_d(const PromptParams& p, hipStream_t stream) {
+  const int64_t items = extend_items(p.num_tokens, p.num_seqs, p.group);
+  hipLaunchKernelGGL((prompt_kernel<QT, D>), dim3((unsigned)(items * p.num_kv_heads), (unsigned)p.splits),
+                     dim3(kPromptThreads), 0, stream, p);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || p.splits == 1) return e;
+  const int64_t rows = (int64_t)p.num_tokens * p.num_heads;
+  hipLaunchKernelGGL((extend_merge_kernel<QT, D>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream,
+                     static_cast<const ExtendParams&>(p));
+  return hipGetLastError();
+}
+
+template <class QT> hipError_t launch_prompt(const PromptParams& p, int head_size, hipStream_t stream) {
+  switch (head_size) {
+    case 32: return launch_prompt_d<QT, 32>(p, stream);
+    case 64: return launch_prompt_d<QT, 64>(p, stream);
+    case 80: return launch_prompt_d<QT, 80>(p, stream);
+    case 96: return launch_prompt_d<QT, 96>(p, stream);
+    case 112: return launch_prompt_d<QT, 112>(p, stream);
+    case 120: return launch_prompt_d<QT, 120>(p, stream);
+    case 128: return launch_prompt_d<QT, 128>(p, stream);
+    case 192: return launch_prompt_d<QT, 192>(p, stream);
+    case 256: return launch_prompt_d<QT, 256>(p, stream);
+  }
+  return hipErrorInvalidValue;
+}
+
+}  // namespace pkv

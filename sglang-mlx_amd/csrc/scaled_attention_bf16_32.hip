@@ -1,0 +1,6 @@
+// Attention over caches with a scale per block and head: queries of type BF16, blocks of 32 tokens.
+#include "scaled_attention_impl.h"
+
+namespace pkv {
+template hipError_t launch_scaled_attention<BF16, 32>(const ScaledAttentionParams&, int, hipStream_t);
+}  // namespace pkv

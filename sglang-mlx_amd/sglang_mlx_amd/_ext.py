@@ -771,6 +771,278 @@ def paged_attention_extend(query, key_cache, value_cache, block_tables, seq_lens
                                 num_sinks, k_scale, v_scale)
 
 
+def _check_scaled_cache(key_cache, value_cache, kv_scales, num_kv_heads, head_size):
+    """Caches of E4M3 codes with a scale for each block and head; returns their block size."""
+    for t in (key_cache, value_cache, kv_scales):
+        _tensor(t)
+    if key_cache.dtype != torch.uint8 or value_cache.dtype != torch.uint8:
+        raise ValueError("key_cache and value_cache must be uint8 (FP8 E4M3 codes)")
+    if key_cache.dim() != 5 or value_cache.dim() != 4:
+        raise ValueError("key_cache/value_cache must use the paged layout")
+    nb, bs, x = key_cache.shape[0], key_cache.shape[3], 16
+    if head_size % x or tuple(key_cache.shape) != (nb, num_kv_heads, head_size // x, bs, x):
+        raise ValueError("key_cache must have shape [num_blocks, num_kv_heads, head_size/x, block_size, x]")
+    if tuple(value_cache.shape) != (nb, num_kv_heads, head_size, bs):
+        raise ValueError("value_cache must have shape [num_blocks, num_kv_heads, head_size, block_size]")
+    if head_size not in _HEAD_SIZES or bs not in _BLOCK_SIZES or nb == 0:
+        raise ValueError("Unsupported head_size/block_size for FP8 caches")
+    if (kv_scales.dtype != torch.float32 or tuple(kv_scales.shape) != (nb, num_kv_heads, 2)
+            or not kv_scales.is_contiguous()):
+        raise ValueError("kv_scales must be a contiguous float32 tensor [num_blocks, num_kv_heads, 2]")
+    return bs
+
+
+def _check_packed(start_loc, num_seqs, name="query_start_loc"):
+    _tensor(start_loc)
+    if start_loc.dim() != 1 or start_loc.shape[0] != num_seqs + 1:
+        raise ValueError(f"{name} must have shape [num_seqs + 1]")
+    _check_index(start_loc)
+
+
+def quantize_and_cache(key, value, key_cache, value_cache, kv_scales, block_tables, context_lens, query_start_loc):
+    """Appends each sequence's newest tokens to caches of E4M3 codes with a scale
+    for each block and head, in place; returns [key_cache, value_cache, kv_scales]
+    (rules: ``kernels.quantize_and_cache``)."""
+    if _native is not None:
+        out = _native.quantize_and_cache(key, value, key_cache, value_cache, kv_scales, block_tables, context_lens,
+                                         query_start_loc)
+        if _done(out):
+            return out
+    for t in (key, value, block_tables, context_lens):
+        _tensor(t)
+    if key.dim() != 3 or value.shape != key.shape:
+        raise ValueError("key and value must have shape [num_tokens, num_kv_heads, head_size]")
+    if value.dtype != key.dtype:
+        raise ValueError("key and value dtypes differ")
+    code = _dtype_code(key)
+    N, H, D = key.shape
+    bs = _check_scaled_cache(key_cache, value_cache, kv_scales, H, D)
+    if block_tables.dim() != 2 or context_lens.dim() != 1 or block_tables.shape[0] != context_lens.shape[0]:
+        raise ValueError("block_tables must be 2D and context_lens must be 1D, of the same sequences")
+    B = context_lens.shape[0]
+    _check_packed(query_start_loc, B)
+    _check_index(block_tables)
+    _check_index(context_lens)
+    if B > 0 and block_tables.shape[1] == 0:
+        raise ValueError("block_tables must have a column")
+    if not key_cache.is_contiguous() or not value_cache.is_contiguous():
+        raise ValueError("key_cache and value_cache must be contiguous (they are updated in place)")
+    dev = _on_gpu("QuantizeAndCache", key, value, key_cache, value_cache, kv_scales, block_tables, context_lens,
+                  query_start_loc)
+    if N == 0 or B == 0:
+        return [key_cache, value_cache, kv_scales]
+    key, k_stride = _aligned_rows(key)
+    value, v_stride = _aligned_rows(value)
+    bt, lens, start = _as_i32(block_tables), _as_i32(context_lens), _as_i32(query_start_loc)
+    lib = _lib.lib()
+    with torch.cuda.device(dev):
+        st = lib.pkv_quantize_and_cache(
+            key.data_ptr(), value.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), kv_scales.data_ptr(),
+            bt.data_ptr(), lens.data_ptr(), start.data_ptr(), N, B, H, D, bs, bt.shape[1], key_cache.shape[0],
+            k_stride, v_stride, code, _stream(dev))
+    _lib.check(st)
+    return [key_cache, value_cache, kv_scales]
+
+
+def dequantize_cache(key_cache, value_cache, kv_scales, block_tables, start_loc, num_tokens, dtype=torch.bfloat16):
+    """The first tokens of each sequence, packed, from caches of E4M3 codes with a
+    scale for each block and head (rules: ``kernels.dequantize_cache``)."""
+    if _native is not None:
+        out = _native.dequantize_cache(key_cache, value_cache, kv_scales, block_tables, start_loc, num_tokens, dtype)
+        if _done(out):
+            return out
+    for t in (key_cache, block_tables):
+        _tensor(t)
+    num_tokens = int(num_tokens)
+    if key_cache.dim() != 5:
+        raise ValueError("key_cache/value_cache must use the paged layout")
+    H, D = key_cache.shape[1], key_cache.shape[2] * key_cache.shape[4]
+    bs = _check_scaled_cache(key_cache, value_cache, kv_scales, H, D)
+    if dtype not in _DTYPE_CODE:
+        raise ValueError("Unsupported dtype")
+    if block_tables.dim() != 2:
+        raise ValueError("block_tables must be 2D")
+    B = block_tables.shape[0]
+    _check_packed(start_loc, B, "start_loc")
+    _check_index(block_tables)
+    if B > 0 and block_tables.shape[1] == 0:
+        raise ValueError("block_tables must have a column")
+    if num_tokens < 0 or num_tokens >= 1 << 31:
+        raise ValueError("num_tokens must be in [0, 2^31)")
+    if not key_cache.is_contiguous() or not value_cache.is_contiguous():
+        raise ValueError("key_cache and value_cache must be contiguous")
+    dev = _on_gpu("DequantizeCache", key_cache, value_cache, kv_scales, block_tables, start_loc)
+    k, v = (torch.empty((num_tokens, H, D), dtype=dtype, device=dev) for _ in range(2))
+    if num_tokens == 0 or H == 0:
+        return k, v
+    if B == 0:
+        return k.zero_(), v.zero_()
+    bt, start = _as_i32(block_tables), _as_i32(start_loc)
+    lib = _lib.lib()
+    with torch.cuda.device(dev):
+        st = lib.pkv_dequantize_cache(
+            k.data_ptr(), v.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), kv_scales.data_ptr(),
+            bt.data_ptr(), start.data_ptr(), num_tokens, B, H, D, bs, bt.shape[1], key_cache.shape[0],
+            _DTYPE_CODE[dtype], _stream(dev))
+    _lib.check(st)
+    return k, v
+
+
+def paged_attention_scaled(query, key_cache, value_cache, kv_scales, block_tables, seq_lens, query_start_loc,
+                           num_kv_heads, scale, block_size, max_seq_len, max_query_len=1, window=0, num_sinks=0):
+    """Attention of single and drafted tokens over caches of E4M3 codes with a
+    scale for each block and head (rules: ``kernels.paged_attention_scaled``)."""
+    if _native is not None:
+        out = _native.paged_attention_scaled(_ws_cache, query, key_cache, value_cache, kv_scales, block_tables,
+                                             seq_lens, query_start_loc, num_kv_heads, scale, block_size, max_seq_len,
+                                             max_query_len, window, num_sinks)
+        if _done(out):
+            return out
+    for t in (query, key_cache, value_cache, kv_scales, block_tables, seq_lens):
+        _tensor(t)
+    num_kv_heads, block_size, max_seq_len = int(num_kv_heads), int(block_size), int(max_seq_len)
+    max_query_len, window, num_sinks, scale = int(max_query_len), int(window), int(num_sinks), float(scale)
+    if query.dim() != 3:
+        raise ValueError("query must have shape [num_tokens, num_heads, head_size]")
+    N, Hq, D = query.shape
+    if num_kv_heads <= 0 or Hq == 0 or Hq % num_kv_heads:
+        raise ValueError("num_heads must be divisible by num_kv_heads")
+    if block_tables.dim() != 2 or seq_lens.dim() != 1:
+        raise ValueError("block_tables must be 2D and context_lens must be 1D")
+    B = seq_lens.shape[0]
+    if block_tables.shape[0] != B or (query_start_loc is None and N != B):
+        raise ValueError("query, block_tables, and context_lens sequence counts differ")
+    if query_start_loc is not None:
+        _check_packed(query_start_loc, B)
+    elif max_query_len != 1:
+        raise ValueError("without query_start_loc a call has one token per sequence")
+    if query.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"Unsupported query dtype for paged_attention_scaled: {query.dtype}")
+    bs = _check_scaled_cache(key_cache, value_cache, kv_scales, num_kv_heads, D)
+    if bs != block_size:
+        raise ValueError("cache block dimensions do not match block_size")
+    if key_cache.stride()[2:] != (bs * 16, 16, 1) or value_cache.stride()[2:] != (bs, 1):
+        raise ValueError("key_cache and value_cache must be contiguous within each (block, head) region")
+    if max_seq_len <= 0:
+        raise ValueError("max_seq_len must be positive")
+    if max_seq_len > block_tables.shape[1] * block_size:
+        raise ValueError("max_seq_len exceeds block table capacity")
+    if max_seq_len > 1 << 30:
+        raise ValueError("max_seq_len must be at most 2^30")
+    if max_query_len <= 0:
+        raise ValueError("max_query_len must be positive")
+    if window < 0 or num_sinks < 0:
+        raise ValueError("window and num_sinks must be non-negative")
+    if not math.isfinite(scale):
+        raise ValueError("scale must be finite")
+    # (Beyond the context, larger ones see no more; sequences have no more rows than the call.)
+    window, num_sinks = min(window, max_seq_len), min(num_sinks, max_seq_len)
+    max_query_len = min(max_query_len, max(N, 1))
+    _check_index(block_tables)
+    _check_index(seq_lens)
+    dev = _on_gpu("PagedAttentionScaled", query, key_cache, value_cache, kv_scales, block_tables, seq_lens,
+                  query_start_loc)
+    out = torch.empty((N, Hq, D), dtype=query.dtype, device=dev)
+    if N == 0:
+        return out
+    query, q_stride = _aligned_rows(query)
+    bt, lens = _as_i32(block_tables), _as_i32(seq_lens)
+    start = None if query_start_loc is None else _as_i32(query_start_loc)
+    lib = _lib.lib()
+    with torch.cuda.device(dev):
+        stream = _stream(dev)
+        need = lib.pkv_paged_attention_scaled_workspace_size(B, Hq, num_kv_heads, D, max_seq_len, max_query_len,
+                                                             window, num_sinks)
+        ws = _decode_scratch(dev, stream, need)
+        st = lib.pkv_paged_attention_scaled(
+            out.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), kv_scales.data_ptr(),
+            bt.data_ptr(), lens.data_ptr(), _ptr(start), N, B, Hq, num_kv_heads, D, block_size, bt.shape[1],
+            max_seq_len, max_query_len, window, num_sinks, key_cache.shape[0], scale, q_stride, key_cache.stride(0),
+            key_cache.stride(1), value_cache.stride(0), value_cache.stride(1), ws.data_ptr(), ws.numel(),
+            _DTYPE_CODE[query.dtype], stream)
+    _lib.check(st)
+    return out
+
+
+def prompt_attention(query, key, value, query_start_loc, scale, max_query_len, key_start_loc=None, max_key_len=None,
+                     window=0, num_sinks=0):
+    """Causal attention of packed prompts over their keys and values as rows
+    (rules: ``kernels.prompt_attention``)."""
+    if _native is not None:
+        out = _native.prompt_attention(_ws_cache, query, key, value, query_start_loc, scale, max_query_len,
+                                       key_start_loc, max_key_len, window, num_sinks)
+        if _done(out):
+            return out
+    for t in (query, key, value, query_start_loc):
+        _tensor(t)
+    _tensor(key_start_loc, allow_none=True)
+    max_query_len, window, num_sinks, scale = int(max_query_len), int(window), int(num_sinks), float(scale)
+    if query.dim() != 3:
+        raise ValueError("query must have shape [num_tokens, num_heads, head_size]")
+    if key.dim() != 3 or value.shape != key.shape:
+        raise ValueError("key and value must have shape [num_keys, num_kv_heads, head_size]")
+    N, Hq, D = query.shape
+    T, H = key.shape[:2]
+    if key.shape[2] != D:
+        raise ValueError("query and key head sizes differ")
+    if H == 0 or Hq == 0 or Hq % H:
+        raise ValueError("num_heads must be divisible by num_kv_heads")
+    if query.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"Unsupported dtype for prompt_attention: {query.dtype}")
+    if key.dtype != query.dtype or value.dtype != query.dtype:
+        raise ValueError("query, key and value dtypes differ")
+    if D not in _HEAD_SIZES:
+        raise ValueError("Unsupported head_size for prompt_attention")
+    if query_start_loc.dim() != 1 or query_start_loc.shape[0] == 0:
+        raise ValueError("query_start_loc must have shape [num_seqs + 1]")
+    B = query_start_loc.shape[0] - 1
+    _check_packed(query_start_loc, B)
+    if key_start_loc is None:
+        if T != N:
+            raise ValueError("without key_start_loc there are as many keys as queries")
+        if max_key_len is not None and int(max_key_len) != max_query_len:
+            raise ValueError("without key_start_loc max_key_len is max_query_len")
+        max_key_len = max_query_len
+    else:
+        _check_packed(key_start_loc, B, "key_start_loc")
+        if max_key_len is None:
+            raise ValueError("key_start_loc needs max_key_len")
+        max_key_len = int(max_key_len)
+    if max_query_len <= 0 or max_key_len <= 0:
+        raise ValueError("max_query_len and max_key_len must be positive")
+    if window < 0 or num_sinks < 0:
+        raise ValueError("window and num_sinks must be non-negative")
+    if not math.isfinite(scale):
+        raise ValueError("scale must be finite")
+    if T > 1 << 30:
+        raise ValueError("num_keys must be at most 2^30")
+    dev = _on_gpu("PromptAttention", query, key, value, query_start_loc, key_start_loc)
+    out = torch.empty((N, Hq, D), dtype=query.dtype, device=dev)
+    if N == 0:
+        return out
+    if B == 0 or T == 0:
+        return out.zero_()
+    query, q_stride = _aligned_rows(query)
+    key, k_stride = _aligned_rows(key)
+    value, v_stride = _aligned_rows(value)
+    start = _as_i32(query_start_loc)
+    key_start = None if key_start_loc is None else _as_i32(key_start_loc)
+    # (Beyond the rows at hand, larger ones say no more; the C entry takes 32 bits.)
+    window, num_sinks = min(window, 1 << 30), min(num_sinks, 1 << 30)
+    max_query_len, max_key_len = min(max_query_len, N), min(max_key_len, T)
+    lib = _lib.lib()
+    with torch.cuda.device(dev):
+        stream = _stream(dev)
+        need = lib.pkv_prompt_attention_workspace_size(N, B, Hq, H, D, max_query_len, max_key_len, window, num_sinks)
+        ws = _decode_scratch(dev, stream, need)
+        st = lib.pkv_prompt_attention(
+            out.data_ptr(), query.data_ptr(), key.data_ptr(), value.data_ptr(), start.data_ptr(), _ptr(key_start), N,
+            T, B, Hq, H, D, max_query_len, max_key_len, window, num_sinks, scale, q_stride, k_stride, v_stride,
+            ws.data_ptr(), ws.numel(), _DTYPE_CODE[query.dtype], stream)
+    _lib.check(st)
+    return out
+
+
 def _block_mapping(block_mapping) -> torch.Tensor:
     _tensor(block_mapping)
     if block_mapping.dim() != 2 or block_mapping.shape[1] != 2:

@@ -134,6 +134,32 @@ SIGNATURES = {
         _f32, _i64, _i64, _i64, _i64, _i64,                       # scale, q_stride, k/v block & head strides
         _c_void_p, _size, _i32, _i32,                             # workspace, bytes, q dtype, cache dtype
         _f32, _f32, _c_void_p]),                                  # k_scale, v_scale (FP8), stream
+    "pkv_quantize_and_cache": (ctypes.c_int, [
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,    # key, value, kc, vc, scales
+        _c_void_p, _c_void_p, _c_void_p,                          # block_tables, ctx, start_loc
+        _i32, _i32, _i32, _i32, _i32, _i32, _i64,                 # tokens, B, Hkv, D, bs, max_blocks, nb
+        _i64, _i64, _i32, _c_void_p]),                            # key/value stride, dtype, stream
+    "pkv_dequantize_cache": (ctypes.c_int, [
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,    # key_out, value_out, kc, vc, scales
+        _c_void_p, _c_void_p,                                     # block_tables, start_loc
+        _i32, _i32, _i32, _i32, _i32, _i32, _i64,                 # tokens, B, Hkv, D, bs, max_blocks, nb
+        _i32, _c_void_p]),                                        # dtype, stream
+    "pkv_paged_attention_scaled_workspace_size": (_size, [_i32] * 8),
+    "pkv_paged_attention_scaled": (ctypes.c_int, [
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,    # out, q, kc, vc, scales
+        _c_void_p, _c_void_p, _c_void_p,                          # block_tables, ctx, query_start_loc
+        _i32, _i32, _i32, _i32, _i32, _i32,                       # tokens, B, Hq, Hkv, D, bs
+        _i32, _i32, _i32, _i32, _i32, _i64,                       # max_blocks, max_seq, max_query, window, sinks, nb
+        _f32, _i64, _i64, _i64, _i64, _i64,                       # scale, q_stride, k/v block & head strides
+        _c_void_p, _size, _i32, _c_void_p]),                      # workspace, bytes, q dtype, stream
+    "pkv_prompt_attention_workspace_size": (_size, [_i32] * 9),
+    "pkv_prompt_attention": (ctypes.c_int, [
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p,               # out, query, key, value
+        _c_void_p, _c_void_p,                                     # query_start_loc, key_start_loc
+        _i32, _i32, _i32, _i32, _i32, _i32,                       # tokens, keys, B, Hq, Hkv, D
+        _i32, _i32, _i32, _i32, _f32,                             # max_query, max_key, window, sinks, scale
+        _i64, _i64, _i64,                                         # q/k/v stride
+        _c_void_p, _size, _i32, _c_void_p]),                      # workspace, bytes, dtype, stream
     "pkv_copy_blocks": (ctypes.c_int, [
         ctypes.POINTER(_c_void_p), ctypes.POINTER(_c_void_p), _i32,  # src/dst planes, count
         _i64, _i64, _i64,                                            # src/dst blocks, block bytes

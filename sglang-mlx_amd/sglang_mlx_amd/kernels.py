@@ -16,6 +16,12 @@ Operations:
     paged_attention_window  decode over a sliding window and a few first tokens
     paged_attention_extend  causal attention of several new tokens per sequence
                          (prefills, chunks of them, drafted tokens)
+    quantize_and_cache   append to FP8 caches with a scale for each block and
+                         head, which the append itself sets
+    dequantize_cache     keys and values back from such caches, packed
+    paged_attention_scaled  attention of single and drafted tokens over them
+    prompt_attention     causal attention of packed prompts over their keys and
+                         values as rows, no cache between
     copy_blocks          block copies inside the caches
     swap_blocks          block copies between two buffers
     convert_fp8          element-wise conversion with a scale, FP8 E4M3 codes
@@ -297,6 +303,144 @@ def paged_attention_extend(
     return _ext.paged_attention_extend(query, key_cache, value_cache, block_tables, context_lens, query_start_loc,
                                        num_kv_heads, scale, block_size, max_seq_len, max_query_len, window, num_sinks,
                                        k_scale, v_scale)
+
+
+def quantize_and_cache(
+    key: torch.Tensor,
+    value: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    kv_scales: torch.Tensor,
+    block_tables: torch.Tensor,
+    context_lens: torch.Tensor,
+    query_start_loc: torch.Tensor,
+) -> list[torch.Tensor]:
+    """Append of each sequence's newest tokens to FP8 caches with a scale for each
+    block and head.  No calibration: the append sets the scales.
+
+    Args:
+        key, value: [num_tokens, num_kv_heads, head_size], the sequences end to
+            end; float32, float16 or bfloat16; rows may be views of a projection
+        key_cache, value_cache: paged 5-D caches of uint8 (E4M3 codes, x = 16),
+            contiguous; head_size a multiple of 16
+        kv_scales: [num_blocks, num_kv_heads, 2] float32: a key code c stands for
+            c * kv_scales[block, head, 0], a value code for c * [..., 1]
+        block_tables: [num_seqs, max_blocks]; ids outside the cache drop tokens
+        context_lens: [num_seqs], tokens of each sequence with its new ones, which
+            are its last
+        query_start_loc: [num_seqs + 1], each sequence's first row, and the number
+            of rows; rows behind it go nowhere
+
+    A block that receives tokens gets, for each head and for K and V apart, the
+    least power of two that brings its largest finite new value to at most 240,
+    and at least the scale it had if it holds earlier tokens of the context; their
+    codes are brought to the new scale where it has grown (exactly, but for
+    subnormal codes).  New tokens at a block's first offset begin it anew.  Codes
+    round to nearest even; inf and NaN are stored as such.  The sequences of a call
+    write different blocks (copy a shared one first: ``copy_blocks`` for the
+    caches, ``swap_blocks(kv_scales, kv_scales, mapping)`` for the scales).
+
+    Returns [key_cache, value_cache, kv_scales], updated in place.
+    """
+    return _ext.quantize_and_cache(key, value, key_cache, value_cache, kv_scales, block_tables, context_lens,
+                                   query_start_loc)
+
+
+def dequantize_cache(
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    kv_scales: torch.Tensor,
+    block_tables: torch.Tensor,
+    start_loc: torch.Tensor,
+    num_tokens: int,
+    dtype: torch.dtype = torch.bfloat16,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Keys and values of the first tokens of each sequence, from caches that
+    ``quantize_and_cache`` wrote.
+
+    Args:
+        start_loc: [num_seqs + 1], from 0: rows [start_loc[s], start_loc[s + 1])
+            are tokens 0, 1, ... of sequence s
+        num_tokens: rows of the outputs
+        dtype: of the outputs (float32, float16 or bfloat16)
+        The others as ``quantize_and_cache``.
+
+    Returns:
+        key, value [num_tokens, num_kv_heads, head_size]: code * scale, rounded
+        once.  Rows without a block, and those behind the last sequence, are zero.
+    """
+    return _ext.dequantize_cache(key_cache, value_cache, kv_scales, block_tables, start_loc, num_tokens, dtype)
+
+
+def paged_attention_scaled(
+    query: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    kv_scales: torch.Tensor,
+    block_tables: torch.Tensor,
+    context_lens: torch.Tensor,
+    query_start_loc: torch.Tensor | None,
+    num_kv_heads: int,
+    scale: float,
+    block_size: int,
+    max_seq_len: int,
+    max_query_len: int = 1,
+    window: int = 0,
+    num_sinks: int = 0,
+) -> torch.Tensor:
+    """Causal attention of each sequence's newest tokens over the caches that
+    ``quantize_and_cache`` writes: single tokens (query_start_loc None or not) and
+    drafted ones.
+
+    bfloat16 or float16 queries; kv_scales may hold any finite scales that are not
+    negative.  The other arguments, the result and the rows that are zero are
+    ``paged_attention_extend``'s.  Every 16 query rows (tokens * num_heads /
+    num_kv_heads) of a sequence read its keys once, so this is for few of them: a
+    prompt's chunk takes less time through ``dequantize_cache`` and
+    ``prompt_attention``.
+    """
+    return _ext.paged_attention_scaled(query, key_cache, value_cache, kv_scales, block_tables, context_lens,
+                                       query_start_loc, num_kv_heads, scale, block_size, max_seq_len, max_query_len,
+                                       window, num_sinks)
+
+
+def prompt_attention(
+    query: torch.Tensor,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    query_start_loc: torch.Tensor,
+    scale: float,
+    max_query_len: int,
+    key_start_loc: torch.Tensor | None = None,
+    max_key_len: int | None = None,
+    window: int = 0,
+    num_sinks: int = 0,
+) -> torch.Tensor:
+    """Causal attention of packed prompts over their keys and values as they left
+    the projection (or, with key_start_loc, behind a context: as
+    ``dequantize_cache`` gives it).
+
+    Args:
+        query: [num_tokens, num_heads, head_size], the sequences end to end;
+            bfloat16 or float16; rows may be views of a projection
+        key, value: [num_keys, num_kv_heads, head_size], of the same type
+        query_start_loc: [num_seqs + 1], each sequence's first query row, and the
+            number of rows; output rows behind it are zero
+        scale: softmax scale
+        max_query_len: the most query rows of a sequence
+        key_start_loc: [num_seqs + 1], each sequence's first key row, and the number
+            of them: the n query rows of a sequence are its last n tokens.  None: the
+            keys are those of the queries
+        max_key_len: the most key rows of a sequence (with key_start_loc)
+        window, num_sinks: with a window > 0 a query sees the ``window`` last
+            tokens up to its own, and the sequence's first ``num_sinks``
+
+    Returns:
+        [num_tokens, num_heads, head_size]; a row that sees no key is zero.
+        max_query_len and max_key_len choose how the work is cut, not the result.
+    """
+    return _ext.prompt_attention(query, key, value, query_start_loc, scale, max_query_len, key_start_loc, max_key_len,
+                                 window, num_sinks)
 
 
 def copy_blocks(

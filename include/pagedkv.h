@@ -661,8 +661,8 @@ size_t pkv_paged_attention_scaled_workspace_size(int32_t num_seqs,
  * negative).  Made for few rows: every 16 rows (query tokens * num_heads /
  * num_kv_heads) of a sequence read its keys once; for a prompt's many rows,
  * pkv_dequantize_cache and pkv_prompt_attention take less.
- * num_seqs * num_kv_heads * ceil(rows / 16) * (max_seq_len / 32 + 4) stays below
- * 2^31.  One launch.
+ * Cache bases and strides are 16-byte aligned.  num_seqs * (max_seq_len / 64 +
+ * 5) stays below 2^31.  One launch.
  */
 int pkv_paged_attention_scaled(
     void* out, const void* query, const void* key_cache, const void* value_cache,

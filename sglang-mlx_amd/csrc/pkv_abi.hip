@@ -695,28 +695,29 @@ int scaled_cache_launch(const pkv::ScaledCacheParams& p, const char* where, void
   return PKV_OK;
 }
 
-// How pkv_paged_attention_scaled is cut: workgroups for the most tiles that its sizes
-// allow, each at least kScaledLeast long, and at most those that stay resident.
+// How pkv_paged_attention_scaled is cut: crews of a workgroup for each unit, as many as
+// the most tiles that its sizes allow keep busy, and no more workgroups than stay resident.
 struct ScaledCut {
-  int64_t slices, tiles, workgroups;  // tiles: of all items, each with its start (a bound)
+  int64_t slices, tiles, workgroups;  // tiles: of all sequences, each with its start (a bound)
 };
 ScaledCut scaled_cut(int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads, int64_t max_seq_len,
                      int64_t max_query_len, int64_t window, int64_t num_sinks) {
-  const int64_t slices = ceil_div(max_query_len * (num_heads / num_kv_heads), 16);
+  const int64_t slices = ceil_div(max_query_len * (num_heads / num_kv_heads), 16), units = num_kv_heads * slices;
   // (The window and the sinks each end inside a tile.)
-  int64_t tiles = ceil_div(max_seq_len, 32);
-  if (window > 0) tiles = std::min(tiles, ceil_div(window + max_query_len, 32) + ceil_div(num_sinks, 32) + 2);
-  const int64_t all = num_seqs * num_kv_heads * slices * (tiles + pkv::kScaledStart);
-  return {slices, all,
-          std::min<int64_t>(pkv::kScaledWorkgroups, std::max<int64_t>(ceil_div(all, pkv::kScaledLeast), 1))};
+  const int64_t T = pkv::kScaledTile;
+  int64_t tiles = ceil_div(max_seq_len, T);
+  if (window > 0) tiles = std::min(tiles, ceil_div(window + max_query_len, T) + ceil_div(num_sinks, T) + 2);
+  const int64_t all = num_seqs * (tiles + pkv::kScaledStart);
+  const int64_t crews = std::min(pkv::kScaledWorkgroups / units, ceil_div(all, pkv::kScaledLeast));
+  return {slices, all, std::max<int64_t>(crews, 1) * units};
 }
 struct ScaledWorkspace {
   size_t ml_bytes, total;
 };
 ScaledWorkspace scaled_workspace(const ScaledCut& cut, int64_t head_size) {
   const size_t rows = (size_t)cut.workgroups * 2 * 16;
-  return {rows * 4 * sizeof(float),
-          (size_t)pkv::kCounterBytes + rows * 4 * sizeof(float) + rows * head_size * sizeof(float)};
+  return {rows * 2 * sizeof(float),
+          (size_t)pkv::kCounterBytes + rows * 2 * sizeof(float) + rows * head_size * sizeof(float)};
 }
 
 // Parts of the keys of pkv_prompt_attention's row tiles: as many as make the launch fill
@@ -1093,7 +1094,7 @@ int pkv_paged_attention_scaled(void* out, const void* query, const void* key_cac
   // (Tiles and query rows are counted in 32 bits; HIP bounds a launch to 2^32 work-items.)
   if (cut.tiles >= ((int64_t)1 << 31) - pkv::kScaledLeast * pkv::kScaledWorkgroups ||
       (int64_t)num_tokens * num_heads >= ((int64_t)1 << 30) ||
-      (cut.workgroups + pkv::extend_tail_groups(num_tokens, num_heads, head_size, 1)) * 256 >= ((int64_t)1 << 32))
+      pkv::scaled_groups(cut.workgroups, num_tokens, num_seqs, num_heads, head_size, true) * 256 >= ((int64_t)1 << 32))
     return fail(PKV_ERR_UNSUPPORTED, "num_seqs * num_heads * max_seq_len exceeds what a launch counts");
   if (num_tokens == 0) return PKV_OK;
   if (!out || !query || !key_cache || !value_cache || !scales || (num_seqs > 0 && (!block_tables || !context_lens)))
@@ -1102,7 +1103,7 @@ int pkv_paged_attention_scaled(void* out, const void* query, const void* key_cac
   if (!aligned16(query) || (q_stride * 2) % 16 != 0 || q_stride < (int64_t)num_heads * head_size)
     return fail(PKV_ERR_INVALID, "query rows must be 16-byte aligned with stride >= num_heads * head_size");
   if (!aligned16(key_cache) || k_block_stride % 16 != 0 || k_head_stride % 16 != 0 ||
-      (reinterpret_cast<uintptr_t>(value_cache) % 8) != 0 || v_block_stride % 8 != 0 || v_head_stride % 8 != 0 ||
+      !aligned16(value_cache) || v_block_stride % 16 != 0 || v_head_stride % 16 != 0 ||
       (reinterpret_cast<uintptr_t>(scales) % 8) != 0)
     return fail(PKV_ERR_INVALID, "cache or scale bases or strides are not aligned for vector loads");
   const ScaledWorkspace w = scaled_workspace(cut, head_size);

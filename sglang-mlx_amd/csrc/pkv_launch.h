@@ -351,16 +351,23 @@ hipError_t launch_scaled_cache(const ScaledCacheParams& p, hipStream_t stream);
 
 // Attention of single and drafted tokens over caches with a scale for each block and
 // head (scaled_attention_impl.h; the rules of pkv_paged_attention_scaled).  Pieces'
-// states: per workgroup two slots of 16 rows, (max, sum, exponent) in ws_ml, outputs in
-// ws_o, and one arrival counter.
+// states: per workgroup two slots of 16 rows, (max, sum) in ws_ml, outputs in ws_o, and
+// one arrival counter.
 struct ScaledAttentionParams : ExtendParams {
   const float* scales;   // [num_blocks, H, 2]: K's, V's
   int32_t workgroups;
 };
-constexpr int kScaledStart = 4;    // what an item's start costs, in tiles
-constexpr int kScaledLeast = 8;    // the least span of a workgroup, in tiles
-constexpr int kScaledWorkgroups = 768;
+constexpr int kScaledTile = 64;    // tokens
+constexpr int kScaledStart = 5;    // what an item's start costs, in tiles
+constexpr int kScaledLeast = 9;    // the least span of a workgroup, in tiles
+constexpr int kScaledWorkgroups = 512;
 constexpr int kNoExponent = -300;  // below the exponent of every scale
+// Workgroups in all: behind those that attend, one for 256 sequences zeroes the rows of
+// sequences that have nothing to attend, and some the rows behind the last sequence.
+constexpr int64_t scaled_groups(int64_t workgroups, int64_t num_tokens, int64_t num_seqs, int64_t num_heads,
+                                int64_t head_size, bool packed) {
+  return workgroups + (num_seqs + 255) / 256 + (packed ? extend_tail_groups(num_tokens, num_heads, head_size, 1) : 0);
+}
 // (one block size a file, scaled_attention_<q>_<block size>.hip)
 template <class QT, int BS>
 hipError_t launch_scaled_attention(const ScaledAttentionParams& p, int head_size, hipStream_t stream);

@@ -1196,8 +1196,8 @@ int pkv_prompt_attention(void* out, const void* query, const void* key, const vo
   if (q_stride < (int64_t)num_heads * head_size || k_stride < row || v_stride < row)
     return fail(PKV_ERR_INVALID, "query/key/value row stride is smaller than a row");
   // (The kernel's offsets within 16 rows of keys are 32-bit.)
-  if (k_stride > (int64_t)1 << 26 || v_stride > (int64_t)1 << 26)
-    return fail(PKV_ERR_UNSUPPORTED, "key/value row stride must be at most 2^26 elements");
+  if (k_stride > (int64_t)1 << 24 || v_stride > (int64_t)1 << 24)
+    return fail(PKV_ERR_UNSUPPORTED, "key/value row stride must be at most 2^24 elements");
   const int32_t group = num_heads / num_kv_heads;
   const int64_t splits = prompt_splits(num_tokens, num_seqs, num_heads, num_kv_heads, max_query_len, max_key_len,
                                        window, num_sinks);

@@ -29,6 +29,24 @@ template <int ROW> __device__ __forceinline__ constexpr int prompt_swizzle(int r
   return ROW >= 16 ? ((r & 3) << 2) | ((r >> 2) & 3) : ROW == 8 ? (((r >> 1) & 1) << 2) | ((r >> 2) & 3) : (r >> 2) & 3;
 }
 
+// Over all 64 lanes, in every lane: within 16 by rotations, between them by exchanges.
+template <class OP> __device__ __forceinline__ int wave_all(int x, OP op) {
+  x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x128, 0xf, 0xf, true));  // row_ror:8
+  x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x124, 0xf, 0xf, true));
+  x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x122, 0xf, 0xf, true));
+  x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x121, 0xf, 0xf, true));
+  const auto a = __builtin_amdgcn_permlane16_swap((uint32_t)x, (uint32_t)x, false, false);
+  x = op((int)a[0], (int)a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap((uint32_t)x, (uint32_t)x, false, false);
+  return __builtin_amdgcn_readfirstlane(op((int)b[0], (int)b[1]));
+}
+__device__ __forceinline__ int wave_sum(int x) {
+  return wave_all(x, [](int a, int b) { return a + b; });
+}
+__device__ __forceinline__ int wave_max(int x) {
+  return wave_all(x, [](int a, int b) { return max(a, b); });
+}
+
 struct PromptSeq {
   int start, count;  // query rows
   int key, ctx;      // key rows
@@ -55,7 +73,8 @@ __global__ __launch_bounds__(kPromptThreads, D <= 128 ? 2 : 1) void prompt_kerne
   constexpr int DT = (D + 31) / 32;      // 32-dimension tiles of the output
   constexpr int ROW = D <= 32 ? 4 : D <= 64 ? 8 : D <= 128 ? 16 : 32;
   constexpr int IMG = kPromptTile * ROW;
-  constexpr int LOADS = ROW / 4;  // 64-lane loads of a wavefront's 16 rows
+  constexpr int SR = kPromptTile / 4;   // rows of a tile that a wavefront stages
+  constexpr int LOADS = SR * ROW / 64;  // and their 64-lane loads
   // Arrays of their own: the compiler then knows that the loads in flight do not touch
   // what is read.
   __shared__ uint4 s_k0[IMG], s_k1[IMG], s_v0[IMG], s_v1[IMG];
@@ -80,28 +99,35 @@ __global__ __launch_bounds__(kPromptThreads, D <= 128 ? 2 : 1) void prompt_kerne
   const int split = blockIdx.y;
   const int group = p.group, h0 = kvh * group;
 
-  // The workgroup's sequence and row tile: tiles of the sequences lie end to end, a
-  // sequence's last tile (the longest) first.
+  // The workgroup's sequence and row tile: of 64 sequences at a time, the tiles that lie
+  // furthest back in their sequences first (the longest, where all begin at position 0).
+  // (Sequence by sequence, each from its end, nine prompts of 155 .. 1665 tokens with 14
+  // heads of 64 took 50 us instead of 41: the last one's longest tiles ran alone.)
   if (wave == 0) {
     int base = 0, found = -1, z = 0;
     for (int s0 = 0; s0 < p.num_seqs; s0 += 64) {
       const int s = s0 + lane;
       int tiles = 0;
       if (s < p.num_seqs) tiles = (prompt_seq(p, s).count * group + kExtendRows - 1) / kExtendRows;
-      int sum = tiles;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const int a = __shfl_up(sum, d);
-        if (lane >= d) sum += a;
-      }
-      const uint64_t past = __ballot(base + sum > item);
-      if (past) {
-        const int w = __builtin_ctzll(past);
-        found = s0 + w;
-        z = base + __shfl(sum, w) - 1 - item;  // counted from the sequence's first tile
+      const int all = wave_sum(tiles);
+      if (item < base + all) {
+        // The last tile index of which more than `rank` tiles lie at it or behind it.
+        const int rank = item - base;
+        int lo = 0, hi = wave_max(tiles);  // (behind(lo) > rank >= behind(hi) = 0)
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) / 2;
+          if (wave_sum(max(tiles - mid, 0)) > rank) lo = mid;
+          else hi = mid;
+        }
+        z = lo;
+        const int nth = rank - wave_sum(max(tiles - lo - 1, 0));  // among the sequences that have tile z
+        const uint64_t have = __ballot(tiles > lo);
+        const bool mine = tiles > lo && __builtin_amdgcn_mbcnt_hi((uint32_t)(have >> 32),
+                                            __builtin_amdgcn_mbcnt_lo((uint32_t)have, 0)) == nth;
+        found = s0 + __builtin_ctzll(__ballot(mine));
         break;
       }
-      base += __shfl(sum, 63);
+      base += all;
     }
     if (lane == 0) s_seq[0] = found, s_seq[1] = z, s_seq[2] = base, s_again = 0;
   }
@@ -176,20 +202,43 @@ __global__ __launch_bounds__(kPromptThreads, D <= 128 ? 2 : 1) void prompt_kerne
   };
   reset();
 
-  // A wavefront stages rows 16 wave ..+15 of a tile of K or V, 16 bytes a lane; what
-  // lies behind the sequence, or behind a row, is zeros.
+  // Addresses that follow from the lane alone, made opaque to the compiler at each tile:
+  // it would otherwise hold what it derives from them in 80 registers over the loop.
+  //   k_at: of chunk 2 j + half of row col of K's image, but for j (which flips its bits);
+  //   v_at: of this lane's 8 bytes for the transposing read of rows 4 half .. (+ 8 i), dim 32 dt;
+  //   a row and a chunk of this lane's piece of a load.
+  uint32_t k_at = (lane & 31) * (ROW * 16) + 16 * (half ^ prompt_swizzle<ROW>(lane & 31)), v_at[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = 4 * half + (lane % 16) / 4 + 8 * i, c = 2 * ((lane / 16) % 2) + (lane % 4) / 2;
+    v_at[i] = r * (ROW * 16) + 16 * (c ^ prompt_swizzle<ROW>(r)) + 8 * (lane & 1);
+  }
+  constexpr int RL = 64 / ROW;  // rows of a load
+  uint32_t load_row = lane / ROW, load_chunk = lane % ROW;
+  auto lane_again = [&]() __attribute__((always_inline)) {
+    asm volatile("" : "+v"(k_at), "+v"(v_at[0]), "+v"(v_at[1]), "+v"(load_row), "+v"(load_chunk));
+  };
+  // A wavefront stages SR rows of a tile of K or V, 16 bytes a lane, by buffer loads: what
+  // lies behind the sequence's last row, or behind a row that is shorter than its image,
+  // is out of the buffer's range and becomes zeros.
   const char* k_rows = static_cast<const char*>(p.k_cache) + (q.key * p.k_stride + (int64_t)kvh * D) * 2;
   const char* v_rows = static_cast<const char*>(p.v_cache) + (q.key * p.v_stride + (int64_t)kvh * D) * 2;
   auto stage = [&](uint4* image, const char* rows_of, int64_t stride, int t0) __attribute__((always_inline)) {
-    const int r0 = 16 * wave;
-    const char* base = rows_of + (t0 + r0) * stride * 2;
+    const uint32_t bytes = (uint32_t)stride * 2;  // (64 rows stay below 2^31)
+    const int r0 = SR * wave;
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int r = (64 * i + lane) / ROW, at = lane % ROW;  // (r0 does not change the swizzle)
-      const int c = at ^ prompt_swizzle<ROW>(r);
-      const char* src = base + (uint32_t)r * (uint32_t)(stride * 2) + 16 * c;
-      const bool have = t0 + r0 + r < q.ctx && (D == 8 * ROW || 8 * c < D);
-      load_to_lds(have ? (const void*)src : (const void*)&kNothing, image + r0 * ROW + 64 * i);
+      // A buffer for each load, of the rows from its first on: the range check counts the
+      // lane's part of an offset, not the scalar part.
+      const int t = t0 + r0 + RL * i, rows_left = min(q.ctx - t, RL);
+      const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<char*>(rows_of + (int64_t)t * stride * 2), 0,
+          rows_left > 0 ? (int)((uint32_t)(rows_left - 1) * bytes + 2 * D) : 0, 0x00027000);
+      const uint32_t c = load_chunk ^ prompt_swizzle<ROW>(r0 + RL * i + load_row);
+      uint32_t at = load_row * bytes + 16 * c;
+      if (D != 8 * ROW) at = 8 * c < D ? at : 0xfffffff0u;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rsrc, (__attribute__((address_space(3))) void*)(image + r0 * ROW + 64 * i), 16, (int)at, 0, 0, 0);
     }
   };
   auto stage_k = [&](auto k, int v) __attribute__((always_inline)) {
@@ -205,32 +254,21 @@ __global__ __launch_bounds__(kPromptThreads, D <= 128 ? 2 : 1) void prompt_kerne
     asm volatile("s_barrier" ::: "memory");
   };
 
-  // S^T of the tile in image k: register r of sub is token 32 sub + r % 4 + 8 (r / 4) + 4 half.
-  const int k_swizzle = half ^ prompt_swizzle<ROW>(col);
-  auto scores = [&](auto k, f32x16 (&s)[2]) __attribute__((always_inline)) {
-    const uint4* ki = k_image(k) + col * ROW;
-#pragma unroll
-    for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[sub][r] = 0.f;
-#pragma unroll
-    for (int j = 0; j < KSTEPS; ++j)
-#pragma unroll
-      for (int sub = 0; sub < 2; ++sub)
-        s[sub] = mma32<QT>(ki[32 * sub * ROW + ((2 * j) ^ k_swizzle)], qf[j], s[sub]);
+  // Register r of sub of a tile's scores is token 32 sub + r % 4 + 8 (r / 4) + 4 half.  K's
+  // part of the product of dimensions 16 j ..+15 with tokens 32 sub ..+31:
+  auto k_piece = [&](auto k, int sub, int j) __attribute__((always_inline)) {
+    const char* at = reinterpret_cast<const char*>(k_image(k)) + 32 * sub * ROW * 16;
+    return *reinterpret_cast<const uint4*>(at + (k_at ^ (32 * j)));
   };
   // Tokens 32 sub + 16 st + 8 i + 4 half ..+3, i = 0 and 1, of dimension 32 dt + col.
-  const int v_row = 4 * half + (lane % 16) / 4;
   auto v_piece = [&](auto k, int dt, int sub, int st) __attribute__((always_inline)) {
     typedef short s16x4 __attribute__((ext_vector_type(4)));
     uint2 x[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int r = v_row + 8 * i, c = 4 * dt + 2 * ((lane / 16) % 2) + (lane % 4) / 2;
-      const uint4* chunk = v_image(k) + (32 * sub + 16 * st + r) * ROW + (c ^ prompt_swizzle<ROW>(r));
-      const char* at = reinterpret_cast<const char*>(chunk) + 8 * (lane & 1);
-      x[i] = __builtin_bit_cast(
-          uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at));
+      const char* at = reinterpret_cast<const char*>(v_image(k)) + (32 * sub + 16 * st) * ROW * 16;
+      x[i] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                           (__attribute__((address_space(3))) s16x4*)(at + (v_at[i] ^ (64 * dt)))));
     }
     return make_uint4(x[0].x, x[0].y, x[1].x, x[1].y);
   };
@@ -281,13 +319,48 @@ __global__ __launch_bounds__(kPromptThreads, D <= 128 ? 2 : 1) void prompt_kerne
   auto weights = [&](const uint32_t (&w)[2][8], int sub, int st) {
     return make_uint4(w[sub][4 * st], w[sub][4 * st + 1], w[sub][4 * st + 2], w[sub][4 * st + 3]);
   };
-  auto products = [&](auto k, const uint32_t (&w)[2][8]) __attribute__((always_inline)) {
+  // The products of a step: s = S^T of the tile in K's image kk (SCORES), then the outputs
+  // of the tile in V's image kv with the weights w (VALUES).  Pieces come from LDS four
+  // products ahead of their use; the fences keep them there (left to itself the compiler
+  // reads each right before its product and waits out LDS 32 times a tile: 870 instead of
+  // 1000 TFLOP/s for 8192 tokens with 32 heads of 128).
+  auto run_products = [&](auto kk, auto kv, auto scores, auto values, f32x16 (&s)[2], const uint32_t (&w)[2][8])
+                          __attribute__((always_inline)) {
+    constexpr int NS = decltype(scores)::value ? 2 * KSTEPS : 0, NV = decltype(values)::value ? 4 * DT : 0;
+    constexpr int N = NS + NV, G = 4;
+    auto piece = [&](int i) __attribute__((always_inline)) {
+      return i < NS ? k_piece(kk, i % 2, i / 2)
+                    : v_piece(kv, (i - NS) % DT, (i - NS) / DT / 2, (i - NS) / DT % 2);
+    };
+    uint4 x[2][G];
 #pragma unroll
-    for (int sub = 0; sub < 2; ++sub)
+    for (int i = 0; i < G; ++i)
+      if (i < N) x[0][i] = piece(i);
+    if (NS > 0)
 #pragma unroll
-      for (int st = 0; st < 2; ++st)
+      for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[dt] = mma32<QT>(v_piece(k, dt, sub, st), weights(w, sub, st), o[dt]);
+        for (int r = 0; r < 16; ++r) s[sub][r] = 0.f;
+#pragma unroll
+    for (int i0 = 0; i0 < N; i0 += G) {
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < G; ++i)
+        if (i0 + G + i < N) x[(i0 / G + 1) % 2][i] = piece(i0 + G + i);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        const int n = i0 + i;
+        if (n >= N) continue;
+        if (n < NS) {
+          s[n % 2] = mma32<QT>(x[i0 / G % 2][i], qf[n / 2], s[n % 2]);
+        } else {
+          const int at = n - NS, dt = at % DT, sub = at / DT / 2, st = at / DT % 2;
+          o[dt] = mma32<QT>(x[i0 / G % 2][i], weights(w, sub, st), o[dt]);
+        }
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
   };
   // A token that some rows do not see must not reach them, whatever its value, but a
   // weight of 0 times inf or NaN is NaN.  A product with zeros tells whether a partly
@@ -329,44 +402,70 @@ __global__ __launch_bounds__(kPromptThreads, D <= 128 ? 2 : 1) void prompt_kerne
     return t0 + kPromptTile - 1 <= w_min && (t0 > w_max - window || t0 + kPromptTile <= sinks);
   };
 
-  // Tile v's weights and second product go beside tile v + 1's scores, while V of tile
-  // v + 1 and K of tile v + 2 load.
+  // A step takes tile v's weights on the vector units, then tile v + 1's scores and tile
+  // v's second product in one run on the matrix units, while V of tile v + 1 and K of tile
+  // v + 2 load.
   if (v0 < v1) {
     f32x16 s[2];
+    uint32_t w[2][8];
+    // Tiles [first_whole, last_whole) are seen in full by every row: behind the sinks'
+    // tiles and the window's edge, before the first row's position.
+    const int first_whole = lead + max(0, (max(pmax - window + 1, 0) + kPromptTile - 1) / kPromptTile - base_tile);
+    const int last_whole = min(v1, lead + (pmin + 1) / kPromptTile - base_tile);
     stage_k(I0{}, v0);
     stage_v(I0{}, v0);
     stage_k(I1{}, v0 + 1);
     meet();
-    auto ready = [&](auto k, int v) __attribute__((always_inline)) {
-      // Scores of tile v, in image k.
-      const int t0 = tile_start(v);
-      if (!some_see(t0)) return;
-      scores(k, s);
-      if (!all_see(t0)) mask(s, t0);
-    };
-    ready(I0{}, v0);
+    if (some_see(tile_start(v0))) run_products(I0{}, I0{}, std::true_type{}, std::false_type{}, s, w);
     auto step = [&](auto k, int v) __attribute__((always_inline)) {
       using KN = std::integral_constant<int, decltype(k)::value ^ 1>;
       const int t0 = tile_start(v);
-      const bool seen = some_see(t0);
-      uint32_t w[2][8];
-      if (seen) {
-        refer(s);
-        weigh(s, w);
-      }
+      lane_again();
       meet();  // V of tile v and K of tile v + 1 have landed; K of tile v and V of tile v - 1 have been read
       stage_k(k, v + 2);
       stage_v(KN{}, v + 1);
-      if (v + 1 < v1) ready(KN{}, v + 1);
+      const bool seen = some_see(t0), sees = v + 1 < v1 && some_see(tile_start(v + 1));
       if (seen) {
-        products(k, w);
-        if (!all_see(t0)) test(k);
+        if (!all_see(t0)) mask(s, t0);
+        refer(s);
+        weigh(s, w);
       }
+      if (seen && sees) {
+        run_products(KN{}, k, std::true_type{}, std::true_type{}, s, w);
+      } else if (seen) {
+        run_products(KN{}, k, std::false_type{}, std::true_type{}, s, w);
+      } else if (sees) {
+        run_products(KN{}, k, std::true_type{}, std::false_type{}, s, w);
+      }
+      if (seen && !all_see(t0)) test(k);
     };
-    for (int v = v0; v < v1; v += 2) {
+    // The same where every row of the workgroup sees both tiles in full: no branch but
+    // that of a moved reference point.  (In one loop with the others, the outputs were
+    // copied between registers where their ways meet, at each tile.)
+    auto whole_step = [&](auto k, int v) __attribute__((always_inline)) {
+      using KN = std::integral_constant<int, decltype(k)::value ^ 1>;
+      lane_again();
+      meet();
+      stage_k(k, v + 2);
+      stage_v(KN{}, v + 1);
+      refer(s);
+      weigh(s, w);
+      run_products(KN{}, k, std::true_type{}, std::true_type{}, s, w);
+    };
+    int v = v0;
+    while (v < v1) {
+      if (v >= first_whole) {
+#pragma unroll 1
+        while (v + 2 < last_whole) {
+          whole_step(I0{}, v);
+          whole_step(I1{}, v + 1);
+          v += 2;
+        }
+      }
       step(I0{}, v);
-      if (v + 1 >= v1) break;
-      step(I1{}, v + 1);
+      if (++v >= v1) break;
+      step(I1{}, v);
+      ++v;
     }
     meet();
     if (__builtin_expect(s_again, 0)) {
@@ -379,8 +478,7 @@ __global__ __launch_bounds__(kPromptThreads, D <= 128 ? 2 : 1) void prompt_kerne
         stage_v(I0{}, v);
         meet();
         if (!some_see(t0)) continue;
-        uint32_t w[2][8];
-        scores(I0{}, s);
+        run_products(I0{}, I0{}, std::true_type{}, std::false_type{}, s, w);
         mask(s, t0);
         refer(s);
         weigh(s, w);

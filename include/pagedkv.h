@@ -598,8 +598,8 @@ int pkv_convert_fp8(void* dst, const void* src, int64_t num_elements,
  *            become the codes of inf and NaN;
  * and where that scale is larger than the block's, the codes of its earlier
  * tokens c become c * (block's scale / scale), rounded the same way.
- * Nothing else of the caches and scales changes.  Sequences of a call write
- * different blocks; a block id outside [0, num_blocks) drops its tokens, and so
+ * Nothing else of the caches and scales changes.  No block receives tokens at two
+ * places of a call's tables; a block id outside [0, num_blocks) drops its tokens, and so
  * does a context beyond max_num_blocks_per_seq * block_size, rows behind the last
  * sequence go nowhere.  The scale of a block that holds earlier tokens is finite
  * and positive.
@@ -662,7 +662,7 @@ size_t pkv_paged_attention_scaled_workspace_size(int32_t num_seqs,
  * num_kv_heads) of a sequence read its keys once; for a prompt's many rows,
  * pkv_dequantize_cache and pkv_prompt_attention take less.
  * Cache bases and strides are 16-byte aligned.  num_seqs * (max_seq_len / 64 +
- * 5) stays below 2^31.  One launch.
+ * 5) stays below 2^31, max_query_len * num_heads below 2^28.  One launch.
  */
 int pkv_paged_attention_scaled(
     void* out, const void* query, const void* key_cache, const void* value_cache,
@@ -705,8 +705,9 @@ size_t pkv_prompt_attention_workspace_size(int32_t num_tokens, int32_t num_seqs,
  * query [num_tokens, num_heads, head_size], key, value [num_keys, num_kv_heads,
  * head_size], all of type dtype (BF16 or F16), row strides q_stride, k_stride and
  * v_stride, the inner two dimensions contiguous, rows 16-byte aligned.  out:
- * contiguous, 16-byte aligned.  key_start_loc may be NULL: query_start_loc (with
- * num_keys = num_tokens).  max_query_len, max_key_len: the most rows of a
+ * contiguous, 16-byte aligned.  k_stride and v_stride are at most 2^24, num_tokens *
+ * num_heads is below 2^30, num_keys at most 2^30.  key_start_loc may be NULL:
+ * query_start_loc (with num_keys = num_tokens).  max_query_len, max_key_len: the most rows of a
  * sequence; they choose how the work is cut, not the result.
  * head_size in {32,64,80,96,112,120,128,192,256}.  One launch, or two where few
  * rows meet many keys.

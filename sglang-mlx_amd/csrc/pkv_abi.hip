@@ -678,8 +678,8 @@ int scaled_cache_args(pkv::ScaledCacheParams& p, const void* key_cache, const vo
   p.block_shift = block_size == 8 ? 3 : block_size == 16 ? 4 : 5;
   p.max_blocks_per_seq = max_num_blocks_per_seq;
   p.dtype = dtype;
-  // (HIP bounds a launch to 2^32 work-items.)
-  if (pkv::scaled_cache_groups(p) * 256 >= ((int64_t)1 << 32))
+  // (HIP bounds a launch to 2^32 work-items; heads apart, so that the product stays in 64 bits.)
+  if (num_kv_heads > 1 << 20 || pkv::scaled_cache_groups(p) * 256 >= ((int64_t)1 << 32))
     return fail(PKV_ERR_UNSUPPORTED, "num_tokens * num_kv_heads exceeds the launch grid limit");
   if (num_tokens == 0) return PKV_OK;
   if (!key_cache || !value_cache || !scales || !start_loc || (num_seqs > 0 && !block_tables))
@@ -1088,12 +1088,11 @@ int pkv_paged_attention_scaled(void* out, const void* query, const void* key_cac
   const float scale_log2 = scale * 1.4426950408889634f;
   if (!std::isfinite(scale_log2)) return fail(PKV_ERR_INVALID, "scale must be finite");
   if (num_blocks <= 0) return fail(PKV_ERR_INVALID, "num_blocks must be positive");
-  max_query_len = std::min(max_query_len, std::max(num_tokens, 1));  // (no sequence has more rows)
   const ScaledCut cut =
       scaled_cut(num_seqs, num_heads, num_kv_heads, max_seq_len, max_query_len, window, num_sinks);
   // (Tiles and query rows are counted in 32 bits; HIP bounds a launch to 2^32 work-items.)
   if (cut.tiles >= ((int64_t)1 << 31) - pkv::kScaledLeast * pkv::kScaledWorkgroups ||
-      (int64_t)num_tokens * num_heads >= ((int64_t)1 << 30) ||
+      (int64_t)num_tokens * num_heads >= ((int64_t)1 << 30) || cut.workgroups >= ((int64_t)1 << 24) ||
       pkv::scaled_groups(cut.workgroups, num_tokens, num_seqs, num_heads, head_size, true) * 256 >= ((int64_t)1 << 32))
     return fail(PKV_ERR_UNSUPPORTED, "num_seqs * num_heads * max_seq_len exceeds what a launch counts");
   if (num_tokens == 0) return PKV_OK;
@@ -1202,8 +1201,8 @@ int pkv_prompt_attention(void* out, const void* query, const void* key, const vo
   const int64_t splits = prompt_splits(num_tokens, num_seqs, num_heads, num_kv_heads, max_query_len, max_key_len,
                                        window, num_sinks);
   // (HIP bounds a launch to 2^32 work-items; rows of a sequence are counted in 32 bits.)
-  if (pkv::extend_items(num_tokens, num_seqs, group) * num_kv_heads * splits * 256 >= ((int64_t)1 << 32) ||
-      (int64_t)num_tokens * num_heads >= ((int64_t)1 << 30))
+  if ((int64_t)num_tokens * num_heads >= ((int64_t)1 << 30) || (int64_t)num_seqs * num_kv_heads >= ((int64_t)1 << 30) ||
+      pkv::extend_items(num_tokens, num_seqs, group) * num_kv_heads * splits * 256 >= ((int64_t)1 << 32))
     return fail(PKV_ERR_UNSUPPORTED, "num_tokens * num_heads exceeds the launch grid limit");
   if (num_tokens == 0) return PKV_OK;
   if (!out || !query || (num_keys > 0 && (!key || !value)) || !query_start_loc)

@@ -224,7 +224,7 @@ __global__ __launch_bounds__(kPromptThreads, D <= 128 ? 2 : 1) void prompt_kerne
   const char* k_rows = static_cast<const char*>(p.k_cache) + (q.key * p.k_stride + (int64_t)kvh * D) * 2;
   const char* v_rows = static_cast<const char*>(p.v_cache) + (q.key * p.v_stride + (int64_t)kvh * D) * 2;
   auto stage = [&](uint4* image, const char* rows_of, int64_t stride, int t0) __attribute__((always_inline)) {
-    const uint32_t bytes = (uint32_t)stride * 2;  // (64 rows stay below 2^31)
+    const uint32_t bytes = (uint32_t)stride * 2;  // (16 rows stay below 2^31)
     const int r0 = SR * wave;
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {

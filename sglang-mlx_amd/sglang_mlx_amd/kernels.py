@@ -327,7 +327,7 @@ def quantize_and_cache(
             c * kv_scales[block, head, 0], a value code for c * [..., 1]
         block_tables: [num_seqs, max_blocks]; ids outside the cache drop tokens
         context_lens: [num_seqs], tokens of each sequence with its new ones, which
-            are its last
+            are its last; a context that its table cannot hold drops all of them
         query_start_loc: [num_seqs + 1], each sequence's first row, and the number
             of rows; rows behind it go nowhere
 
@@ -336,9 +336,9 @@ def quantize_and_cache(
     and at least the scale it had if it holds earlier tokens of the context; their
     codes are brought to the new scale where it has grown (exactly, but for
     subnormal codes).  New tokens at a block's first offset begin it anew.  Codes
-    round to nearest even; inf and NaN are stored as such.  The sequences of a call
-    write different blocks (copy a shared one first: ``copy_blocks`` for the
-    caches, ``swap_blocks(kv_scales, kv_scales, mapping)`` for the scales).
+    round to nearest even; inf and NaN are stored as such.  No block receives tokens
+    at two places of a call's tables (copy a shared one first: ``copy_blocks`` for
+    the caches, ``swap_blocks(kv_scales, kv_scales, mapping)`` for the scales).
 
     Returns [key_cache, value_cache, kv_scales], updated in place.
     """

@@ -32,33 +32,46 @@ constexpr int kScaledWaves = 4;  // per workgroup
 // end, sequence s from start_loc[s] / bs + extra * s on (a sum that grows by at least
 // the blocks that n tokens touch: n / bs + 1 from a block's start on, + 2 from
 // anywhere).  The last s whose items begin at or before `item`, by 64 probes at a time.
+// The last round's probes hold the sequence's own numbers, its context (or null: none)
+// among them.
 struct Found {
-  int seq, start, count, nth;
+  int seq, start, count, ctx, nth;
 };
-__device__ __forceinline__ Found find_item(const int32_t* start_loc, int num_seqs, int num_tokens, int shift, int extra,
-                                           int item) {
+__device__ __forceinline__ Found find_item(const int32_t* start_loc, const int32_t* context_lens, int num_seqs,
+                                           int num_tokens, int shift, int extra, int item) {
   const int lane = threadIdx.x & 63;
   auto at = [&](int s) { return s > num_seqs ? num_tokens : min(max(start_loc[s], 0), num_tokens); };
+  auto before = [&](int s, int loc) { return (loc >> shift) + extra * s <= item; };
   int lo = 0, hi = num_seqs + 1;  // (the rows behind the last sequence are one more)
-  while (hi - lo > 1) {
+  while (hi - lo > 63) {
     const int step = (hi - lo + 63) / 64;
     const int s = lo + lane * step;
-    const bool before = s < hi && (at(s) >> shift) + extra * s <= item;
-    const int n = max(__popcll(__ballot(before)), 1);
+    const bool yes = s < hi && before(s, at(min(s, hi)));
+    const int n = max(__popcll(__ballot(yes)), 1);
     lo += (n - 1) * step;
     hi = min(lo + step, hi);
   }
+  const int s = lo + lane, loc = at(min(s, num_seqs + 1));
+  const int ctx = context_lens != nullptr && s < num_seqs ? context_lens[s] : 0;
+  const int n = max(__popcll(__ballot(s < hi && before(s, loc))), 1);
   Found f;
-  f.seq = __builtin_amdgcn_readfirstlane(lo);
-  f.start = __builtin_amdgcn_readfirstlane(at(f.seq));
-  f.count = max(__builtin_amdgcn_readfirstlane(at(f.seq + 1)) - f.start, 0);
+  f.seq = lo + n - 1;
+  f.start = __builtin_amdgcn_readlane(loc, n - 1);
+  f.count = max(__builtin_amdgcn_readlane(loc, n) - f.start, 0);  // (n < 64: hi - lo is)
+  f.ctx = __builtin_amdgcn_readlane(ctx, n - 1);
   f.nth = item - ((f.start >> shift) + extra * f.seq);
   return f;
 }
 
-__device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-  for (int d = 1; d < 16; d <<= 1) x = fmaxf(x, __shfl_xor(x, d));
+__device__ __forceinline__ float wave_max(float x) {  // (not NaN)
+  auto turned = [&](auto by) {
+    const int i = __builtin_bit_cast(int, x);
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(i, i, 0x120 + decltype(by)::value, 0xf, 0xf, true));
+  };
+  x = fmaxf(x, turned(std::integral_constant<int, 8>{}));
+  x = fmaxf(x, turned(std::integral_constant<int, 4>{}));
+  x = fmaxf(x, turned(std::integral_constant<int, 2>{}));
+  x = fmaxf(x, turned(std::integral_constant<int, 1>{}));
   return xchg32_max(xchg16_max(x));
 }
 
@@ -154,20 +167,83 @@ template <class S> __device__ __forceinline__ Pair<S> no_pair() {
   return p;
 }
 
-__device__ __forceinline__ uint32_t byte_of(const uint32_t* w, int i) { return (w[i >> 2] >> (8 * (i & 3))) & 0xffu; }
+// The largest size among pairs, by their bits: sizes order as integers do, those of inf
+// and NaN behind the finite ones.
+template <class S> struct Largest {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  static constexpr uint32_t kInf = std::is_same<S, BF16>::value ? 0x7f80u : std::is_same<S, F16>::value ? 0x7c00u
+                                                                                                        : 0x7f800000u;
+  uint32_t m = 0;
+  __device__ __forceinline__ void add(const Pair<S>& x) {
+    if constexpr (std::is_same<S, F32>::value)
+      m = max(m, max(__float_as_uint(x.a) & 0x7fffffffu, __float_as_uint(x.b) & 0x7fffffffu));
+    else
+      m = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, m),
+                                                                 __builtin_bit_cast(u16x2, x.w & 0x7fff7fffu)));
+  }
+  __device__ __forceinline__ uint32_t bits() const {
+    return std::is_same<S, F32>::value ? m : max(m & 0xffffu, m >> 16);
+  }
+  __device__ __forceinline__ bool finite() const { return bits() < kInf; }
+  __device__ __forceinline__ float value() const {
+    if constexpr (std::is_same<S, F32>::value) return __uint_as_float(m);
+    else if constexpr (std::is_same<S, BF16>::value) return __uint_as_float(bits() << 16);
+    else return f16_bits_to_f32(bits());
+  }
+};
+
+// The largest finite size of a wavefront's pairs; odd: whether any is inf or NaN.
+template <class S, int A, int B>
+__device__ __forceinline__ float largest_of(const Pair<S> (&x)[A][B], bool& odd) {
+  Largest<S> most;
+#pragma unroll
+  for (int i = 0; i < A; ++i)
+#pragma unroll
+    for (int j = 0; j < B; ++j) most.add(x[i][j]);
+  odd = __ballot(!most.finite()) != 0;
+  float a = most.value();
+  if (__builtin_expect(odd, 0)) {
+    a = 0.f;
+#pragma unroll
+    for (int i = 0; i < A; ++i)
+#pragma unroll
+      for (int j = 0; j < B; ++j) a = fmaxf(a, fmaxf(finite_size(x[i][j].lo()), finite_size(x[i][j].hi())));
+  }
+  return wave_max(a);
+}
+
+// Codes of four values: QUICK where all are finite and the scale is a power of two.
+template <bool QUICK>
+__device__ __forceinline__ uint32_t codes_of(const Divide& by, float a, float b, float c, float d) {
+  if constexpr (QUICK) {
+    const int w = __builtin_amdgcn_cvt_pk_fp8_f32(a * by.inv, b * by.inv, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c * by.inv, d * by.inv, w, true);
+  } else {
+    const float q[4] = {by(a), by(b), by(c), by(d)};
+    return encode4(q);
+  }
+}
 
 }  // namespace
 
 // BS tokens a block; NS: 128-dimension slices of a head.
 //
-// Bound: HBM.  A lane of K's wavefronts holds 16 dimensions of a token (two loads, one
-// 16-byte store; the wavefront's stores are contiguous), one of V's two dimensions of
-// all tokens (256 bytes a load, BS contiguous bytes a dimension).
+// Bound: HBM for a prompt, the chain of dependent loads (sequence, rows and block, old
+// scale) for single tokens.  A lane of K's wavefronts holds 16 dimensions of a token (two
+// loads, one 16-byte store; the wavefront's stores are contiguous), one of V's two
+// dimensions of all tokens (256 bytes a load, BS contiguous bytes a dimension).  Four
+// wavefronts a workgroup: with eight, 23 prompts of 14000 tokens in all took 29.2 us
+// instead of 26.6; with two, the way back of 32000 tokens 41.4 instead of 38.5.
 template <class S, int BS, int NS>
 __global__ __launch_bounds__(64 * kScaledWaves) void quantize_kernel(ScaledCacheParams p) {
   constexpr int SHIFT = BS == 8 ? 3 : BS == 16 ? 4 : 5;
   constexpr int NU = (NS * BS + 7) / 8;  // (token, 16 dimensions) units of a lane
   constexpr int W = BS / 4;              // words of a row of V
+  // Up to so many tokens a wavefront takes one after the other (with the code below for a
+  // block's worth, most of it for tokens that are not there, 200 sequences took 12.2 us
+  // instead of 4.9 for a token each, 8.8 instead of 7.8 for four, 12.3 instead of 11.4 for
+  // eight; 4 heads of 128, then 8).
+  constexpr int FEW = 8;
   using SS = typename Elem<S>::storage;
   const int lane = threadIdx.x & 63;
   const int64_t wave = (int64_t)blockIdx.x * kScaledWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -175,29 +251,86 @@ __global__ __launch_bounds__(64 * kScaledWaves) void quantize_kernel(ScaledCache
   const int is_v = (int)(wave & 1);
   const int head = (int)((wave >> 1) % H);
   const int item = (int)((wave >> 1) / H);
-  const Found f = find_item(p.start_loc, p.num_seqs, p.num_tokens, SHIFT, 2, item);
+  const Found f = find_item(p.start_loc, p.context_lens, p.num_seqs, p.num_tokens, SHIFT, 2, item);
   if (f.seq >= p.num_seqs || f.count == 0) return;
-  const uint32_t ctx = (uint32_t)p.context_lens[f.seq];
+  const uint32_t ctx = (uint32_t)f.ctx;
   if (ctx == 0 || ctx > (uint64_t)p.max_blocks_per_seq * BS) return;
   // Token i of the sequence sits at position first + i; those before position 0 nowhere.
   const int64_t first = (int64_t)ctx - f.count;
   const int64_t block = (max(first, (int64_t)0) >> SHIFT) + f.nth;
   if (block * BS >= ctx) return;
+  // (The rows are asked for before the block's id is there.)
   const int32_t id = p.block_tables[(int64_t)f.seq * p.max_blocks_per_seq + block];
-  if (id < 0 || id >= p.num_blocks) return;
   const int o0 = (int)(max(max(first, (int64_t)0), block * BS) - block * BS);
   const int o1 = (int)(min((int64_t)ctx, (block + 1) * BS) - block * BS);
   const int64_t row0 = f.start + (block * BS + o0 - first) - o0;  // row of offset o is row0 + o
-  float* scale_at = p.scales + ((int64_t)id * H + head) * 2 + is_v;
-  const float before = o0 > 0 ? *scale_at : 0.f;
-  uint8_t* region = static_cast<uint8_t*>(is_v ? p.v_cache : p.k_cache) + ((int64_t)id * H + head) * D * BS;
-
-  // The block's scale from its largest new value, and the codes it holds brought to it.
-  auto settle = [&](float a) { return fmaxf(scale_for(wave_max(a)), before); };
+  const bool in_cache = id >= 0 && id < p.num_blocks;
+  const int64_t at = (int64_t)id * H + head;
+  float* scale_at = p.scales + at * 2 + is_v;
+  uint8_t* region = static_cast<uint8_t*>(is_v ? p.v_cache : p.k_cache) + at * D * BS;
+  // Brings the earlier tokens' codes to a larger scale, a word a lane: of K four dimensions,
+  // of V up to four tokens of a dimension.
+  auto regrow = [&](float before, const Divide& by) __attribute__((always_inline)) {
+#pragma unroll 1
+    for (int i = lane; i < D * BS / 4; i += 64) {
+      const int t = is_v ? 4 * i & (BS - 1) : (i >> 2) & (BS - 1);
+      if (t >= o0) continue;
+      uint32_t* to = reinterpret_cast<uint32_t*>(region) + i;
+      const uint32_t now = rescale4(*to, before, by);
+      if (!is_v || t + 4 <= o0) {
+        *to = now;
+        continue;
+      }
+#pragma unroll
+      for (int k = 0; k < 3; ++k)
+        if (t + k < o0) reinterpret_cast<uint8_t*>(to)[k] = (uint8_t)(now >> (8 * k));
+    }
+  };
+  bool odd;
+  if (o1 - o0 <= FEW && o1 - o0 < BS) {
+    // A few tokens: two dimensions a lane.
+    const int64_t stride = is_v ? p.value_stride : p.key_stride;
+    const SS* src = static_cast<const SS*>(is_v ? p.value : p.key) + (row0 + o0) * stride + (int64_t)head * D;
+    const int n = o1 - o0;
+    Pair<S> x[FEW][NS];
+#pragma unroll
+    for (int t = 0; t < FEW; ++t)
+#pragma unroll
+      for (int j = 0; j < NS; ++j) {
+        const int d = 2 * lane + 128 * j;
+        x[t][j] = no_pair<S>();
+        if (t < n && d < D) x[t][j] = *reinterpret_cast<const Pair<S>*>(src + t * stride + d);
+      }
+    if (!in_cache) return;
+    const float before = o0 > 0 ? *scale_at : 0.f;
+    const float scale = fmaxf(scale_for(largest_of(x, odd)), before);
+    const Divide by(scale);
+    const bool grown = o0 > 0 && scale != before;
+    if (grown) regrow(before, by);
+    auto write = [&](auto quick) __attribute__((always_inline)) {
+#pragma unroll
+      for (int t = 0; t < FEW; ++t)
+#pragma unroll
+        for (int j = 0; j < NS; ++j) {
+          const int d = 2 * lane + 128 * j;
+          if (t >= n || d >= D) continue;
+          const uint32_t w = codes_of<decltype(quick)::value>(by, x[t][j].lo(), x[t][j].hi(), 0.f, 0.f);
+          if (is_v) {
+            region[d * BS + o0 + t] = (uint8_t)w;
+            region[(d + 1) * BS + o0 + t] = (uint8_t)(w >> 8);
+          } else {
+            *reinterpret_cast<uint16_t*>(region + ((d >> 4) * BS + o0 + t) * 16 + (d & 15)) = (uint16_t)w;
+          }
+        }
+    };
+    if (!odd && by.inv != 0.f) write(std::true_type{});
+    else write(std::false_type{});
+    if (lane == 0 && (o0 == 0 || grown)) *scale_at = scale;
+    return;
+  }
   if (!is_v) {
     const SS* src = static_cast<const SS*>(p.key) + row0 * p.key_stride + (int64_t)head * D;
     Pair<S> x[NU][8];
-    float a = 0.f;
 #pragma unroll
     for (int j = 0; j < NU; ++j) {
       const int u = lane + 64 * j, c = u >> SHIFT, t = u & (BS - 1);
@@ -213,39 +346,32 @@ __global__ __launch_bounds__(64 * kScaledWaves) void quantize_kernel(ScaledCache
         }
       }
     }
-#pragma unroll
-    for (int j = 0; j < NU; ++j)
-#pragma unroll
-      for (int k = 0; k < 8; ++k) a = fmaxf(a, fmaxf(finite_size(x[j][k].lo()), finite_size(x[j][k].hi())));
-    const float scale = settle(a);
+    if (!in_cache) return;
+    const float before = o0 > 0 ? *scale_at : 0.f;
+    const float scale = fmaxf(scale_for(largest_of(x, odd)), before);
     const Divide by(scale);
     const bool grown = o0 > 0 && scale != before;
+    auto write = [&](auto quick) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < NU; ++j) {
-      const int u = lane + 64 * j, c = u >> SHIFT, t = u & (BS - 1);
-      if (16 * c >= D) continue;
-      uint4* to = reinterpret_cast<uint4*>(region) + u;
-      if (t >= o0 && t < o1) {
+      for (int j = 0; j < NU; ++j) {
+        const int u = lane + 64 * j, c = u >> SHIFT, t = u & (BS - 1);
+        if (16 * c >= D || t < o0 || t >= o1) continue;
         uint32_t w[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float q[4] = {by(x[j][2 * k].lo()), by(x[j][2 * k].hi()), by(x[j][2 * k + 1].lo()),
-                              by(x[j][2 * k + 1].hi())};
-          w[k] = encode4(q);
-        }
-        *to = make_uint4(w[0], w[1], w[2], w[3]);
-      } else if (grown && t < o0) {
-        const uint4 was = *to;
-        *to = make_uint4(rescale4(was.x, before, by), rescale4(was.y, before, by), rescale4(was.z, before, by),
-                         rescale4(was.w, before, by));
+        for (int k = 0; k < 4; ++k)
+          w[k] = codes_of<decltype(quick)::value>(by, x[j][2 * k].lo(), x[j][2 * k].hi(), x[j][2 * k + 1].lo(),
+                                                  x[j][2 * k + 1].hi());
+        reinterpret_cast<uint4*>(region)[u] = make_uint4(w[0], w[1], w[2], w[3]);
       }
-    }
+    };
+    if (!odd && by.inv != 0.f) write(std::true_type{});
+    else write(std::false_type{});
+    if (grown) regrow(before, by);
     if (lane == 0 && (o0 == 0 || grown)) *scale_at = scale;
     return;
   }
   const SS* src = static_cast<const SS*>(p.value) + row0 * p.value_stride + (int64_t)head * D;
   Pair<S> x[NS][BS];
-  float a = 0.f;
 #pragma unroll
   for (int j = 0; j < NS; ++j) {
     const int d = 2 * lane + 128 * j;
@@ -255,52 +381,44 @@ __global__ __launch_bounds__(64 * kScaledWaves) void quantize_kernel(ScaledCache
       if (d < D && t >= o0 && t < o1) x[j][t] = *reinterpret_cast<const Pair<S>*>(src + t * p.value_stride + d);
     }
   }
-#pragma unroll
-  for (int j = 0; j < NS; ++j)
-#pragma unroll
-    for (int t = 0; t < BS; ++t) a = fmaxf(a, fmaxf(finite_size(x[j][t].lo()), finite_size(x[j][t].hi())));
-  const float scale = settle(a);
+  if (!in_cache) return;
+  const float before = o0 > 0 ? *scale_at : 0.f;
+  const float scale = fmaxf(scale_for(largest_of(x, odd)), before);
   const Divide by(scale);
   const bool grown = o0 > 0 && scale != before;
   const bool whole = o0 == 0 && o1 == BS;
+  auto write = [&](auto quick) __attribute__((always_inline)) {
 #pragma unroll
-  for (int j = 0; j < NS; ++j) {
-    const int d = 2 * lane + 128 * j;
-    if (d >= D) continue;
+    for (int j = 0; j < NS; ++j) {
+      const int d = 2 * lane + 128 * j;
+      if (d >= D) continue;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      uint32_t* row = reinterpret_cast<uint32_t*>(region + (int64_t)(d + i) * BS);
-      uint32_t w[W];
+      for (int i = 0; i < 2; ++i) {
+        uint32_t* row = reinterpret_cast<uint32_t*>(region + (d + i) * BS);
+        auto value = [&](int t) { return i == 0 ? x[j][t].lo() : x[j][t].hi(); };
+        uint32_t w[W];
 #pragma unroll
-      for (int k = 0; k < W; ++k) {
-        float q[4];
+        for (int k = 0; k < W; ++k)
+          w[k] = codes_of<decltype(quick)::value>(by, value(4 * k), value(4 * k + 1), value(4 * k + 2), value(4 * k + 3));
+        if (whole) {
+          if constexpr (W == 2)
+            *reinterpret_cast<uint2*>(row) = make_uint2(w[0], w[1]);
+          else
 #pragma unroll
-        for (int t = 0; t < 4; ++t) q[t] = by(i == 0 ? x[j][4 * k + t].lo() : x[j][4 * k + t].hi());
-        w[k] = encode4(q);
-      }
-      if (whole) {
-        if constexpr (W == 2)
-          *reinterpret_cast<uint2*>(row) = make_uint2(w[0], w[1]);
-        else
-#pragma unroll
-          for (int k = 0; k < W; k += 4) *reinterpret_cast<uint4*>(row + k) = make_uint4(w[k], w[k + 1], w[k + 2], w[k + 3]);
-        continue;
-      }
-#pragma unroll
-      for (int k = 0; k < W; ++k) {
-        // (Offsets behind the new tokens stay as they were.)
-        if (grown && 4 * k < o0) {
-          const uint32_t old = rescale4(row[k], before, by);
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-            if (4 * k + t < o0) reinterpret_cast<uint8_t*>(row)[4 * k + t] = (uint8_t)(old >> (8 * t));
+            for (int k = 0; k < W; k += 4)
+              *reinterpret_cast<uint4*>(row + k) = make_uint4(w[k], w[k + 1], w[k + 2], w[k + 3]);
+          continue;
         }
+        // (Offsets behind the new tokens stay as they were.)
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
-          if (4 * k + t >= o0 && 4 * k + t < o1) reinterpret_cast<uint8_t*>(row)[4 * k + t] = (uint8_t)(w[k] >> (8 * t));
+        for (int t = 0; t < BS; ++t)
+          if (t >= o0 && t < o1) reinterpret_cast<uint8_t*>(row)[t] = (uint8_t)(w[t / 4] >> (8 * (t % 4)));
       }
     }
-  }
+  };
+  if (!odd && by.inv != 0.f) write(std::true_type{});
+  else write(std::false_type{});
+  if (grown) regrow(before, by);
   if (lane == 0 && (o0 == 0 || grown)) *scale_at = scale;
 }
 
@@ -328,7 +446,7 @@ __global__ __launch_bounds__(64 * kScaledWaves) void dequantize_kernel(ScaledCac
   const int is_v = (int)(wave & 1);
   const int head = (int)((wave >> 1) % H);
   const int item = (int)((wave >> 1) / H);
-  const Found f = find_item(p.start_loc, p.num_seqs, p.num_tokens, SHIFT, 1, item);
+  const Found f = find_item(p.start_loc, nullptr, p.num_seqs, p.num_tokens, SHIFT, 1, item);
   if ((int64_t)f.nth * BS >= f.count) return;
   const int n = min(f.count - f.nth * BS, BS);
   int32_t id = -1;

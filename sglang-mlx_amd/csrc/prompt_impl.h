@@ -206,7 +206,7 @@ __global__ __launch_bounds__(kPromptThreads, D <= 128 ? 2 : 1) void prompt_kerne
   // it would otherwise hold what it derives from them in 80 registers over the loop.
   //   k_at: of chunk 2 j + half of row col of K's image, but for j (which flips its bits);
   //   v_at: of this lane's 8 bytes for the transposing read of rows 4 half .. (+ 8 i), dim 32 dt;
-  //   a row and a chunk of this lane's piece of a load.
+  //   k_row, v_row, load_chunk: this lane's row in the first load of a tile, its 16 bytes there.
   uint32_t k_at = (lane & 31) * (ROW * 16) + 16 * (half ^ prompt_swizzle<ROW>(lane & 31)), v_at[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -214,38 +214,42 @@ __global__ __launch_bounds__(kPromptThreads, D <= 128 ? 2 : 1) void prompt_kerne
     v_at[i] = r * (ROW * 16) + 16 * (c ^ prompt_swizzle<ROW>(r)) + 8 * (lane & 1);
   }
   constexpr int RL = 64 / ROW;  // rows of a load
-  uint32_t load_row = lane / ROW, load_chunk = lane % ROW;
+  const int load_row = SR * wave + lane / ROW;
+  uint32_t k_row = load_row * (uint32_t)p.k_stride * 2, v_row = load_row * (uint32_t)p.v_stride * 2;
+  uint32_t load_chunk = 16 * ((lane % ROW) ^ prompt_swizzle<ROW>(load_row));
   auto lane_again = [&]() __attribute__((always_inline)) {
-    asm volatile("" : "+v"(k_at), "+v"(v_at[0]), "+v"(v_at[1]), "+v"(load_row), "+v"(load_chunk));
+    asm volatile("" : "+v"(k_at), "+v"(v_at[0]), "+v"(v_at[1]), "+v"(k_row), "+v"(v_row), "+v"(load_chunk));
   };
   // A wavefront stages SR rows of a tile of K or V, 16 bytes a lane, by buffer loads: what
   // lies behind the sequence's last row, or behind a row that is shorter than its image,
-  // is out of the buffer's range and becomes zeros.
+  // is out of the buffer's range and becomes zeros.  (One buffer a tile: with one for each
+  // load their scalar instructions took 568 us instead of 554 for 8192 tokens.)
   const char* k_rows = static_cast<const char*>(p.k_cache) + (q.key * p.k_stride + (int64_t)kvh * D) * 2;
   const char* v_rows = static_cast<const char*>(p.v_cache) + (q.key * p.v_stride + (int64_t)kvh * D) * 2;
-  auto stage = [&](uint4* image, const char* rows_of, int64_t stride, int t0) __attribute__((always_inline)) {
-    const uint32_t bytes = (uint32_t)stride * 2;  // (16 rows stay below 2^31)
-    const int r0 = SR * wave;
+  auto stage = [&](uint4* image, const char* rows_of, int64_t stride, uint32_t row_at, int t0)
+                   __attribute__((always_inline)) {
+    const uint32_t bytes = (uint32_t)stride * 2;  // (64 rows stay below 2^31)
+    const int rows_left = min(q.ctx - t0, kPromptTile);
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<char*>(rows_of + (int64_t)t0 * stride * 2), 0,
+        rows_left > 0 ? (int)((uint32_t)(rows_left - 1) * bytes + 2 * D) : 0, 0x00027000);
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      // A buffer for each load, of the rows from its first on: the range check counts the
-      // lane's part of an offset, not the scalar part.
-      const int t = t0 + r0 + RL * i, rows_left = min(q.ctx - t, RL);
-      const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(
-          const_cast<char*>(rows_of + (int64_t)t * stride * 2), 0,
-          rows_left > 0 ? (int)((uint32_t)(rows_left - 1) * bytes + 2 * D) : 0, 0x00027000);
-      const uint32_t c = load_chunk ^ prompt_swizzle<ROW>(r0 + RL * i + load_row);
-      uint32_t at = load_row * bytes + 16 * c;
-      if (D != 8 * ROW) at = 8 * c < D ? at : 0xfffffff0u;
+      // (A load's rows and a wavefront's have their bits apart: the swizzles add up.)  The
+      // whole offset stands in the lane's part of the address: the range check counts that
+      // part, not the scalar one.
+      const uint32_t c = load_chunk ^ (16 * prompt_swizzle<ROW>(RL * i));
+      uint32_t at = row_at + RL * i * bytes + c;
+      if (D != 8 * ROW) at = c < 2 * D ? at : 0xfffffff0u;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          rsrc, (__attribute__((address_space(3))) void*)(image + r0 * ROW + 64 * i), 16, (int)at, 0, 0, 0);
+          rsrc, (__attribute__((address_space(3))) void*)(image + SR * wave * ROW + 64 * i), 16, (int)at, 0, 0, 0);
     }
   };
   auto stage_k = [&](auto k, int v) __attribute__((always_inline)) {
-    if (v < v1) stage(k_image(k), k_rows, p.k_stride, tile_start(v));
+    if (v < v1) stage(k_image(k), k_rows, p.k_stride, k_row, tile_start(v));
   };
   auto stage_v = [&](auto k, int v) __attribute__((always_inline)) {
-    if (v < v1) stage(v_image(k), v_rows, p.v_stride, tile_start(v));
+    if (v < v1) stage(v_image(k), v_rows, p.v_stride, v_row, tile_start(v));
   };
   // The workgroup meets at a bare s_barrier, each wavefront's own loads and LDS accesses
   // awaited before.
@@ -441,7 +445,8 @@ __global__ __launch_bounds__(kPromptThreads, D <= 128 ? 2 : 1) void prompt_kerne
     };
     // The same where every row of the workgroup sees both tiles in full: no branch but
     // that of a moved reference point.  (In one loop with the others, the outputs were
-    // copied between registers where their ways meet, at each tile.)
+    // copied between registers where their ways meet, at each tile.)  The products come
+    // first on a SIMD whose other wavefront takes weights: 544 us instead of 552.
     auto whole_step = [&](auto k, int v) __attribute__((always_inline)) {
       using KN = std::integral_constant<int, decltype(k)::value ^ 1>;
       lane_again();
@@ -450,7 +455,9 @@ __global__ __launch_bounds__(kPromptThreads, D <= 128 ? 2 : 1) void prompt_kerne
       stage_v(KN{}, v + 1);
       refer(s);
       weigh(s, w);
+      __builtin_amdgcn_s_setprio(1);
       run_products(KN{}, k, std::true_type{}, std::true_type{}, s, w);
+      __builtin_amdgcn_s_setprio(0);
     };
     int v = v0;
     while (v < v1) {

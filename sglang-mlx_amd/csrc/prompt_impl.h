@@ -434,13 +434,10 @@ __global__ __launch_bounds__(kPromptThreads, D <= 128 ? 2 : 1) void prompt_kerne
         refer(s);
         weigh(s, w);
       }
-      if (seen && sees) {
-        run_products(KN{}, k, std::true_type{}, std::true_type{}, s, w);
-      } else if (seen) {
-        run_products(KN{}, k, std::false_type{}, std::true_type{}, s, w);
-      } else if (sees) {
-        run_products(KN{}, k, std::true_type{}, std::false_type{}, s, w);
-      }
+      // (With a third way, both in one run, what they share was copied between registers: 18
+      // us instead of 12 for 23 tokens at head size 256, 264 instead of 205 for 4096.)
+      if (seen) run_products(KN{}, k, std::false_type{}, std::true_type{}, s, w);
+      if (sees) run_products(KN{}, k, std::true_type{}, std::false_type{}, s, w);
       if (seen && !all_see(t0)) test(k);
     };
     // The same where every row of the workgroup sees both tiles in full: no branch but

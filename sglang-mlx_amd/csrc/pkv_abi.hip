@@ -708,7 +708,7 @@ ScaledCut scaled_cut(int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads, 
   int64_t tiles = ceil_div(max_seq_len, T);
   if (window > 0) tiles = std::min(tiles, ceil_div(window + max_query_len, T) + ceil_div(num_sinks, T) + 2);
   const int64_t all = num_seqs * (tiles + pkv::kScaledStart);
-  const int64_t crews = std::min(pkv::kScaledWorkgroups / units, ceil_div(all, pkv::kScaledLeast));
+  const int64_t crews = std::min(pkv::kScaledWorkgroups / units, std::max(ceil_div(all, pkv::kScaledLeast), num_seqs));
   return {slices, all, std::max<int64_t>(crews, 1) * units};
 }
 struct ScaledWorkspace {

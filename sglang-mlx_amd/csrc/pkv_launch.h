@@ -360,6 +360,7 @@ struct ScaledAttentionParams : ExtendParams {
 constexpr int kScaledTile = 64;    // tokens
 constexpr int kScaledStart = 5;    // what an item's start costs, in tiles
 constexpr int kScaledLeast = 9;    // the least span of a workgroup, in tiles
+constexpr int kScaledWhole = 13;   // the longest item, its start with it, of sequences that get a crew each
 constexpr int kScaledWorkgroups = 512;
 constexpr int kNoExponent = -300;  // below the exponent of every scale
 // Workgroups in all: behind those that attend, one for 256 sequences zeroes the rows of

@@ -115,6 +115,17 @@ def test_schedule(B):
     c.check(c.call(start=False))
 
 
+@pytest.mark.parametrize("B,Hq,H", [(1, 8, 2), (5, 32, 8), (64, 32, 8), (65, 32, 8), (256, 4, 2), (257, 4, 2)])
+@pytest.mark.parametrize("longest", [64, 512, 513])
+def test_short_sequences(B, Hq, H, longest):
+    """On both sides of the rule that gives each its own workgroups: their number, their longest."""
+    ctx = [(37 * i + 5 * i * i) % (longest + 1) for i in range(B)]
+    ctx[B // 2] = longest
+    c = Case(31, torch.bfloat16, Hq, H, 64, 16, ctx, [1] * B)
+    c.check(c.call(start=False))
+    c.check(c.call(window=100, sinks=3), 100, 3)
+
+
 def test_long_context():
     c = Case(3, torch.bfloat16, 8, 1, 128, 16, [70001, 5], [1, 1])
     c.check(c.call(start=False))

@@ -358,10 +358,14 @@ struct ScaledAttentionParams : ExtendParams {
   int32_t workgroups;
 };
 constexpr int kScaledTile = 64;    // tokens
-constexpr int kScaledStart = 5;    // what an item's start costs, in tiles
-constexpr int kScaledLeast = 9;    // the least span of a workgroup, in tiles
+// What an item's start costs, in tiles (3, 5 and 8: four sequences of 4096 tokens 19.2, 17.7
+// and 17.5 us, 64 of 533 .. 4097 69.1, 71.4 and 71.4, 256 of 300 .. 1700 114, 113 and 112).
+constexpr int kScaledStart = 5;
+// The least span of a workgroup, in tiles (5, 7 and 9: one sequence of 500 tokens 11.5, 11.6
+// and 10.4 us, four of 4096 18.8, 18.9 and 17.6, one of 8190 16.5, 15.7 and 16.5).
+constexpr int kScaledLeast = 9;
 constexpr int kScaledWhole = 13;   // the longest item, its start with it, of sequences that get a crew each
-constexpr int kScaledWorkgroups = 512;
+constexpr int kScaledWorkgroups = 512;  // two a CU stay resident
 constexpr int kNoExponent = -300;  // below the exponent of every scale
 // Workgroups in all: behind those that attend, one for 256 sequences zeroes the rows of
 // sequences that have nothing to attend, and some the rows behind the last sequence.

@@ -31,9 +31,10 @@ constexpr int kScaledWaves = 4;  // per workgroup
 // A wavefront's sequence and its place in it: work items of the sequences lie end to
 // end, sequence s from start_loc[s] / bs + extra * s on (a sum that grows by at least
 // the blocks that n tokens touch: n / bs + 1 from a block's start on, + 2 from
-// anywhere).  The last s whose items begin at or before `item`, by 64 probes at a time.
-// The last round's probes hold the sequence's own numbers, its context (or null: none)
-// among them.
+// anywhere).  The last s whose items begin at or before `item`, by 64 probes at a time;
+// the last round's probes hold the sequence's own numbers, its context (or null: none)
+// among them.  Starts that decrease, which no call may have, can end at a sequence whose
+// items begin behind `item`: nth is negative there, and the kernels leave.
 struct Found {
   int seq, start, count, ctx, nth;
 };
@@ -252,7 +253,7 @@ __global__ __launch_bounds__(64 * kScaledWaves) void quantize_kernel(ScaledCache
   const int head = (int)((wave >> 1) % H);
   const int item = (int)((wave >> 1) / H);
   const Found f = find_item(p.start_loc, p.context_lens, p.num_seqs, p.num_tokens, SHIFT, 2, item);
-  if (f.seq >= p.num_seqs || f.count == 0) return;
+  if (f.seq >= p.num_seqs || f.count == 0 || f.nth < 0) return;
   const uint32_t ctx = (uint32_t)f.ctx;
   if (ctx == 0 || ctx > (uint64_t)p.max_blocks_per_seq * BS) return;
   // Token i of the sequence sits at position first + i; those before position 0 nowhere.
@@ -448,7 +449,7 @@ __global__ __launch_bounds__(64 * kScaledWaves) void dequantize_kernel(ScaledCac
   const int head = (int)((wave >> 1) % H);
   const int item = (int)((wave >> 1) / H);
   const Found f = find_item(p.start_loc, nullptr, p.num_seqs, p.num_tokens, SHIFT, 1, item);
-  if ((int64_t)f.nth * BS >= f.count) return;
+  if (f.nth < 0 || (int64_t)f.nth * BS >= f.count) return;
   const int n = min(f.count - f.nth * BS, BS);
   int32_t id = -1;
   if (f.seq < p.num_seqs && f.nth < p.max_blocks_per_seq) {

@@ -315,6 +315,33 @@ def test_no_tokens_and_no_sequences():
         assert out.shape == w.q.shape and (out == 0).all()
 
 
+def test_starts_that_decrease_reach_nothing_else():
+    """No call may have them; what they name is then unspecified, and nothing outside it is written."""
+    nb, n = 40, 400
+    guard = 1 << 16
+    sizes = [nb * H * D * BS] * 2
+    whole = [torch.full((size + 2 * guard,), 0x55, dtype=torch.uint8, device=DEV) for size in sizes]
+    kc = whole[0][guard:-guard].view(nb, H, D // 16, BS, 16)
+    vc = whole[1][guard:-guard].view(nb, H, D, BS)
+    scales = torch.ones((nb, H, 2), device=DEV)
+    table = torch.arange(5 * 6, device=DEV).int().view(5, 6)  # blocks 30 .. 39 stand in no table
+    k = torch.ones((n, H, D), device=DEV, dtype=torch.bfloat16)
+    q = torch.ones((n, Hq, D), device=DEV, dtype=torch.bfloat16)
+    lens = ints([90, 60, 80, 96, 33])
+    for starts in ([0, 300, 100, 250, 20, 200], [399, 350, 300, 200, 100, 0], [50, -7, 1000, 3, 2, 1]):
+        loc = ints(starts)
+        kernels.quantize_and_cache(k, k, kc, vc, scales, table, lens, loc)
+        ck, cv = kernels.dequantize_cache(kc, vc, scales, table, loc, n)
+        assert ck.shape == cv.shape == (n, H, D)
+        assert kernels.paged_attention_scaled(q, kc, vc, scales, table, lens, loc, H, SCALE, BS, 96, 300).shape == q.shape
+        assert kernels.prompt_attention(q, k, k, loc, SCALE, 300).shape == q.shape
+        assert kernels.prompt_attention(q, k, k, ints([0, 90, 150, 230, 326, 359]), SCALE, 96, loc, 300).shape == q.shape
+    torch.cuda.synchronize()
+    for t, cache in zip(whole, (kc, vc)):
+        assert (t[:guard] == 0x55).all() and (t[-guard:] == 0x55).all() and (cache[30:] == 0x55).all()
+    assert (scales[30:] == 1).all()
+
+
 def test_caches_past_32_bit_offsets():
     """Blocks whose bytes lie beyond 2^32, of caches and of scales' table rows."""
     nb, h, d = 300000, 8, 128  # 4.9 GB of K and of V

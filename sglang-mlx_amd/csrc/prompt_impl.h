@@ -17,7 +17,7 @@
 // Bound: the matrix units (64 % of the time) and the exponentials and sums beside them
 // (vector units 61 %).  8192 tokens, 32 heads over 8 of 128: 507 .. 540 us, 1020 .. 1080
 // TFLOP/s; the products alone took 297 us, with the weights 434, with all but the reads of
-// LDS 506.  128 rows a workgroup, two workgroups a CU, one tile ahead: 256 rows by eight
+// LDS 506.  128 rows a workgroup, two or three workgroups a CU, one tile ahead: 256 rows by eight
 // wavefronts took 555 us and left short prompts waiting (177 tokens 15 us instead of 11).
 #pragma once
 
@@ -27,6 +27,10 @@ namespace pkv {
 
 constexpr int kPromptTile = 64;
 constexpr int kPromptThreads = 256;
+// Wavefronts a SIMD.  Three at head size 64, with pieces of LDS two products ahead, take 119
+// us for 54 prompts of 365 .. 485 tokens and 347 for 8192 tokens (32 heads over 8); two, with
+// four ahead, 134 and 359.
+constexpr int prompt_waves(int D) { return D <= 64 ? 3 : D <= 128 ? 2 : 1; }
 
 // 16-byte chunk c of row r of an image with ROW chunks a row sits at chunk
 // c ^ prompt_swizzle(r).  Reads meet no bank twice: 16 rows at one chunk (K) and 4 rows of
@@ -73,7 +77,7 @@ __device__ __forceinline__ uint32_t seen32(int pos, int a, int window, int sinks
 }
 
 template <class QT, int D>
-__global__ __launch_bounds__(kPromptThreads, D <= 128 ? 2 : 1) void prompt_kernel(PromptParams p) {
+__global__ __launch_bounds__(kPromptThreads, prompt_waves(D)) void prompt_kernel(PromptParams p) {
   using QS = typename Elem<QT>::storage;
   constexpr int KSTEPS = (D + 15) / 16;  // score products per 32 tokens
   constexpr int DT = (D + 31) / 32;      // 32-dimension tiles of the output
@@ -120,6 +124,7 @@ __global__ __launch_bounds__(kPromptThreads, D <= 128 ? 2 : 1) void prompt_kerne
         // The last tile index of which more than `rank` tiles lie at it or behind it.
         const int rank = item - base;
         int lo = 0, hi = wave_max(tiles);  // (behind(lo) > rank >= behind(hi) = 0)
+        if (all == hi) lo = hi - 1 - rank, hi = lo + 1;  // (a single sequence's: 0.2 us sooner)
         while (hi - lo > 1) {
           const int mid = (lo + hi) / 2;
           if (wave_sum(max(tiles - mid, 0)) > rank) lo = mid;
@@ -330,14 +335,14 @@ __global__ __launch_bounds__(kPromptThreads, D <= 128 ? 2 : 1) void prompt_kerne
     return make_uint4(w[sub][4 * st], w[sub][4 * st + 1], w[sub][4 * st + 2], w[sub][4 * st + 3]);
   };
   // The products of a step: s = S^T of the tile in K's image kk (SCORES), then the outputs
-  // of the tile in V's image kv with the weights w (VALUES).  Pieces come from LDS four
-  // products ahead of their use; the fences keep them there (left to itself the compiler
-  // reads each right before its product and waits out LDS 32 times a tile: 870 instead of
-  // 1000 TFLOP/s for 8192 tokens with 32 heads of 128).
+  // of the tile in V's image kv with the weights w (VALUES).  Pieces come from LDS four (or
+  // two) products ahead of their use; the fences keep them there (left to itself the
+  // compiler reads each right before its product and waits out LDS 32 times a tile: 870
+  // instead of 1000 TFLOP/s for 8192 tokens with 32 heads of 128).
   auto run_products = [&](auto kk, auto kv, auto scores, auto values, f32x16 (&s)[2], const uint32_t (&w)[2][8])
                           __attribute__((always_inline)) {
     constexpr int NS = decltype(scores)::value ? 2 * KSTEPS : 0, NV = decltype(values)::value ? 4 * DT : 0;
-    constexpr int N = NS + NV, G = 4;
+    constexpr int N = NS + NV, G = prompt_waves(D) == 3 ? 2 : 4;
     auto piece = [&](int i) __attribute__((always_inline)) {
       return i < NS ? k_piece(kk, i % 2, i / 2)
                     : v_piece(kv, (i - NS) % DT, (i - NS) / DT / 2, (i - NS) / DT % 2);

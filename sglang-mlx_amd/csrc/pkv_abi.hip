@@ -1142,6 +1142,8 @@ int pkv_paged_attention_scaled(void* out, const void* query, const void* key_cac
   p.window = std::min(window, max_seq_len);  // (a longer one sees no more)
   p.sinks = std::min(num_sinks, max_seq_len);
   p.workgroups = (int32_t)cut.workgroups;
+  p.crews = p.workgroups / p.units;
+  p.unit_reciprocal = (uint32_t)std::min<int64_t>(ceil_div((int64_t)1 << 32, p.units), UINT32_MAX);
   std::lock_guard<std::mutex> together(launches_of(workspace));
   clear_pending_error();
   const hipStream_t s = static_cast<hipStream_t>(stream);

@@ -354,8 +354,9 @@ hipError_t launch_scaled_cache(const ScaledCacheParams& p, hipStream_t stream);
 // states: per workgroup two slots of 16 rows, (max, sum) in ws_ml, outputs in ws_o, and
 // one arrival counter.
 struct ScaledAttentionParams : ExtendParams {
-  const float* scales;   // [num_blocks, H, 2]: K's, V's
-  int32_t workgroups;
+  const float* scales;       // [num_blocks, H, 2]: K's, V's
+  int32_t workgroups, crews;
+  uint32_t unit_reciprocal;  // 2^32 / units, rounded up (units > 1)
 };
 constexpr int kScaledTile = 64;    // tokens
 // What an item's start costs, in tiles (3, 5 and 8: four sequences of 4096 tokens 19.2, 17.7

@@ -103,12 +103,13 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void scaled_attention_kernel
   const int run = (p.num_seqs + 255) / 256;
   int mine = 0;
   for (int s = tid * run; s < min((tid + 1) * run, p.num_seqs); ++s) mine += item_length(scaled_seq(p, s));
-  int sum = mine;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int a = __shfl_up(sum, d);
-    if (lane >= d) sum += a;
-  }
+  int sum = mine;  // of this lane and those before it: within 16 lanes, then by their last
+  sum += __builtin_amdgcn_update_dpp(0, sum, 0x111, 0xf, 0xf, false);  // row_shr:1
+  sum += __builtin_amdgcn_update_dpp(0, sum, 0x112, 0xf, 0xf, false);
+  sum += __builtin_amdgcn_update_dpp(0, sum, 0x114, 0xf, 0xf, false);
+  sum += __builtin_amdgcn_update_dpp(0, sum, 0x118, 0xf, 0xf, false);
+  sum += __builtin_amdgcn_update_dpp(0, sum, 0x142, 0xa, 0xf, false);  // row_bcast:15
+  sum += __builtin_amdgcn_update_dpp(0, sum, 0x143, 0xc, 0xf, false);  // row_bcast:31
   const bool any_long = __any(mine > kScaledWhole);
   if (lane == 63) s_sum[wave] = sum, s_long[wave] = any_long;
   __syncthreads();
@@ -120,12 +121,19 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void scaled_attention_kernel
     total += a;
     longer |= __builtin_amdgcn_readfirstlane(s_long[w]);
   }
-  const int crews = p.workgroups / p.units, crew = blockIdx.x / p.units, unit = blockIdx.x - crew * p.units;
+  // A wavefront pays for each instruction of a start in full: here the quotient comes by the
+  // divisor's reciprocal (exact for the up to kScaledWorkgroups workgroups of several crews).
+  // That, the sum over the lanes without trips through LDS and one division a row instead of
+  // one an output element took a call with one token from 8.4 to 6.9 us.
+  const int quotient = p.units == 1 ? blockIdx.x : __umulhi(blockIdx.x, p.unit_reciprocal);
+  const int crews = p.crews, crew = crews == 1 ? 0 : quotient;
+  const int unit = blockIdx.x - crew * p.units;
   // Where all are short and there are crews enough, each sequence is one crew's (cut and
   // joined by the span, four of 8 .. 50 tokens took 13.1 us instead of 8.6, sixty of 300 ..
   // 512 21.8 instead of 16.4).
   const bool apiece = longer == 0 && p.num_seqs <= crews;
-  const int span = max((total + crews - 1) / crews, kScaledLeast);
+  int span = kScaledLeast;
+  if (!apiece) span = max((total + crews - 1) / crews, kScaledLeast);
   if (apiece ? crew >= p.num_seqs : (int64_t)crew * span >= total) return;
   int x0 = crew * span, x1 = apiece ? 0 : min(span, total - x0) + x0;
   if (apiece) {
@@ -156,7 +164,9 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void scaled_attention_kernel
     ScaledSeq q;
     int seq, nr, v0, v1, w_first, parts;
   };
-  const int kvh = unit / p.slices, row0 = 16 * (unit - kvh * p.slices), h0 = kvh * group;
+  // (ONE: a sequence has one token's rows.)
+  auto token_of = [&](int row) __attribute__((always_inline)) { return ONE ? 0 : row / group; };
+  const int kvh = p.slices == 1 ? unit : unit / p.slices, row0 = 16 * (unit - kvh * p.slices), h0 = kvh * group;
   // The next sequence of this crew's span.
   int seq = __builtin_amdgcn_readfirstlane(s_first), base = __builtin_amdgcn_readfirstlane(s_base);
   auto next_piece = [&](Piece& c) __attribute__((always_inline)) -> bool {
@@ -182,9 +192,13 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void scaled_attention_kernel
       const int from = x0 <= begin ? begin : cut(x0), to = x1 >= end ? end : cut(x1);
       c.nr = min(16, q.q.count * group - row0);
       if (from >= to || c.nr <= 0) continue;
-      const int k0 = (begin + kScaledStart + snap + span - 1) / span, k1 = (end - snap) / span;
-      c.parts = apiece ? 1 : max(k1 - k0 + 1, 0) + 1;
-      c.w_first = c.parts > 1 ? k0 - 1 : crew;
+      c.parts = 1;
+      c.w_first = crew;
+      if (!apiece) {
+        const int k0 = (begin + kScaledStart + snap + span - 1) / span, k1 = (end - snap) / span;
+        c.parts = max(k1 - k0 + 1, 0) + 1;
+        if (c.parts > 1) c.w_first = k0 - 1;
+      }
       c.v0 = max(from - begin - kScaledStart, 0);
       c.v1 = to - begin - kScaledStart;
       c.q = q;
@@ -212,10 +226,10 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void scaled_attention_kernel
     q = c.q;
     v0 = c.v0, v1 = c.v1;
     const int first_pos = q.q.ctx - q.q.count;
-    pmin = first_pos + row0 / group, pmax = first_pos + (row0 + c.nr - 1) / group;
+    pmin = first_pos + token_of(row0), pmax = first_pos + token_of(row0 + c.nr - 1);
     // Row row0 + i, i < nr, is head (row0 + i) % group of token (row0 + i) / group; this
     // lane's is i = col.
-    const int my_row = row0 + min(col, c.nr - 1), token = my_row / group;
+    const int my_row = row0 + min(col, c.nr - 1), token = token_of(my_row);
     pos = first_pos + token;
     const QS* src =
         static_cast<const QS*>(p.q) + (q.q.start + token) * p.q_stride + (int64_t)(h0 + (my_row - token * group)) * D;
@@ -464,13 +478,12 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void scaled_attention_kernel
     const Piece& done = c;
     __syncthreads();
     auto row_of = [&](int i) {
-      const int tok = (row0 + i) / group;
+      const int tok = token_of(row0 + i);
       return ((int64_t)done.q.q.start + tok) * p.num_heads + h0 + (row0 + i - tok * group);
     };
-    // out = O 2^E / L (NaN stays NaN).
-    auto finish = [](float o, float l, float e) {
-      return l > 0.f ? __builtin_amdgcn_ldexpf(o / l, (int)e) : l == 0.f ? 0.f : l;
-    };
+    // out = O 2^E / L (NaN stays NaN, a row without tokens is zero).
+    auto inverse = [](float l) { return l > 0.f ? 1.f / l : l == 0.f ? 0.f : l; };
+    const float inv = inverse(L);
     // Wavefront w sums the 16-dimension tiles w, w + 4, ...
     const int nr = done.nr;
     const int64_t slot = (int64_t)blockIdx.x * 2 + (crew == done.w_first ? 1 : 0);
@@ -485,7 +498,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void scaled_attention_kernel
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int at = dt * 4 + r;
-        y[r] = finish(s_o[0][at][lane] + s_o[1][at][lane] + s_o[2][at][lane] + s_o[3][at][lane], L, E);
+        const float sum = s_o[0][at][lane] + s_o[1][at][lane] + s_o[2][at][lane] + s_o[3][at][lane];
+        y[r] = __builtin_amdgcn_ldexpf(sum * inv, (int)E);
       }
       if (done.parts == 1) {
         uint2 z;
@@ -548,9 +562,10 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void scaled_attention_kernel
               float* mine = &s_o[0][0][0] + i * 8;
               mine[0] = mm, mine[1] = ll, mine[2] = y[0], mine[3] = y[1], mine[4] = y[2], mine[5] = y[3];
             } else {
+              const float by = inverse(ll);
               uint2 z;
-              z.x = pack2(from_f32<QT>(finish(y[0], ll, 0.f)), from_f32<QT>(finish(y[1], ll, 0.f)));
-              z.y = pack2(from_f32<QT>(finish(y[2], ll, 0.f)), from_f32<QT>(finish(y[3], ll, 0.f)));
+              z.x = pack2(from_f32<QT>(y[0] * by), from_f32<QT>(y[1] * by));
+              z.y = pack2(from_f32<QT>(y[2] * by), from_f32<QT>(y[3] * by));
               *reinterpret_cast<uint2*>(static_cast<QS*>(p.out) + row_of(r) * D + d) = z;
             }
           }
@@ -568,9 +583,10 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void scaled_attention_kernel
 #pragma unroll
                 for (int j = 0; j < 4; ++j) y[j] += f * from[2 + j];
               }
+              const float by = inverse(ll);
               uint2 z;
-              z.x = pack2(from_f32<QT>(finish(y[0], ll, 0.f)), from_f32<QT>(finish(y[1], ll, 0.f)));
-              z.y = pack2(from_f32<QT>(finish(y[2], ll, 0.f)), from_f32<QT>(finish(y[3], ll, 0.f)));
+              z.x = pack2(from_f32<QT>(y[0] * by), from_f32<QT>(y[1] * by));
+              z.y = pack2(from_f32<QT>(y[2] * by), from_f32<QT>(y[3] * by));
               *reinterpret_cast<uint2*>(static_cast<QS*>(p.out) + row_of(r) * D + d) = z;
             }
           }

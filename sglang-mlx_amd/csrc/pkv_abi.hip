@@ -1237,6 +1237,8 @@ int pkv_prompt_attention(void* out, const void* query, const void* key, const vo
   p.num_heads = num_heads;
   p.num_kv_heads = num_kv_heads;
   p.group = group;
+  p.by_group = pkv::reciprocal(group);
+  p.by_kv_heads = pkv::reciprocal(num_kv_heads);
   p.window = std::min(window, kExtendMaxSeq);  // (a longer one sees no more)
   p.sinks = std::min(num_sinks, kExtendMaxSeq);
   p.splits = (int32_t)splits;

@@ -378,12 +378,29 @@ constexpr int64_t scaled_groups(int64_t workgroups, int64_t num_tokens, int64_t 
 template <class QT, int BS>
 hipError_t launch_scaled_attention(const ScaledAttentionParams& p, int head_size, hipStream_t stream);
 
+// n / d for n below 2^31 by a product: with 2^shift the least power of two that is at least
+// d, m = 2^(31 + shift) / d rounded up exceeds the quotient by under 2^-31, too little to
+// reach n's next multiple of d.
+struct Reciprocal {
+  uint32_t m;
+  int32_t shift;  // 0: d is 1
+  __device__ __forceinline__ int of(int n) const { return shift == 0 ? n : (int)(__umulhi((uint32_t)n, m) >> (shift - 1)); }
+};
+
+inline Reciprocal reciprocal(int64_t d) {
+  Reciprocal r = {0, 0};
+  while ((int64_t)1 << r.shift < d) ++r.shift;
+  if (r.shift > 0) r.m = (uint32_t)((((uint64_t)1 << (31 + r.shift)) + (uint64_t)d - 1) / (uint64_t)d);
+  return r;
+}
+
 // Attention of packed prompts over their keys and values as rows (prompt_impl.h; the
 // rules of pkv_prompt_attention): k_cache and v_cache are the first rows.
 struct PromptParams : ExtendParams {
   const int32_t* key_start_loc;  // [num_seqs + 1]
   int64_t k_stride, v_stride;    // of rows, in elements
   int32_t num_keys;
+  Reciprocal by_group, by_kv_heads;
 };
 template <class QT>
 hipError_t launch_prompt(const PromptParams& p, int head_size, hipStream_t stream);

@@ -103,9 +103,7 @@ __global__ __launch_bounds__(kPromptThreads, prompt_waves(D)) void prompt_kernel
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
-  const int kvh = blockIdx.x % p.num_kv_heads;
-  const int item = blockIdx.x / p.num_kv_heads;
-  const int items = gridDim.x / p.num_kv_heads;
+  const int item = p.by_kv_heads.of(blockIdx.x), kvh = blockIdx.x - item * p.num_kv_heads;
   const int split = blockIdx.y;
   const int group = p.group, h0 = kvh * group;
 
@@ -149,6 +147,7 @@ __global__ __launch_bounds__(kPromptThreads, prompt_waves(D)) void prompt_kernel
     const int tiles = s_seq[2];
     if (split != 0) return;
     const int last = min(max(p.query_start_loc[p.num_seqs], 0), p.num_tokens);
+    const int items = gridDim.x / p.num_kv_heads;
     const int share = (p.num_tokens - last + items - tiles - 1) / (items - tiles);
     const int64_t t0 = last + (int64_t)(item - tiles) * share;
     zero_tokens<QT, kPromptThreads>(p, D, t0, min(t0 + share, (int64_t)p.num_tokens), h0, group);
@@ -161,19 +160,19 @@ __global__ __launch_bounds__(kPromptThreads, prompt_waves(D)) void prompt_kernel
   const int row0 = z * kExtendRows;
   const int row_end = min(row0 + kExtendRows, rows);
   // Positions of the workgroup's rows; tokens before position 0 see nothing.
-  const int pmin = first_pos + row0 / group, pmax = first_pos + (row_end - 1) / group;
+  const int pmin = first_pos + p.by_group.of(row0), pmax = first_pos + p.by_group.of(row_end - 1);
 
   // This lane's row.
   const int wr0 = row0 + wave * 32, wr1 = min(wr0 + 32, rows);
   const int row = wr0 + col;
   const bool live = row < rows;
-  const int tok = live ? row / group : 0;
+  const int tok = live ? p.by_group.of(row) : 0;
   const int head = h0 + (live ? row - tok * group : 0);
   const int64_t qrow = q.start + tok;
   const int pos = live ? first_pos + tok : -1;
   // Positions of the wavefront's rows (uniform): none where w_min > w_max.
   const bool w_any = wr0 < wr1;
-  const int w_min = w_any ? first_pos + wr0 / group : 0, w_max = w_any ? first_pos + (wr1 - 1) / group : -1;
+  const int w_min = w_any ? first_pos + p.by_group.of(wr0) : 0, w_max = w_any ? first_pos + p.by_group.of(wr1 - 1) : -1;
 
   // The tiles to visit: those of the sinks, then those of the window.
   const int window = p.window > 0 ? p.window : 1 << 30;

@@ -15,7 +15,7 @@
 // receives element i of the rows 0 .. 3.
 //
 // Bound: the matrix units (64 % of the time) and the exponentials and sums beside them
-// (vector units 61 %).  8192 tokens, 32 heads over 8 of 128: 507 .. 540 us, 1020 .. 1080
+// (vector units 61 %).  8192 tokens, 32 heads over 8 of 128: 495 .. 540 us, 1020 .. 1110
 // TFLOP/s; the products alone took 297 us, with the weights 434, with all but the reads of
 // LDS 506.  128 rows a workgroup, up to three workgroups a CU, one tile ahead: 256 rows by eight
 // wavefronts took 555 us and left short prompts waiting (177 tokens 15 us instead of 11).

@@ -25,10 +25,10 @@
 // states in the workspace; the one that arrives last merges them in their order (no result
 // depends on timing, nobody waits for another workgroup).
 //
-// Bound: HBM reads, behind a start of 4.5 us (launch, lengths -> span -> blocks -> first
+// Bound: HBM reads, behind a start of 4 us (launch, lengths -> span -> blocks -> first
 // tile) and an end of 4 to 12 us (states in LDS, arrival, merge).  64 sequences of 533 ..
-// 4097 tokens, 8 KV heads of 128: 68 us, 4.5 TB/s; with the loads alone, nothing computed,
-// the same schedule took 66.
+// 4097 tokens, 8 KV heads of 128: 65 us, 4.7 TB/s (68 at the time when the same schedule with
+// the loads alone, nothing computed, took 66).
 #pragma once
 
 #include "extend_impl.h"

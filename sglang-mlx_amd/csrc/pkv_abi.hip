@@ -698,7 +698,7 @@ int scaled_cache_launch(const pkv::ScaledCacheParams& p, const char* where, void
 // How pkv_paged_attention_scaled is cut: crews of a workgroup for each unit, as many as
 // the most tiles that its sizes allow keep busy, and no more workgroups than stay resident.
 struct ScaledCut {
-  int64_t slices, tiles, workgroups;  // tiles: of all sequences, each with its start (a bound)
+  int64_t slices, tiles, crews, workgroups;  // tiles: of all sequences, each with its start (a bound)
 };
 ScaledCut scaled_cut(int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads, int64_t max_seq_len,
                      int64_t max_query_len, int64_t window, int64_t num_sinks) {
@@ -708,14 +708,17 @@ ScaledCut scaled_cut(int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads, 
   int64_t tiles = ceil_div(max_seq_len, T);
   if (window > 0) tiles = std::min(tiles, ceil_div(window + max_query_len, T) + ceil_div(num_sinks, T) + 2);
   const int64_t all = num_seqs * (tiles + pkv::kScaledStart);
-  const int64_t crews = std::min(pkv::kScaledWorkgroups / units, std::max(ceil_div(all, pkv::kScaledLeast), num_seqs));
-  return {slices, all, std::max<int64_t>(crews, 1) * units};
+  const int64_t crews = std::max<int64_t>(
+      std::min(pkv::kScaledWorkgroups / units, std::max(ceil_div(all, pkv::kScaledLeast), num_seqs)), 1);
+  return {slices, all, crews, crews * units};
 }
 struct ScaledWorkspace {
   size_t ml_bytes, total;
 };
+// (A single crew takes every sequence whole and leaves no states; more than one are at most
+// kScaledWorkgroups workgroups.)
 ScaledWorkspace scaled_workspace(const ScaledCut& cut, int64_t head_size) {
-  const size_t rows = (size_t)cut.workgroups * 2 * 16;
+  const size_t rows = cut.crews > 1 ? (size_t)cut.workgroups * 2 * 16 : 0;
   return {rows * 2 * sizeof(float),
           (size_t)pkv::kCounterBytes + rows * 2 * sizeof(float) + rows * head_size * sizeof(float)};
 }
@@ -1142,7 +1145,7 @@ int pkv_paged_attention_scaled(void* out, const void* query, const void* key_cac
   p.window = std::min(window, max_seq_len);  // (a longer one sees no more)
   p.sinks = std::min(num_sinks, max_seq_len);
   p.workgroups = (int32_t)cut.workgroups;
-  p.crews = p.workgroups / p.units;
+  p.crews = (int32_t)cut.crews;
   p.unit_reciprocal = (uint32_t)std::min<int64_t>(ceil_div((int64_t)1 << 32, p.units), UINT32_MAX);
   std::lock_guard<std::mutex> together(launches_of(workspace));
   clear_pending_error();

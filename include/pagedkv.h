@@ -658,7 +658,8 @@ size_t pkv_paged_attention_scaled_workspace_size(int32_t num_seqs,
  * FP8 caches, with K = decode(code) * scales[block][head][0] and V = decode(code)
  * * scales[block][head][1] in the place of k_scale and v_scale (scales as
  * pkv_quantize_and_cache writes them, or any others that are finite and not
- * negative).  Made for few rows: every 16 rows (query tokens * num_heads /
+ * negative, however far apart).  A token whose weight is below 2^-126 of its row's
+ * largest counts for nothing (float32's normal range).  Made for few rows: every 16 rows (query tokens * num_heads /
  * num_kv_heads) of a sequence read its keys once; for a prompt's many rows,
  * pkv_dequantize_cache and pkv_prompt_attention take less.
  * Cache bases and strides are 16-byte aligned.  num_seqs * (max_seq_len / 64 +

@@ -367,7 +367,12 @@ constexpr int kScaledStart = 5;
 constexpr int kScaledLeast = 9;
 constexpr int kScaledWhole = 13;   // the longest item, its start with it, of sequences that get a crew each
 constexpr int kScaledWorkgroups = 512;  // two a CU stay resident
-constexpr int kNoExponent = -300;  // below the exponent of every scale
+// log2 of a row's weights, relative to its largest: those below are zeros, as float32's normal
+// range has it.  The weights are summed 2^kSumShift times as large, so that they and the scales
+// by which they are multiplied stay in that range.
+constexpr float kLeastWeight = -126.f;
+constexpr int kSumShift = 12;
+constexpr float kNoExponent = -300.f;  // below the exponent of every such weight's product with its scale
 // Workgroups in all: behind those that attend, one for 256 sequences zeroes the rows of
 // sequences that have nothing to attend, and some the rows behind the last sequence.
 constexpr int64_t scaled_groups(int64_t workgroups, int64_t num_tokens, int64_t num_seqs, int64_t num_heads,

@@ -5,9 +5,11 @@
 //   out = sum_t w_t vs_b d_t / sum_t w_t,   w_t = exp(scale ks_b (q . c_t) - m).
 // The codes are exact in the queries' 16-bit type, so both products run on them as they
 // are; ks multiplies a score in float32, vs a weight before it is rounded to 16 bits.
-// There vs enters as vs / 2^e, e the largest exponent of a scale that the row has seen: the
-// weights keep the range that float16 has, whatever the scales' size, and the output
-// returns to true size at the end (2^e; powers of two, so that nothing is rounded).
+// There vs enters as vs / 2^e, 2^(m + e) being at least the largest product of exp(score)
+// and scale that the row has seen: the weights keep the range that float16 has, whatever the
+// scales' size (with e the largest exponent of a scale seen, a block of scale 2^16 and weight
+// 2^-60 cost blocks of scale 2^-16 a third of their value), and the output returns to true
+// size at the end (2^e; powers of two, so that nothing is rounded).
 //
 // Query rows, products and masks are those of extend_few_kernel (extend_impl.h): 16 rows
 // of a sequence and KV head, straight from the cache to the matrix units' registers,
@@ -220,8 +222,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void scaled_attention_kernel
   const float* scales;
   uint4 qf[2 * KL];
   f32x4 o[DT];
-  float m, l;
-  int e;
+  float m, l, e;
   auto begin_piece = [&]() __attribute__((always_inline)) {
     q = c.q;
     v0 = c.v0, v1 = c.v1;
@@ -342,9 +343,9 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void scaled_attention_kernel
       have = (b.v[0] >= 0 ? (NB == 1 ? 0xffffu : 0xffu) : 0u) | (NB == 2 && b.v[NB - 1] >= 0 ? 0xff00u : 0u);
     }
     const uint32_t sees = whole ? 0xffffu : have & seen16(pos, tv, window, sinks);
-    float ks[NB], mt = kNoScore;
+    float ks[NB], top[NB];
 #pragma unroll
-    for (int i = 0; i < NB; ++i) ks[i] = sx[i].x * p.scale_log2;
+    for (int i = 0; i < NB; ++i) ks[i] = sx[i].x * p.scale_log2, top[i] = kNoScore;
 #pragma unroll
     for (int u = 0; u < 4; ++u)
 #pragma unroll
@@ -357,32 +358,41 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void scaled_attention_kernel
 #pragma unroll
     for (int u = 0; u < 4; ++u)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) mt = fmaxf(mt, s[u][r]);
-    // (A block of zeros, or without tokens that the row sees, has no say.)
-    int ve = kNoExponent;
+      for (int r = 0; r < 4; ++r) top[NB == 2 ? u / 2 : 0] = fmaxf(top[NB == 2 ? u / 2 : 0], s[u][r]);
+    float mt = fmaxf(top[0], top[NB - 1]);
+    // log2 of the largest product of a weight, 2^(score - from), and its scale.  (A block of
+    // zeros has no say, nor one without weight: nothing that the row sees, or less than
+    // float32's normal range holds.)
+    auto weighs = [&](int i, float from) { return top[i] - from >= kLeastWeight; };
+    auto product = [&](float from) __attribute__((always_inline)) {
+      float x = kNoScore;
 #pragma unroll
-    for (int i = 0; i < NB; ++i)
-      if ((NB == 1 ? sees : sees & (0xffu << (8 * i))) != 0u && sx[i].y > 0.f)
-        ve = max(ve, __builtin_amdgcn_frexp_expf(sx[i].y));
-    if (__any(mt > m + kExtendSlack<QT> || ve > e || (m == kNoScore && mt != kNoScore))) {
-      mt = fmaxf(column_max(mt), m);
-      const int et = max(e, (int)column_max((float)ve));
-      const float alpha = __builtin_amdgcn_exp2f(m - (mt == kNoScore ? 0.f : mt));
-      const float alpha_o = __builtin_amdgcn_ldexpf(alpha, max(e - et, -200));
-      m = mt;
-      e = et;
+      for (int i = 0; i < NB; ++i)
+        if (weighs(i, from) && sx[i].y > 0.f)
+          x = fmaxf(x, top[i] - from + (float)__builtin_amdgcn_frexp_expf(sx[i].y));
+      return x;
+    };
+    if (__any(mt > m + kExtendSlack<QT> || product(m) > e + kExtendSlack<QT> || (m == kNoScore && mt != kNoScore))) {
+      // m moves by whole steps, e against them: m + e stays where no product passes it.
+      mt = column_max(mt);
+      const float up = mt > m ? __builtin_ceilf(mt - m) : 0.f;
+      const float next = m == kNoScore ? mt : m + up;
+      const float e1 = fmaxf(fmaxf(e - up, __builtin_ceilf(column_max(product(next)))), kNoExponent);
+      const float by = m - (next == kNoScore ? 0.f : next);
+      const float alpha = __builtin_amdgcn_exp2f(by), alpha_o = __builtin_amdgcn_exp2f(by + (e - e1));
+      m = next;
+      e = e1;
       l *= alpha;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int r = 0; r < 4; ++r) o[dt][r] *= alpha_o;
     }
-    const float from = (m == kNoScore ? 0.f : m) - weight_shift<QT>(kExtendSlack<QT> + 1.f);
+    const float from = (m == kNoScore ? 0.f : m) - (weight_shift<QT>(kExtendSlack<QT>) + kSumShift);
     float vs[NB];
 #pragma unroll
     for (int i = 0; i < NB; ++i)
-      vs[i] = (NB == 1 ? sees : sees & (0xffu << (8 * i))) != 0u
-                  ? __builtin_amdgcn_ldexpf(sx[i].y, -max(e, kNoExponent + 1)) : 0.f;
+      vs[i] = weighs(i, m) ? __builtin_amdgcn_ldexpf(sx[i].y, -(int)e - kSumShift) : 0.f;
     uint4 wf[2];
     {
       uint32_t w[8];
@@ -459,17 +469,21 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void scaled_attention_kernel
     }
 
     // The wavefronts' states: column col is row row0 + col.
-    l = column_sum(l);
-    if (g == 0) s_m[wave][col] = m, s_l[wave][col] = l, s_e[wave][col] = (float)e;
+    l = column_sum(l) * (1.f / (1 << kSumShift));
+    if (g == 0) s_m[wave][col] = m, s_l[wave][col] = l, s_e[wave][col] = e;
     __syncthreads();
-    float M = kNoScore, L = 0.f, E = (float)kNoExponent;
+    float M = kNoScore, L = 0.f, E = kNoExponent;
 #pragma unroll
-    for (int w = 0; w < NW; ++w) M = fmaxf(M, s_m[w][col]), E = fmaxf(E, s_e[w][col]);
+    for (int w = 0; w < NW; ++w) M = fmaxf(M, s_m[w][col]);
     {
       const float ref = M == kNoScore ? 0.f : M;
 #pragma unroll
-      for (int w = 0; w < NW; ++w) L += s_l[w][col] * __builtin_amdgcn_exp2f(s_m[w][col] - ref);
-      const float f = __builtin_amdgcn_exp2f(m - ref) * __builtin_amdgcn_exp2f(fmaxf((float)e - E, -126.f));
+      for (int w = 0; w < NW; ++w) {
+        const float by = s_m[w][col] - ref;
+        L += s_l[w][col] * __builtin_amdgcn_exp2f(by);
+        E = fmaxf(E, __builtin_ceilf(by + s_e[w][col]));
+      }
+      const float f = __builtin_amdgcn_exp2f(m - ref + (e - E));
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll

@@ -1146,7 +1146,7 @@ int pkv_paged_attention_scaled(void* out, const void* query, const void* key_cac
   p.sinks = std::min(num_sinks, max_seq_len);
   p.workgroups = (int32_t)cut.workgroups;
   p.crews = (int32_t)cut.crews;
-  p.unit_reciprocal = (uint32_t)std::min<int64_t>(ceil_div((int64_t)1 << 32, p.units), UINT32_MAX);
+  p.unit_reciprocal = pkv::unit_reciprocal(p.units);
   std::lock_guard<std::mutex> together(launches_of(workspace));
   clear_pending_error();
   const hipStream_t s = static_cast<hipStream_t>(stream);

@@ -9,6 +9,8 @@
 #include <atomic>
 #include <type_traits>
 
+#include "pkv_schedule.h"
+
 namespace pkv {
 
 enum { kF32 = 0, kF16 = 1, kBF16 = 2, kFP8 = 3 };
@@ -358,15 +360,6 @@ struct ScaledAttentionParams : ExtendParams {
   int32_t workgroups, crews;
   uint32_t unit_reciprocal;  // 2^32 / units, rounded up (units > 1)
 };
-constexpr int kScaledTile = 64;    // tokens
-// What an item's start costs, in tiles (3, 5 and 8: four sequences of 4096 tokens 19.2, 17.7
-// and 17.5 us, 64 of 533 .. 4097 69.1, 71.4 and 71.4, 256 of 300 .. 1700 114, 113 and 112).
-constexpr int kScaledStart = 5;
-// The least span of a workgroup, in tiles (5, 7 and 9: one sequence of 500 tokens 11.5, 11.6
-// and 10.4 us, four of 4096 18.8, 18.9 and 17.6, one of 8190 16.5, 15.7 and 16.5).
-constexpr int kScaledLeast = 9;
-constexpr int kScaledWhole = 13;   // the longest item, its start with it, of sequences that get a crew each
-constexpr int kScaledWorkgroups = 512;  // two a CU stay resident
 // log2 of a row's weights, relative to its largest: those below are zeros, as float32's normal
 // range has it.  The weights are summed 2^kSumShift times as large, so that they and the scales
 // by which they are multiplied stay in that range.
@@ -382,22 +375,6 @@ constexpr int64_t scaled_groups(int64_t workgroups, int64_t num_tokens, int64_t 
 // (one block size a file, scaled_attention_<q>_<block size>.hip)
 template <class QT, int BS>
 hipError_t launch_scaled_attention(const ScaledAttentionParams& p, int head_size, hipStream_t stream);
-
-// n / d for n below 2^31 by a product: with 2^shift the least power of two that is at least
-// d, m = 2^(31 + shift) / d rounded up exceeds the quotient by under 2^-31, too little to
-// reach n's next multiple of d.
-struct Reciprocal {
-  uint32_t m;
-  int32_t shift;  // 0: d is 1
-  __device__ __forceinline__ int of(int n) const { return shift == 0 ? n : (int)(__umulhi((uint32_t)n, m) >> (shift - 1)); }
-};
-
-inline Reciprocal reciprocal(int64_t d) {
-  Reciprocal r = {0, 0};
-  while ((int64_t)1 << r.shift < d) ++r.shift;
-  if (r.shift > 0) r.m = (uint32_t)((((uint64_t)1 << (31 + r.shift)) + (uint64_t)d - 1) / (uint64_t)d);
-  return r;
-}
 
 // Attention of packed prompts over their keys and values as rows (prompt_impl.h; the
 // rules of pkv_prompt_attention): k_cache and v_cache are the first rows.

@@ -127,8 +127,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void scaled_attention_kernel
   // divisor's reciprocal (exact for the up to kScaledWorkgroups workgroups of several crews).
   // That, the sum over the lanes without trips through LDS and one division a row instead of
   // one an output element took a call with one token from 8.4 to 6.9 us.
-  const int quotient = p.units == 1 ? blockIdx.x : __umulhi(blockIdx.x, p.unit_reciprocal);
-  const int crews = p.crews, crew = crews == 1 ? 0 : quotient;
+  const int crews = p.crews, crew = crew_of(blockIdx.x, p.units, crews, p.unit_reciprocal);
   const int unit = blockIdx.x - crew * p.units;
   // Where all are short and there are crews enough, each sequence is one crew's (cut and
   // joined by the span, four of 8 .. 50 tokens took 13.1 us instead of 8.6, sixty of 300 ..
@@ -158,7 +157,6 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void scaled_attention_kernel
 
   const int window = p.window > 0 ? p.window : p.max_seq_len;
   const int sinks = p.window > 0 ? p.sinks : 0;
-  const int snap = min(4, span / 4);
 
   // A piece: tiles [v0, v1) of a sequence, one of `parts` pieces, the first by crew
   // w_first.  Everything here is the same for all threads.
@@ -186,23 +184,13 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void scaled_attention_kernel
       c.seq = seq;
       base = end;
       ++seq;
-      // A cut near a sequence's begin or end moves there: a piece costs about kScaledStart
-      // tiles, wherever it is.
-      auto cut = [&](int x) {
-        return x <= begin || x - begin < kScaledStart + snap ? begin : x >= end || end - x < snap ? end : x;
-      };
-      const int from = x0 <= begin ? begin : cut(x0), to = x1 >= end ? end : cut(x1);
+      const ScaledPiece piece = scaled_piece(begin, end, x0, x1, span, crew, apiece);
       c.nr = min(16, q.q.count * group - row0);
-      if (from >= to || c.nr <= 0) continue;
-      c.parts = 1;
-      c.w_first = crew;
-      if (!apiece) {
-        const int k0 = (begin + kScaledStart + snap + span - 1) / span, k1 = (end - snap) / span;
-        c.parts = max(k1 - k0 + 1, 0) + 1;
-        if (c.parts > 1) c.w_first = k0 - 1;
-      }
-      c.v0 = max(from - begin - kScaledStart, 0);
-      c.v1 = to - begin - kScaledStart;
+      if (piece.from >= piece.to || c.nr <= 0) continue;
+      c.parts = piece.parts;
+      c.w_first = piece.first;
+      c.v0 = max(piece.from - begin - kScaledStart, 0);
+      c.v1 = piece.to - begin - kScaledStart;
       c.q = q;
       return true;
     }

@@ -210,6 +210,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void scaled_attention_kernel
   const float* scales;
   uint4 qf[2 * KL];
   f32x4 o[DT];
+  // m: log2 of the weights' reference point; m + e: of the largest product of a weight and its
+  // scale, whose reference point is 2^(m + ceil(e)).
   float m, l, e;
   auto begin_piece = [&]() __attribute__((always_inline)) {
     q = c.q;
@@ -361,15 +363,14 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void scaled_attention_kernel
       return x;
     };
     if (__any(mt > m + kExtendSlack<QT> || product(m) > e + kExtendSlack<QT> || (m == kNoScore && mt != kNoScore))) {
-      // m moves by whole steps, e against them: m + e stays where no product passes it.
-      mt = column_max(mt);
-      const float up = mt > m ? __builtin_ceilf(mt - m) : 0.f;
-      const float next = m == kNoScore ? mt : m + up;
-      const float e1 = fmaxf(fmaxf(e - up, __builtin_ceilf(column_max(product(next)))), kNoExponent);
-      const float by = m - (next == kNoScore ? 0.f : next);
-      const float alpha = __builtin_amdgcn_exp2f(by), alpha_o = __builtin_amdgcn_exp2f(by + (e - e1));
-      m = next;
-      e = e1;
+      // (m is the largest score itself: a row's heaviest weight is then a power of two, and
+      // nothing of it is lost when it is rounded.  With m moved by whole steps errors against
+      // 64 bits were 0.0024 instead of 0.0017.)
+      mt = fmaxf(column_max(mt), m);
+      const float by = m - (mt == kNoScore ? 0.f : mt), was = __builtin_ceilf(e);
+      e = fmaxf(fmaxf(e - (mt - m), column_max(product(mt))), kNoExponent);
+      m = mt;
+      const float alpha = __builtin_amdgcn_exp2f(by), alpha_o = __builtin_amdgcn_exp2f(by + (was - __builtin_ceilf(e)));
       l *= alpha;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
@@ -380,7 +381,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void scaled_attention_kernel
     float vs[NB];
 #pragma unroll
     for (int i = 0; i < NB; ++i)
-      vs[i] = weighs(i, m) ? __builtin_amdgcn_ldexpf(sx[i].y, -(int)e - kSumShift) : 0.f;
+      vs[i] = weighs(i, m) ? __builtin_amdgcn_ldexpf(sx[i].y, -(int)__builtin_ceilf(e) - kSumShift) : 0.f;
     uint4 wf[2];
     {
       uint32_t w[8];
@@ -458,6 +459,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void scaled_attention_kernel
 
     // The wavefronts' states: column col is row row0 + col.
     l = column_sum(l) * (1.f / (1 << kSumShift));
+    e = __builtin_ceilf(e);
     if (g == 0) s_m[wave][col] = m, s_l[wave][col] = l, s_e[wave][col] = e;
     __syncthreads();
     float M = kNoScore, L = 0.f, E = kNoExponent;

@@ -26,10 +26,10 @@ def attend(q, k, codes, vs, first, scale):
     most 2^-34 of the largest one, times its code.  An output below the type's normal range is a multiple of its
     smallest subnormal.
 
-    Weights are float32 numbers relative to 2^m, and those below its normal range are zeros.  m moves to less than one
-    above the largest score so far (log2), never further: what is left out has s - m < -126, so s - max < -125.  Pieces
-    of a row meet by factors 2^(m - M), M one of these m, which are zeros below 2^-126 too: m >= max of the piece there,
-    so that its tokens have s - max < -125 again.  The whole of such tokens' share is allowed for."""
+    Weights are float32 numbers relative to 2^m, m one of the row's scores (log2), and those below its normal range
+    are zeros: s - m < -126, so that s is more than 126 below the largest.  Pieces of a row meet by factors 2^(m - M),
+    which are zeros below 2^-126 too.  The whole of such tokens' share is allowed for (a score's own error, (D + 8)
+    2^-24 of the sum of the sizes, is below 0.001 here)."""
     n, Hq, D = q.shape
     T, H = codes.shape[:2]
     u = torch.finfo(q.dtype).eps / 2
@@ -45,7 +45,7 @@ def attend(q, k, codes, vs, first, scale):
         p = (p - p.amax(1, keepdim=True)).exp()
         p = p / p.sum(1, keepdim=True)
         w = p * vs[:, g]
-        gone = torch.where(p < 2.0 ** -125 * p.amax(1, keepdim=True), w, 0.0)
+        gone = torch.where(p < 1.001 * 2.0 ** -126 * p.amax(1, keepdim=True), w, 0.0)
         # (Scores' errors of the tokens that weigh: exp(error) of the others has no say.)
         size = (qh.abs() @ kh.abs().t().contiguous()) * abs(scale)
         e32 = 2 * (D + 8) * 2.0 ** -24 * torch.where(sees, size, 0.0).amax(1, keepdim=True) + 2.0 ** -20

@@ -623,12 +623,12 @@ int pkv_quantize_and_cache(const void* key, const void* value, void* key_cache,
 
 /*
  * The way back: tokens 0, 1, ... of sequence s into rows [start_loc[s],
- * start_loc[s + 1]) of key_out and value_out, code * scale rounded once to dtype
- * (F32, F16 or BF16).  Rows without a block (its id outside [0, num_blocks), past
- * max_num_blocks_per_seq * block_size tokens) and rows behind the last sequence
- * are zero; start_loc[0] is 0.  key_out, value_out: [num_tokens, num_kv_heads,
- * head_size], contiguous, 16-byte aligned.  The others as for
- * pkv_quantize_and_cache.  One launch.
+ * start_loc[s + 1]) of key_out and value_out, code * scale in float32 (exact with the
+ * scales that pkv_quantize_and_cache sets), rounded to dtype (F32, F16 or BF16).
+ * Rows without a block (its id outside [0, num_blocks), past max_num_blocks_per_seq *
+ * block_size tokens) and rows behind the last sequence are zero; start_loc begins at 0
+ * and does not decrease.  key_out, value_out: [num_tokens, num_kv_heads, head_size],
+ * contiguous, 16-byte aligned.  The others as for pkv_quantize_and_cache.  One launch.
  */
 int pkv_dequantize_cache(void* key_out, void* value_out, const void* key_cache,
                          const void* value_cache, const float* scales,
@@ -641,7 +641,8 @@ int pkv_dequantize_cache(void* key_out, void* value_out, const void* key_cache,
 /*
  * Workspace bytes that pkv_paged_attention_scaled needs: PKV_COUNTER_BYTES of
  * arrival counters (as pkv_paged_attention's, with which a workspace may be
- * shared), then the states of items' pieces.  0 for invalid sizes.
+ * shared), then the states of items' pieces (at most 512 workgroups', none where a
+ * sequence has more than 256 row groups).  0 for invalid sizes.
  */
 size_t pkv_paged_attention_scaled_workspace_size(int32_t num_seqs,
                                                  int32_t num_heads,
@@ -659,11 +660,14 @@ size_t pkv_paged_attention_scaled_workspace_size(int32_t num_seqs,
  * * scales[block][head][1] in the place of k_scale and v_scale (scales as
  * pkv_quantize_and_cache writes them, or any others that are finite and not
  * negative, however far apart).  A token whose weight is below 2^-126 of its row's
- * largest counts for nothing (float32's normal range).  Made for few rows: every 16 rows (query tokens * num_heads /
- * num_kv_heads) of a sequence read its keys once; for a prompt's many rows,
- * pkv_dequantize_cache and pkv_prompt_attention take less.
- * Cache bases and strides are 16-byte aligned.  num_seqs * (max_seq_len / 64 +
- * 5) stays below 2^31, max_query_len * num_heads below 2^28.  One launch.
+ * largest counts for nothing (float32's normal range).  Made for few rows: every 16
+ * rows (query tokens * num_heads / num_kv_heads) of a sequence read its keys once;
+ * for a prompt's many rows, pkv_dequantize_cache and pkv_prompt_attention take less.
+ * Cache bases and strides are 16-byte aligned.  num_seqs * (max_seq_len / 64,
+ * rounded up, + 5) stays below 2^31 - 4608 (with a window the tiles that it and the
+ * sinks can touch count, if fewer), num_tokens * num_heads below 2^30, the row
+ * groups of a sequence (num_kv_heads * (max_query_len * num_heads / num_kv_heads / 16,
+ * rounded up)) below 2^24.  One launch.
  */
 int pkv_paged_attention_scaled(
     void* out, const void* query, const void* key_cache, const void* value_cache,
@@ -702,14 +706,14 @@ size_t pkv_prompt_attention_workspace_size(int32_t num_tokens, int32_t num_seqs,
  *   out = sum_t softmax_t(scale * q . k_t) v_t,
  * GQA as in pkv_paged_attention.  Rows that see no key and rows behind the last
  * sequence are zero.  What a row does not see does not reach it, inf and NaN
- * included.
+ * included.  Both starts begin at 0 and do not decrease.
  * query [num_tokens, num_heads, head_size], key, value [num_keys, num_kv_heads,
  * head_size], all of type dtype (BF16 or F16), row strides q_stride, k_stride and
  * v_stride, the inner two dimensions contiguous, rows 16-byte aligned.  out:
  * contiguous, 16-byte aligned.  k_stride and v_stride are at most 2^24, num_tokens *
  * num_heads is below 2^30, num_keys at most 2^30.  key_start_loc may be NULL:
- * query_start_loc (with num_keys = num_tokens).  max_query_len, max_key_len: the most rows of a
- * sequence; they choose how the work is cut, not the result.
+ * query_start_loc (with num_keys = num_tokens).  max_query_len, max_key_len: the most
+ * rows of a sequence; they choose how the work is cut, not the result.
  * head_size in {32,64,80,96,112,120,128,192,256}.  One launch, or two where few
  * rows meet many keys.
  */

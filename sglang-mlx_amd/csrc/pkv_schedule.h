@@ -33,7 +33,7 @@ constexpr int kScaledStart = 5;
 // and 10.4 us, four of 4096 18.8, 18.9 and 17.6, one of 8190 16.5, 15.7 and 16.5).
 constexpr int kScaledLeast = 9;
 constexpr int kScaledWhole = 13;   // the longest item, its start with it, of sequences that get a crew each
-constexpr int kScaledWorkgroups = 512;  // two a CU stay resident
+constexpr int kScaledWorkgroups = 512;  // two a CU stay resident (one above head size 128)
 
 // Crew of a workgroup, of crews of `units` workgroups each: by 2^32 / units rounded up (units
 // of one crew alone are never taken apart, nor is a crew of one).

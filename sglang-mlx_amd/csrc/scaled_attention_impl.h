@@ -27,10 +27,15 @@
 // states in the workspace; the one that arrives last merges them in their order (no result
 // depends on timing, nobody waits for another workgroup).
 //
-// Bound: HBM reads, behind a start of 4 us (launch, lengths -> span -> blocks -> first
-// tile) and an end of 4 to 12 us (states in LDS, arrival, merge).  64 sequences of 533 ..
-// 4097 tokens, 8 KV heads of 128: 65 us, 4.7 TB/s (68 at the time when the same schedule with
-// the loads alone, nothing computed, took 66).
+// Bound: this kernel's reads, behind a start and an end.  64 sequences of 533 .. 4097 tokens,
+// 8 KV heads of 128: 65 .. 67 us, 4.5 .. 4.7 TB/s (68 at the time when the same schedule with
+// the loads alone, nothing computed, took 66).  That is these loads' rate, not the card's: a K
+// load touches 16 places of 64 bytes, at the default cache policy, where the decode kernel of
+// caches with one scale reads runs of 1 KiB, non-temporal, and as many bytes in 52 us.  In a
+// graph a call with one token takes 6.1 us (launch, lengths -> span -> blocks -> first tile,
+// states in LDS, output), one sequence of 512, a piece, 8.0, one of 1024, several, 11.0: the
+// arrival and the merge cost 3 us.  Beyond 16 rows of a KV head its codes are read again for
+// each 16 (28 heads over 4, five drafted tokens: 138 MB for 45).
 #pragma once
 
 #include "extend_impl.h"

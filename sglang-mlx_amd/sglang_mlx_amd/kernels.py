@@ -366,8 +366,9 @@ def dequantize_cache(
         The others as ``quantize_and_cache``.
 
     Returns:
-        key, value [num_tokens, num_kv_heads, head_size]: code * scale, rounded
-        once.  Rows without a block, and those behind the last sequence, are zero.
+        key, value [num_tokens, num_kv_heads, head_size]: code * scale in float32
+        (exact with the scales that ``quantize_and_cache`` sets), rounded to dtype.
+        Rows without a block, and those behind the last sequence, are zero.
     """
     return _ext.dequantize_cache(key_cache, value_cache, kv_scales, block_tables, start_loc, num_tokens, dtype)
 
@@ -393,7 +394,7 @@ def paged_attention_scaled(
     drafted ones.
 
     bfloat16 or float16 queries; kv_scales may hold any finite scales that are not
-    negative.  The other arguments, the result and the rows that are zero are
+    negative, however far apart.  The other arguments, the result and the rows that are zero are
     ``paged_attention_extend``'s.  Every 16 query rows (tokens * num_heads /
     num_kv_heads) of a sequence read its keys once, so this is for few of them: a
     prompt's chunk takes less time through ``dequantize_cache`` and
@@ -424,12 +425,12 @@ def prompt_attention(
         query: [num_tokens, num_heads, head_size], the sequences end to end;
             bfloat16 or float16; rows may be views of a projection
         key, value: [num_keys, num_kv_heads, head_size], of the same type
-        query_start_loc: [num_seqs + 1], each sequence's first query row, and the
-            number of rows; output rows behind it are zero
+        query_start_loc: [num_seqs + 1], from 0, each sequence's first query row, and
+            the number of rows; output rows behind it are zero
         scale: softmax scale
         max_query_len: the most query rows of a sequence
-        key_start_loc: [num_seqs + 1], each sequence's first key row, and the number
-            of them: the n query rows of a sequence are its last n tokens.  None: the
+        key_start_loc: [num_seqs + 1], from 0, each sequence's first key row, and the
+            number of them: the n query rows of a sequence are its last n tokens.  None: the
             keys are those of the queries
         max_key_len: the most key rows of a sequence (with key_start_loc)
         window, num_sinks: with a window > 0 a query sees the ``window`` last
